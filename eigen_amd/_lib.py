@@ -11,7 +11,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libeigen_amd_blas.so")
 
-F32, F64, C32, C64 = 0, 1, 2, 3
+F32, F64, C32, C64, BF16, F16 = 0, 1, 2, 3, 4, 5
 OP_N, OP_T, OP_C, OP_CONJ = 0, 1, 2, 3
 OK, ERR_ARG, ERR_DEVICE, ERR_NO_GPU, ERR_NOT_RESIDENT = 0, -1, -2, -3, -4
 
@@ -120,6 +120,22 @@ lib.eigamd_trsm_host.restype = ctypes.c_int
 lib.eigamd_trsm_host.argtypes = [ctypes.c_int] * 5 + [_i64, _i64, _vp, _vp, _i64, _vp, _i64]
 lib.eigamd_trsm_dev.restype = ctypes.c_int
 lib.eigamd_trsm_dev.argtypes = [ctypes.c_int] * 5 + [_i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp]
+_int = ctypes.c_int
+for _name, _res, _args in (
+        ("lora_plan_ints", _i64, [_i64] * 2),
+        ("lora_plan_dev", _int, [_i64] * 2 + [_vp] * 3),
+        ("lora_work_bytes", _i64, [_int] * 2 + [_i64] * 3),
+        ("lora_dev", _int, [_int] * 4 + [_i64] * 5 + [_vp, _i64, _vp, _i64] + [_vp, _i64, _i64] * 2 + [_vp, _vp, _vp, _i64, _vp, _i64,
+                                                                                               _vp, _i64, _vp]),
+        ("lora_wgrad_work_bytes", _i64, [_i64] * 4),
+        ("lora_wgrad_dev", _int, [_int] * 2 + [_i64] * 4 + [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp]),
+        ("ckpt8_pack_dev", _int, [_int] + [_i64] * 2 + [_vp, _i64] * 3 + [_vp]),
+        ("ckpt8_unpack_dev", _int, [_int] + [_i64] * 2 + [_vp, _i64] * 3 + [_vp]),
+        ("ckpt8_wgrad_work_bytes", _i64, [_int] + [_i64] * 3),
+        ("ckpt8_wgrad_dev", _int, [_int] * 2 + [_i64] * 3 + [_vp, _i64] * 3 + [_vp, _vp, _i64, _vp, _i64, _vp])):
+    _f = getattr(lib, "eigamd_" + _name)
+    _f.restype = _res
+    _f.argtypes = _args
 _i64p = ctypes.POINTER(ctypes.c_int64)
 lib.eigamd_ipc_export.restype = ctypes.c_int
 lib.eigamd_ipc_export.argtypes = [_vp, _vp, _i64p, _i64p]

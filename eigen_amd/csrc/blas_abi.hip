@@ -671,6 +671,7 @@ int op_of(char ch) {  // blas/common.h:47-50
 
 namespace eigamd {
 int abi_fail(int code, const std::string& what) { return fail(code, what); }  // for the other translation units of the ABI
+int abi_ensure_device() { return ensure_device(); }
 
 // rows x cols elements between a caller's (pageable) matrix and memory of the current device, through
 // this device's pinned chunks and copy threads; returns when the data has arrived (with wait = false: once it is

@@ -1,0 +1,231 @@
+// Activations held in 8 bits for the backward pass, and the weight gradient that reads them.
+//
+// 32 consecutive features of a token share a power-of-two scale 2^e, e the smallest with max|x| <= 127 2^e: q = round(x / 2^e)
+// to whole numbers, ties to even.  A power of two costs up to one of the eight bits against a free scale and makes the rest
+// exact: the division, and q 2^e as a bf16, f16 or float (7 bits of significand), so a product with the checkpoint rounds
+// nothing that a product with the unpacked matrix would not.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "gemm_launch.hpp"
+#include "half_gemm.hpp"
+#include "lowrank.hpp"
+
+namespace eigamd {
+
+namespace {
+
+// Limits of a type: smallest exponent of a scale (f16: its subnormals are whole multiples of 2^-24), and the exponent of its
+// largest values, above which 127 2^e would leave the type and q stops at 63.
+template <typename T> struct Range { static constexpr int low = -126, top = 127; };
+template <> struct Range<F16> { static constexpr int low = -24, top = 15; };
+
+struct PackArgs {
+  int k, chunks;          // features; chunks of 8 features a token takes (whole blocks of 32)
+  int64_t total;          // chunks in all
+  const void* x; int64_t ldx;
+  int8_t* q; int64_t ldq;
+  uint8_t* e; int64_t lde;
+  void* out;
+};
+
+__device__ __forceinline__ bool chunk_of(const PackArgs& g, int64_t& token, int& c) {
+  const int64_t first = (int64_t)blockIdx.x * 256;         // one 64-bit division per workgroup
+  const int64_t t0 = first / g.chunks;
+  const unsigned in = (unsigned)(first - t0 * g.chunks) + threadIdx.x;
+  token = t0 + in / (unsigned)g.chunks;
+  c = (int)(in % (unsigned)g.chunks);
+  return first + threadIdx.x < g.total;
+}
+
+// A thread takes 8 features, four neighbours a block (`chunks` is a multiple of 4, so a block never leaves its wave).
+template <typename T> __global__ __launch_bounds__(256) void ckpt8_pack_kernel(PackArgs g) {
+  using E = typename T::elem;
+  using x8 = typename T::x8;
+  int64_t token;
+  int c;
+  const bool on = chunk_of(g, token, c);
+  const int n = on ? g.k - c * 8 : 0;
+  const x8 v = load_up_to_8<E, x8>(static_cast<const E*>(g.x) + token * g.ldx + c * 8, n);
+  float top = 0.0f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = __builtin_fabsf((float)v[i]);
+    bad |= !(a < __builtin_inff());
+    top = fmaxf(top, a);
+  }
+  top = fmaxf(top, __shfl_xor(top, 1));
+  top = fmaxf(top, __shfl_xor(top, 2));
+  int flag = bad;
+  flag |= __shfl_xor(flag, 1);
+  flag |= __shfl_xor(flag, 2);
+  if (!on) return;
+  const int bits = __float_as_int(top);
+  int e = (bits >> 23) - 127 - ((bits & 0x7fffff) > 0x7e0000 ? 5 : 6);     // 127 = 1.984375 * 2^6
+  e = e < Range<T>::low ? Range<T>::low : e;
+  const float most = e > Range<T>::top - 6 ? 63.0f : 127.0f, inverse = __int_as_float((127 - e) << 23);
+  uint64_t q = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float r = rintf((float)v[i] * inverse);
+    r = fminf(fmaxf(r, -most), most);
+    q |= (uint64_t)(uint8_t)(int8_t)(int)(flag ? 0.0f : r) << (8 * i);
+  }
+  int8_t* to = g.q + token * g.ldq + c * 8;
+  if (n >= 8) {
+    __builtin_memcpy(to, &q, 8);
+  } else {
+    for (int i = 0; i < 8; ++i)
+      if (i < n) to[i] = (int8_t)(q >> (8 * i));
+  }
+  if (c % 4 == 0) g.e[token * g.lde + c / 4] = (uint8_t)(flag ? 255 : e + 127);
+}
+
+template <typename T> __global__ __launch_bounds__(256) void ckpt8_unpack_kernel(PackArgs g) {
+  using E = typename T::elem;
+  using x8 = typename T::x8;
+  int64_t token;
+  int c;
+  if (!chunk_of(g, token, c)) return;
+  const int n = g.k - c * 8;
+  if (n <= 0) return;
+  const int8_t* from = g.q + token * g.ldq + c * 8;
+  uint64_t q = 0;
+  if (n >= 8) {
+    __builtin_memcpy(&q, from, 8);
+  } else {
+    for (int i = 0; i < 8; ++i)
+      if (i < n) q |= (uint64_t)(uint8_t)from[i] << (8 * i);
+  }
+  const float scale = exponent_scale(g.e[token * g.lde + c / 4]);
+  x8 v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (E)((float)(int8_t)(q >> (8 * i)) * scale);
+  E* to = static_cast<E*>(g.out) + token * g.ldx + c * 8;
+  if (n >= 8) {
+    __builtin_memcpy(to, &v, sizeof v);
+  } else {
+    for (int i = 0; i < 8; ++i)
+      if (i < n) to[i] = v[i];
+  }
+}
+
+PackArgs pack_args(int64_t k, int64_t n) {
+  PackArgs g = {};
+  g.k = (int)k;
+  g.chunks = (int)((k + 31) / 32 * 4);
+  g.total = n * g.chunks;
+  return g;
+}
+
+// C = beta C + the pieces of a split reduction, in their order; C is rows x cols.
+__global__ __launch_bounds__(256) void ckpt8_join_kernel(const float* __restrict__ partial, int splits, int rows, int64_t total, float beta,
+                                                         float* __restrict__ c, int64_t ldc) {
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
+    float sum = 0.0f;
+    for (int z = 0; z < splits; ++z) sum += partial[(int64_t)z * total + q];
+    const int64_t col = q / rows;
+    float* at = c + col * ldc + (q - col * rows);
+    *at = sum + (beta != 0.0f ? beta * *at : 0.0f);
+  }
+}
+
+int choose_pieces(int64_t m, int64_t k, int64_t n, int64_t* n_piece) {
+  const int64_t tiles = ((m + 127) / 128) * ((k + 127) / 128);
+  const int64_t want = std::min<int64_t>(std::max<int64_t>(512 / std::max<int64_t>(tiles, 1), 1), std::max<int64_t>(n / 512, 1));
+  *n_piece = std::max<int64_t>(((n + want - 1) / want + 63) / 64 * 64, 64);
+  return (int)std::max<int64_t>((n + *n_piece - 1) / *n_piece, 1);
+}
+
+template <typename T, int SRC, int OUT, int B, int WM, int WN> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
+  const dim3 grid((unsigned)(((g.m + B - 1) / B) * ((g.n + B - 1) / B)), g.splits);
+  hipLaunchKernelGGL((half_gemm_kernel<T, MC, QUANT, MC, SRC, OUT, B, B, WM, WN>), grid, dim3(WM * WN * 64), 0, s, g);
+  return hipGetLastError();
+}
+template <typename T, int OUT> hipError_t launch_out(const HalfGemm& g, bool direct, bool large, hipStream_t s) {
+  if (!direct) return launch_tiles<T, STAGED, OUT, 128, 2, 2>(g, s);
+  return large ? launch_tiles<T, DIRECT, OUT, 256, 2, 4>(g, s) : launch_tiles<T, DIRECT, OUT, 128, 2, 2>(g, s);
+}
+
+}  // namespace
+
+hipError_t ckpt8_pack_device(int kind, int64_t k, int64_t n, const void* x, int64_t ldx, int8_t* q, int64_t ldq, uint8_t* e,
+                             int64_t lde, hipStream_t s) {
+  PackArgs g = pack_args(k, n);
+  g.x = x; g.ldx = ldx; g.q = q; g.ldq = ldq; g.e = e; g.lde = lde;
+  const dim3 grid((unsigned)((g.total + 255) / 256));
+  if (kind == BF16) hipLaunchKernelGGL(ckpt8_pack_kernel<Bf16>, grid, dim3(256), 0, s, g);
+  else if (kind == F16K) hipLaunchKernelGGL(ckpt8_pack_kernel<F16>, grid, dim3(256), 0, s, g);
+  else hipLaunchKernelGGL(ckpt8_pack_kernel<Fp32>, grid, dim3(256), 0, s, g);
+  return hipGetLastError();
+}
+
+hipError_t ckpt8_unpack_device(int kind, int64_t k, int64_t n, const int8_t* q, int64_t ldq, const uint8_t* e, int64_t lde,
+                               void* x, int64_t ldx, hipStream_t s) {
+  PackArgs g = pack_args(k, n);
+  g.out = x; g.ldx = ldx; g.q = const_cast<int8_t*>(q); g.ldq = ldq; g.e = const_cast<uint8_t*>(e); g.lde = lde;
+  const dim3 grid((unsigned)((g.total + 255) / 256));
+  if (kind == BF16) hipLaunchKernelGGL(ckpt8_unpack_kernel<Bf16>, grid, dim3(256), 0, s, g);
+  else if (kind == F16K) hipLaunchKernelGGL(ckpt8_unpack_kernel<F16>, grid, dim3(256), 0, s, g);
+  else hipLaunchKernelGGL(ckpt8_unpack_kernel<Fp32>, grid, dim3(256), 0, s, g);
+  return hipGetLastError();
+}
+
+int64_t ckpt8_grad_work_bytes(int kind, int64_t m, int64_t n, int64_t k) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  if (kind == F32) return (k * n * 4 + 255) / 256 * 256 + std::min<int64_t>(16 * m * k * 4, (int64_t)256 << 20);
+  int64_t piece;
+  const int splits = choose_pieces(m, k, n, &piece);
+  return splits > 1 ? splits * m * k * 4 : 0;
+}
+
+hipError_t ckpt8_grad_device(const Ckpt8GradArgs& c, hipStream_t s) {
+  if (c.kind == F32) {
+    // unpacked once, then the library's own product
+    float* x = static_cast<float*>(c.work);
+    hipError_t e = c.n > 0 ? ckpt8_unpack_device(F32, c.k, c.n, c.q, c.ldq, c.e, c.lde, x, c.k, s) : hipSuccess;
+    if (e != hipSuccess) return e;
+    GemmCall q;
+    q.kind = F32;
+    q.m = c.trans ? c.k : c.m; q.n = c.trans ? c.m : c.k; q.k = c.n;
+    q.opa = OP_N; q.opb = OP_T;
+    q.alpha[0] = 1.0; q.alpha[1] = 0.0; q.beta[0] = c.beta; q.beta[1] = 0.0;
+    q.A = c.trans ? x : c.dy; q.lda = c.trans ? c.k : c.lddy;
+    q.B = c.trans ? c.dy : x; q.ldb = c.trans ? c.lddy : c.k;
+    q.C = c.dw; q.ldc = c.lddw;
+    const int64_t used = (c.k * c.n * 4 + 255) / 256 * 256;
+    q.partials = c.work ? static_cast<char*>(c.work) + used : static_cast<void*>(c.dw);
+    q.partials_bytes = c.work && c.work_bytes > used ? (size_t)(c.work_bytes - used) : 0;
+    return launch_gemm_f32(q, s);
+  }
+  HalfGemm g;
+  g.m = (int)c.k; g.n = (int)c.m; g.k = (int)c.n;
+  g.a = c.q; g.lda = c.ldq;
+  g.exponents = c.e; g.lde = c.lde;
+  g.b = c.dy; g.ldb = c.lddy;
+  g.c = c.dw; g.ldc = c.lddw;
+  g.beta = c.beta;
+  int64_t piece;
+  const int splits = choose_pieces(c.m, c.k, c.n, &piece);
+  g.k_piece = (int)std::max<int64_t>((c.n + 63) / 64 * 64, 64);
+  if (splits > 1 && c.work && c.work_bytes >= splits * c.m * c.k * 4) {
+    g.splits = splits;
+    g.k_piece = (int)piece;
+    g.partial = static_cast<float*>(c.work);
+  }
+  const bool direct = (uintptr_t)c.dy % 16 == 0 && c.lddy % 8 == 0 && c.m % 8 == 0;
+  const bool large = g.splits == 1 && ((c.m + 255) / 256) * ((c.k + 255) / 256) >= 200;
+  hipError_t e;
+  if (c.kind == BF16) e = c.trans ? launch_out<Bf16, OUT_F32>(g, direct, large, s) : launch_out<Bf16, OUT_F32_SWAPPED>(g, direct, large, s);
+  else e = c.trans ? launch_out<F16, OUT_F32>(g, direct, large, s) : launch_out<F16, OUT_F32_SWAPPED>(g, direct, large, s);
+  if (e != hipSuccess || g.splits == 1) return e;
+  const int64_t total = c.m * c.k;
+  hipLaunchKernelGGL(ckpt8_join_kernel, dim3((unsigned)std::min<int64_t>((total + 255) / 256, 4096)), dim3(256), 0, s, g.partial, g.splits,
+                     (int)(c.trans ? c.k : c.m), total, c.beta, c.dw, c.lddw);
+  return hipGetLastError();
+}
+
+}  // namespace eigamd

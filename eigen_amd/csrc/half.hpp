@@ -1,0 +1,120 @@
+// 16-bit scalars, their matrix instructions and the small pieces the low-rank and checkpoint kernels share.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace eigamd {
+
+using f32x4 = float __attribute__((ext_vector_type(4)));
+using i16x4 = short __attribute__((ext_vector_type(4)));
+
+#define EIGAMD_LDS(T, p) ((__attribute__((address_space(3))) T*)(p))
+#define EIGAMD_GLOBAL(p) ((const __attribute__((address_space(1))) void*)(p))
+
+// Eight consecutive elements along the reduction are what a lane hands to one 16 x 16 x 32 product: lane l holds row (or
+// column) l % 16 and positions 8 (l / 16) .. + 7 of the reduction.  The result holds column l % 16, rows 4 (l / 16) .. + 3.
+struct Bf16 {
+  using elem = __bf16;
+  using x8 = __bf16 __attribute__((ext_vector_type(8)));
+  using x4 = __bf16 __attribute__((ext_vector_type(4)));
+  static constexpr int bytes = 2;
+  static __device__ __forceinline__ f32x4 mma(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ x4 read_transposed(const void* p) { return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(EIGAMD_LDS(i16x4, p))); }
+};
+struct F16 {
+  using elem = _Float16;
+  using x8 = _Float16 __attribute__((ext_vector_type(8)));
+  using x4 = _Float16 __attribute__((ext_vector_type(4)));
+  static constexpr int bytes = 2;
+  static __device__ __forceinline__ f32x4 mma(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ x4 read_transposed(const void* p) { return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(EIGAMD_LDS(i16x4, p))); }
+};
+// Single precision has no 32-deep product; the eight values of a lane go through eight 4-deep ones, which reduce over the
+// same 32 positions (in another order, the same one for both operands).
+struct Fp32 {
+  using elem = float;
+  using x8 = float __attribute__((ext_vector_type(8)));
+  static constexpr int bytes = 4;
+  static __device__ __forceinline__ f32x4 mma(x8 a, x8 b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// A float as a sum of NP values of the 16-bit type: each piece takes the leading bits of what is left.  Two pieces of a
+// normalised v leave 2^-17 (bf16) or 2^-23 (f16) of it out.  Three bf16 pieces hold all 24 bits of any finite v: they are cut,
+// not rounded, 8 bits each (rounding up could leave the range).  What is not finite stays in the first piece (a difference of
+// infinities would be a NaN).
+template <typename T, int NP> __device__ __forceinline__ void split(float v, typename T::elem (&piece)[NP]) {
+  const bool finite = __builtin_fabsf(v) < __builtin_inff();
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    if constexpr (__is_same(T, Bf16) && NP == 3) {
+      const float cut = finite ? __int_as_float(__float_as_int(v) & 0xffff0000) : v;
+      piece[i] = (typename T::elem)cut;
+      v = finite ? v - cut : 0.0f;
+    } else {
+      piece[i] = (typename T::elem)v;
+      v = finite ? v - (float)piece[i] : 0.0f;
+    }
+  }
+}
+
+// Power of two that brings the largest of |v| into [2^13, 2^14), and its inverse (1 where that is zero or not finite).  The
+// second piece of an f16 value then stays clear of f16's subnormals for everything down to 2^-27 of the largest.
+struct Norm {
+  float down, up;
+};
+__device__ __forceinline__ Norm norm_of(float largest) {
+  int e = (__float_as_int(largest) >> 23) & 255;
+  if (e == 255 || e == 0) return {1.0f, 1.0f};
+  e = e < 14 ? 14 : (e > 250 ? 250 : e);
+  return {__int_as_float((267 - e) << 23), __int_as_float((e - 13) << 23)};
+}
+
+// 2^(e - 127) for an exponent byte.  255 gives infinity: a block that held infinities or NaN is stored as zeros with
+// exponent 255 and comes back as 0 * inf = NaN.
+__device__ __forceinline__ float exponent_scale(unsigned e) { return __int_as_float((int)(e << 23)); }
+
+template <typename E, typename V> __device__ __forceinline__ V load_8(const E* p) {
+  V v;
+  __builtin_memcpy(&v, p, 8 * sizeof(E));
+  return v;
+}
+// n <= 8 elements from p (any alignment), the rest zero.
+template <typename E, typename V> __device__ __forceinline__ V load_up_to_8(const E* p, int n) {
+  if (n >= 8) return load_8<E, V>(p);
+  V v;
+  {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (E)0.0f;
+  }
+  return v;
+}
+
+// Which piece of which adapter workgroup-slot t stands for, when every adapter's run of the sorted batch is cut into pieces of
+// `size` tokens.  Adapter j's pieces take the slots from starts[j] / size + j on: the base of j + 1 is never below the base of
+// j plus j's pieces, so slots are unique without a prefix sum, and there are at most n / size + adapters + 1 of them.
+// One wave finds j by counting bases <= t.  Returns false for a slot that no piece has.
+struct Piece {
+  int adapter, begin, end, run_begin, run_end;
+};
+__device__ __forceinline__ bool find_piece(const int* starts, int segments, int size, int t, Piece& out) {
+  const int lane = threadIdx.x & 63;
+  int below = 0;
+  for (int j0 = 0; j0 < segments; j0 += 64) {
+    const int j = j0 + lane;
+    const bool on = j < segments && starts[j] / size + j <= t;
+    below += __popcll(__ballot(on));
+  }
+  const int j = below - 1;   // base of adapter 0 is 0
+  out.adapter = j;
+  out.run_begin = starts[j];
+  out.run_end = starts[j + 1];
+  out.begin = out.run_begin + (t - (out.run_begin / size + j)) * size;
+  out.end = out.begin + size < out.run_end ? out.begin + size : out.run_end;
+  return out.begin < out.run_end;
+}
+
+}  // namespace eigamd

@@ -1,0 +1,596 @@
+// Low-rank adapters of many requests beside a shared projection:
+//   P(:,i) = op(A_j) x_i,   Y(:,i) = op(W) x_i + s_j op(B_j) P(:,i),   j the adapter of token i,
+// and the gradients of the factors,
+//   G_j = s_j sum over j's tokens of u_i p_i^T   (dB: u = dY, p = P; dA: u = X, p = op(B_j)^T dY).
+// dX is the first operator again with the factors transposed and their roles exchanged.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "gemm_launch.hpp"
+#include "half_gemm.hpp"
+#include "lowrank.hpp"
+
+namespace eigamd {
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------------- plan
+// One wave per adapter (and one for the tokens without): it counts the tokens in front of its run and lists its own in their
+// order, by ballots -- no atomics, no prefix sum over adapters, the same list every time.
+__global__ __launch_bounds__(256) void lora_plan_kernel(const int* __restrict__ ids, int n, int adapters, int* __restrict__ order,
+                                                        int* __restrict__ seg, int* __restrict__ starts) {
+  const int j = blockIdx.x * 4 + threadIdx.x / 64, l = threadIdx.x & 63;
+  if (j > adapters) return;
+  int before = 0;
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const int i = i0 + l;
+    int id = i < n ? ids[i] : -1;
+    if (id < 0 || id >= adapters) id = adapters;
+    before += __popcll(__ballot(i < n && id < j));
+  }
+  if (l == 0) {
+    starts[j] = before;
+    if (j == adapters) starts[adapters + 1] = n;
+  }
+  int at = before;
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const int i = i0 + l;
+    int id = i < n ? ids[i] : -1;
+    if (id < 0 || id >= adapters) id = adapters;
+    const unsigned long long mine = __ballot(i < n && id == j);
+    if (i < n && id == j) {
+      const int to = at + __popcll(mine & ((1ull << l) - 1));
+      order[to] = i;
+      seg[to] = j;
+    }
+    at += __popcll(mine);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------- projection
+constexpr int kProjTokens = 32;
+struct ProjectArgs {
+  int n, k, rank, none;
+  const void* x; int64_t ldx;
+  const void* a; int64_t a_row, a_k, a_stride;    // strides of op(A_j)(r, k) and of j
+  const int* order;
+  const int* starts;
+  float* p; int64_t ldp;
+};
+
+// P for up to 32 tokens of one adapter and 16 RT ranks.  Eight waves share the reduction, each straight from memory to the
+// matrix unit: a lane reads 32 consecutive positions of its token (64 bytes), so the order of the reduction is permuted the
+// same way for both operands.
+template <typename T, int RT> __global__ __launch_bounds__(512) void lora_project_kernel(ProjectArgs g) {
+  using E = typename T::elem;
+  using x8 = typename T::x8;
+  Piece piece;
+  if (!find_piece(g.starts, g.none + 1, kProjTokens, blockIdx.x, piece)) return;
+  const int w = threadIdx.x / 64, l = threadIdx.x & 63, r0 = blockIdx.y * 64;
+  __shared__ f32x4 red[8][RT][2][64];
+  const bool live = piece.adapter != g.none;
+  if (live) {
+    // lanes past the piece or the rank repeat the last one; what they compute is not stored
+    f32x4 acc[RT][2] = {};
+    const E* x[2];
+    const E* a[RT];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int at = piece.begin + c * 16 + (l & 15);
+      x[c] = static_cast<const E*>(g.x) + (int64_t)g.order[at < piece.end ? at : piece.end - 1] * g.ldx;
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int r = r0 + t * 16 + (l & 15);
+      a[t] = static_cast<const E*>(g.a) + (int64_t)piece.adapter * g.a_stride + (int64_t)(r < g.rank ? r : g.rank - 1) * g.a_row;
+    }
+    for (int k0 = w * 128; k0 < g.k; k0 += 8 * 128) {
+      const bool whole = k0 + 128 <= g.k;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int k = k0 + (l / 16) * 32 + s * 8, left = whole ? 8 : g.k - k;
+        x8 fx[2], fa[RT];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) fx[c] = whole ? load_8<E, x8>(x[c] + k) : load_up_to_8<E, x8>(x[c] + k, left);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          if (g.a_k == 1) {
+            fa[t] = whole ? load_8<E, x8>(a[t] + k) : load_up_to_8<E, x8>(a[t] + k, left);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) fa[t][e] = e < left ? a[t][(int64_t)(k + e) * g.a_k] : (E)0.0f;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) acc[t][c] = T::mma(fa[t], fx[c], acc[t][c]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) red[w][t][c][l] = acc[t][c];
+  }
+  __syncthreads();
+  for (int q = threadIdx.x; q < RT * 2 * 64; q += 512) {
+    const int t = q / 128, c = (q / 64) % 2, at = piece.begin + c * 16 + (l & 15);
+    if (at >= piece.end) continue;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (live)
+      for (int z = 0; z < 8; ++z) sum += red[z][t][c][l];
+    const int r = r0 + t * 16 + (l / 16) * 4;
+    float* out = g.p + (int64_t)g.order[at] * g.ldp + r;
+    for (int e = 0; e < 4; ++e)
+      if (r + e < g.rank) out[e] = sum[e];
+  }
+}
+
+template <typename T> hipError_t launch_project(const ProjectArgs& g, hipStream_t s) {
+  const dim3 grid(g.n / kProjTokens + g.none + 1, (g.rank + 63) / 64);
+  if (g.rank <= 16) hipLaunchKernelGGL((lora_project_kernel<T, 1>), grid, dim3(512), 0, s, g);
+  else if (g.rank <= 32) hipLaunchKernelGGL((lora_project_kernel<T, 2>), grid, dim3(512), 0, s, g);
+  else hipLaunchKernelGGL((lora_project_kernel<T, 4>), grid, dim3(512), 0, s, g);
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------------------------------------------ few tokens (KC)
+// Y for at most 16 NG tokens, W's reduction contiguous: the time is that of reading W once, so nothing is staged.  A workgroup
+// owns 16 rows; its eight waves share the reduction (128 positions a turn) and feed the matrix unit straight from memory.
+template <typename T, int NG> __global__ __launch_bounds__(512) void lora_few_kernel(HalfGemm g) {
+  using E = typename T::elem;
+  using x8 = typename T::x8;
+  const int w = threadIdx.x / 64, l = threadIdx.x & 63, row0 = blockIdx.x * 16;
+  const int row = row0 + (l & 15);
+  const E* a = static_cast<const E*>(g.a) + (int64_t)(row < g.m ? row : g.m - 1) * g.lda;
+  const E* b[NG];                     // columns past the last repeat it and are not stored
+#pragma unroll
+  for (int c = 0; c < NG; ++c) {
+    const int at = c * 16 + (l & 15);
+    b[c] = static_cast<const E*>(g.b) + (int64_t)g.order[at < g.n ? at : g.n - 1] * g.ldb;
+  }
+  f32x4 acc[NG] = {};
+  for (int k0 = w * 128; k0 < g.k; k0 += 8 * 128) {
+    x8 fa[4], fb[4][NG];
+    const bool whole = k0 + 128 <= g.k;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int k = k0 + (l / 16) * 32 + s * 8, left = g.k - k;
+      fa[s] = whole ? load_8<E, x8>(a + k) : load_up_to_8<E, x8>(a + k, left);
+#pragma unroll
+      for (int c = 0; c < NG; ++c) fb[s][c] = whole ? load_8<E, x8>(b[c] + k) : load_up_to_8<E, x8>(b[c] + k, left);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int c = 0; c < NG; ++c) acc[c] = T::mma(fa[s], fb[s][c], acc[c]);
+  }
+  __shared__ f32x4 red[8][NG][64];
+#pragma unroll
+  for (int c = 0; c < NG; ++c) red[w][c][l] = acc[c];
+  __syncthreads();
+  // one output per thread and turn: 16 rows of a token are 16 neighbouring threads
+  for (int q = threadIdx.x; q < 256 * NG; q += 512) {
+    const int r = q % 16, col = q / 16;
+    if (col >= g.n || row0 + r >= g.m) continue;
+    float sum = 0.0f;
+    for (int z = 0; z < 8; ++z) sum += red[z][col / 16][(r / 4) * 16 + col % 16][r % 4];
+    const int token = g.order[col], who = g.seg[col];
+    if (who != g.none && g.rank > 0) {
+      const E* up = static_cast<const E*>(g.up) + (int64_t)who * g.up_stride + (int64_t)(row0 + r) * g.up_row;
+      const float* p = g.p + (int64_t)token * g.ldp;
+      float d = 0.0f;
+      for (int t = 0; t < g.rank; ++t) d += (float)up[(int64_t)t * g.up_rank] * p[t];
+      sum += g.scale[who] * d;
+    }
+    static_cast<E*>(g.c)[(int64_t)token * g.ldc + row0 + r] = (E)sum;
+  }
+}
+
+// Sums of a split reduction, in the order of the pieces.
+template <typename E> __global__ __launch_bounds__(256) void lora_join_kernel(HalfGemm g) {
+  const int64_t total = (int64_t)g.m * g.n;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
+    float sum = 0.0f;
+    for (int z = 0; z < g.splits; ++z) sum += g.partial[(int64_t)z * total + q];
+    const int col = (int)(q / g.m), row = (int)(q - (int64_t)col * g.m);
+    static_cast<E*>(g.c)[(int64_t)g.order[col] * g.ldc + row] = (E)sum;
+  }
+}
+
+// Y += s_j op(B_j) P in single precision, behind the plain product.
+__global__ __launch_bounds__(256) void lora_add_f32_kernel(HalfGemm g) {
+  const int w = threadIdx.x / 64, l = threadIdx.x & 63;
+  const int row0 = blockIdx.y * 256 + w * 64, col0 = blockIdx.x * 64;
+  if (row0 >= g.m) return;
+  f32x4 acc[4][4] = {};
+  add_adapters<Fp32, 4, 4>(g, row0, col0, acc);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = col0 + j * 16 + (l & 15);
+    if (c >= g.n || g.seg[c] == g.none) continue;
+    float* y = static_cast<float*>(g.c) + (int64_t)g.order[c] * g.ldc;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      for (int t = 0; t < 4; ++t) {
+        const int r = row0 + i * 16 + (l / 16) * 4 + t;
+        if (r < g.m) y[r] += acc[i][j][t];
+      }
+  }
+}
+
+// Pieces of the reduction for a grid of `tiles` workgroups: enough to fill the 256 compute units about twice, none shorter
+// than 256 positions.
+int choose_pieces(int64_t tiles, int64_t k, int64_t* k_piece) {
+  int64_t want = std::min<int64_t>(std::max<int64_t>(512 / std::max<int64_t>(tiles, 1), 1), std::max<int64_t>(k / 256, 1));
+  const int64_t piece = ((k + want - 1) / want + 63) / 64 * 64;
+  *k_piece = std::max<int64_t>(piece, 64);
+  return (int)std::max<int64_t>((k + *k_piece - 1) / *k_piece, 1);
+}
+
+int64_t tiles128(int64_t m, int64_t n) { return ((m + 127) / 128) * ((n + 127) / 128); }
+int64_t tiles256(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256); }
+bool few(bool w_trans, int64_t n) { return w_trans && n <= 64; }
+
+template <typename T, int LA, int SRC, int B, int WM, int WN> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
+  const dim3 grid((unsigned)(B == 256 ? tiles256(g.m, g.n) : tiles128(g.m, g.n)), g.splits);
+  hipLaunchKernelGGL((half_gemm_kernel<T, LA, SRC, KC, SRC, OUT_HALF, B, B, WM, WN>), grid, dim3(WM * WN * 64), 0, s, g);
+  return hipGetLastError();
+}
+
+template <typename T> hipError_t launch_half(const LoraArgs& c, hipStream_t s) {
+  HalfGemm g;
+  g.m = (int)c.m; g.n = (int)c.n; g.k = (int)c.k;
+  g.a = c.w; g.lda = c.ldw;
+  g.b = c.x; g.ldb = c.ldx;
+  g.c = c.y; g.ldc = c.ldy;
+  g.order = c.plan.order;
+  g.seg = c.plan.seg;
+  g.none = c.plan.adapters;
+  g.rank = c.plan.adapters > 0 ? (int)c.rank : 0;
+  g.up = c.b;
+  g.up_row = c.b_trans ? c.ldb : 1;
+  g.up_rank = c.b_trans ? 1 : c.ldb;
+  g.up_stride = c.stride_b;
+  g.p = c.p; g.ldp = c.ldp;
+  g.scale = c.scale;
+  g.k_piece = (int)std::max<int64_t>((c.k + 63) / 64 * 64, 64);
+  if (few(c.w_trans, c.n)) {
+    const dim3 grid((unsigned)((c.m + 15) / 16));
+    switch ((c.n + 15) / 16) {
+      case 1: hipLaunchKernelGGL((lora_few_kernel<T, 1>), grid, dim3(512), 0, s, g); break;
+      case 2: hipLaunchKernelGGL((lora_few_kernel<T, 2>), grid, dim3(512), 0, s, g); break;
+      case 3: hipLaunchKernelGGL((lora_few_kernel<T, 3>), grid, dim3(512), 0, s, g); break;
+      default: hipLaunchKernelGGL((lora_few_kernel<T, 4>), grid, dim3(512), 0, s, g); break;
+    }
+    return hipGetLastError();
+  }
+  int64_t piece = g.k_piece;
+  const int splits = choose_pieces(tiles128(c.m, c.n), c.k, &piece);
+  if (splits > 1 && c.work && c.work_bytes >= (int64_t)splits * c.m * c.n * 4) {
+    g.splits = splits;
+    g.k_piece = (int)piece;
+    g.partial = static_cast<float*>(c.work);
+  }
+  // whole 16-byte chunks everywhere: the loads go to LDS without passing through registers
+  const bool direct = ((uintptr_t)c.w | (uintptr_t)c.x) % 16 == 0 && c.ldw % 8 == 0 && c.ldx % 8 == 0 && c.k % 8 == 0 &&
+                      (c.w_trans || c.m % 8 == 0);
+  hipError_t e;
+  if (direct && g.splits == 1 && tiles256(c.m, c.n) >= 200)
+    e = c.w_trans ? launch_tiles<T, KC, DIRECT, 256, 2, 4>(g, s) : launch_tiles<T, MC, DIRECT, 256, 2, 4>(g, s);
+  else if (direct)
+    e = c.w_trans ? launch_tiles<T, KC, DIRECT, 128, 2, 2>(g, s) : launch_tiles<T, MC, DIRECT, 128, 2, 2>(g, s);
+  else
+    e = c.w_trans ? launch_tiles<T, KC, STAGED, 128, 2, 2>(g, s) : launch_tiles<T, MC, STAGED, 128, 2, 2>(g, s);
+  if (e == hipSuccess && g.splits > 1) {
+    const unsigned blocks = (unsigned)std::min<int64_t>((c.m * c.n + 255) / 256, 4096);
+    hipLaunchKernelGGL((lora_join_kernel<typename T::elem>), dim3(blocks), dim3(256), 0, s, g);
+    e = hipGetLastError();
+  }
+  return e;
+}
+
+// ------------------------------------------------------------------------------------------------ gradients of the factors
+constexpr int kGradRows = 256;
+
+struct GradArgs {
+  int rows, rank, n, none, chunk;
+  bool trans;
+  const void* u; int64_t ldu;
+  const uint8_t* exponents; int64_t lde;
+  const float* p; int64_t ldp;
+  const float* scale;
+  const int* order;
+  const int* starts;
+  float beta;
+  float* g; int64_t ldg, stride_g;
+  float* partial;
+};
+
+// Tokens per workgroup: about 512 workgroups in all, between 128 and 1024 tokens each.
+int grad_chunk(int64_t rows, int64_t n) {
+  const int64_t across = (rows + kGradRows - 1) / kGradRows;
+  const int64_t pieces = std::max<int64_t>(512 / across, 1);
+  const int64_t c = ((n + pieces - 1) / pieces + 31) / 32 * 32;
+  return (int)std::min<int64_t>(std::max<int64_t>(c, 128), 1024);
+}
+
+// 32 tokens x 256 rows of u in LDS: lines of tokens, chunks permuted as in SliceLoader (MC).  Single precision lies unpermuted
+// and is read one element a lane.
+template <typename T, int SRC> struct GradTile {
+  using E = typename T::elem;
+  using x8 = typename T::x8;
+  static constexpr int bytes = 32 * kGradRows * T::bytes;
+  x8 reg[4];
+  static __device__ __forceinline__ int swizzle(int line) { return T::bytes == 4 ? 0 : ((line & 3) | ((line >> 1) & 4)) << 1; }
+  // token of line i: tok[i], -1 past the end
+  __device__ __forceinline__ void load(char* lds, const GradArgs& g, const int* tok, int row0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int ch = threadIdx.x + i * 256, line = ch / 32, c = (ch % 32) ^ swizzle(line), row = row0 + c * 8;
+      const int t = tok[line], n = t < 0 ? 0 : g.rows - row;
+      if constexpr (SRC == DIRECT) {
+        const char* q = static_cast<const char*>(g.u) + ((int64_t)t * g.ldu + row) * 2;
+        const char* from = n > 0 ? q : reinterpret_cast<const char*>(zero_page);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+        __builtin_amdgcn_global_load_lds(EIGAMD_GLOBAL(from), EIGAMD_LDS(void, lds + (i * 256 + wave * 64) * 16), 16, 0, 0);
+      } else if constexpr (SRC == STAGED) {
+        reg[i] = load_up_to_8<E, x8>(static_cast<const E*>(g.u) + (int64_t)t * g.ldu + row, n);
+      } else {
+        const int8_t* q = static_cast<const int8_t*>(g.u) + (int64_t)t * g.ldu + row;
+        uint64_t v = 0;
+        if (n >= 8) {
+          __builtin_memcpy(&v, q, 8);
+        } else {
+          for (int e = 0; e < 8; ++e)
+            if (e < n) v |= (uint64_t)(uint8_t)q[e] << (8 * e);
+        }
+        const float sc = exponent_scale(n > 0 ? g.exponents[(int64_t)t * g.lde + row / 32] : 0u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) reg[i][e] = (E)((float)(int8_t)(v >> (8 * e)) * sc);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* lds) {
+    if constexpr (SRC == DIRECT) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<x8*>(lds + (threadIdx.x + i * 256) * 8 * T::bytes) = reg[i];
+  }
+  static __device__ __forceinline__ x8 fragment(const char* lds, int row) {
+    const int l = threadIdx.x & 63;
+    if constexpr (T::bytes == 4) {
+      x8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const float*>(lds + (((l / 16) * 8 + e) * kGradRows + row + (l & 15)) * 4);
+      return v;
+    } else {
+      union { x8 v; typename T::x4 h[2]; } f;
+      const int line = (l / 16) * 8 + (l & 15) / 4, at = row / 8 + (l & 3) / 2;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        f.h[h] = T::read_transposed(lds + (line + 4 * h) * (kGradRows * 2) + ((at ^ swizzle(line + 4 * h)) * 16) + (l & 1) * 8);
+      return f.v;
+    }
+  }
+};
+
+// G_j over one piece of j's tokens: 256 rows x 16 RT ranks per workgroup, 32 tokens a turn.  p keeps (nearly) all of its 32 bits
+// as several 16-bit pieces; the sums are the matrix unit's 32 bits.  A run that is one piece goes straight to G_j.
+template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(256) void lora_grad_kernel(GradArgs g) {
+  using E = typename T::elem;
+  using x8 = typename T::x8;
+  constexpr int NP = T::bytes == 4 ? 1 : (__is_same(T, Bf16) ? 3 : 2);
+  Piece piece;
+  if (!find_piece(g.starts, g.none + 1, g.chunk, blockIdx.y, piece) || piece.adapter == g.none) return;
+  using Tile = GradTile<T, SRC>;
+  __shared__ __align__(1024) char lds[2 * Tile::bytes];
+  __shared__ int tok[1024 + 32];
+  __shared__ float tops[4];
+  const int count = piece.end - piece.begin, turns = (count + 31) / 32;
+  const int w = threadIdx.x / 64, l = threadIdx.x & 63;
+  const int row0 = blockIdx.x * kGradRows, r0 = blockIdx.z * 64;
+  for (int i = threadIdx.x; i < turns * 32; i += 256) tok[i] = i < count ? g.order[piece.begin + i] : -1;
+  __syncthreads();
+  Norm nm = {1.0f, 1.0f};
+  if constexpr (__is_same(T, F16)) {
+    // one power of two for the piece's p, so that f16 pieces neither overflow nor vanish
+    float top = 0.0f;
+    const int width = g.rank - r0 < RT * 16 ? g.rank - r0 : RT * 16;
+    for (int i = threadIdx.x; i < count * width; i += 256) {
+      const float v = __builtin_fabsf(g.p[(int64_t)tok[i / width] * g.ldp + r0 + i % width]);
+      top = v < __builtin_inff() ? fmaxf(top, v) : top;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    if (l == 0) tops[w] = top;
+    __syncthreads();
+    nm = norm_of(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
+  }
+  Tile tile;
+  f32x4 acc[4][RT] = {};
+  tile.load(lds, g, tok, row0);
+  tile.store(lds);
+  __syncthreads();
+  for (int s = 0; s < turns; ++s) {
+    char* here = lds + (s & 1) * Tile::bytes;
+    char* next = lds + ((s & 1) ^ 1) * Tile::bytes;
+    float pv[RT][8];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int r = r0 + t * 16 + (l & 15);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int token = tok[s * 32 + (l / 16) * 8 + e];
+        pv[t][e] = token >= 0 && r < g.rank ? g.p[(int64_t)token * g.ldp + r] : 0.0f;
+      }
+    }
+    if (s + 1 < turns) tile.load(next, g, tok + (s + 1) * 32, row0);
+    x8 fu[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fu[i] = Tile::fragment(here, w * 64 + i * 16);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      x8 fp[NP];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (NP == 1) {
+          fp[0][e] = pv[t][e];
+        } else {
+          E q[NP];
+          split<T, NP>(pv[t][e] * nm.down, q);
+#pragma unroll
+          for (int z = 0; z < NP; ++z) fp[z][e] = q[z];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int z = NP - 1; z >= 0; --z) acc[i][t] = TRANS ? T::mma(fp[z], fu[i], acc[i][t]) : T::mma(fu[i], fp[z], acc[i][t]);
+    }
+    if (s + 1 < turns) tile.store(next);
+    __syncthreads();
+  }
+  const bool whole = piece.run_end - piece.run_begin <= g.chunk;
+  const float sj = whole ? g.scale[piece.adapter] : 1.0f;
+  float* out = whole ? g.g + (int64_t)piece.adapter * g.stride_g : g.partial + (int64_t)blockIdx.y * g.rows * g.rank;
+  const int64_t ld = whole ? g.ldg : (TRANS ? g.rank : g.rows);
+  const float beta = whole ? g.beta : 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int fast = TRANS ? r0 + t * 16 + (l / 16) * 4 : row0 + w * 64 + i * 16 + (l / 16) * 4;
+      const int slow = TRANS ? row0 + w * 64 + i * 16 + (l & 15) : r0 + t * 16 + (l & 15);
+      if (slow >= (TRANS ? g.rows : g.rank)) continue;
+      float* at = out + (int64_t)slow * ld + fast;
+      for (int e = 0; e < 4; ++e)
+        if (fast + e < (TRANS ? g.rank : g.rows)) at[e] = acc[i][t][e] * nm.up * sj + (beta != 0.0f ? beta * at[e] : 0.0f);
+    }
+}
+
+// G_j = beta G_j + s_j (sum of j's pieces, in the order of the batch); an adapter without tokens gets beta G_j.
+__global__ __launch_bounds__(256) void lora_grad_join_kernel(GradArgs g) {
+  const int j = blockIdx.y, begin = g.starts[j], count = g.starts[j + 1] - begin;
+  if (count > 0 && count <= g.chunk) return;
+  const int pieces = (count + g.chunk - 1) / g.chunk, slot = begin / g.chunk + j;
+  const int64_t size = (int64_t)g.rows * g.rank;
+  const int fast = g.trans ? g.rank : g.rows;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < size; q += (int64_t)gridDim.x * 256) {
+    float sum = 0.0f;
+    for (int z = 0; z < pieces; ++z) sum += g.partial[(int64_t)(slot + z) * size + q];
+    const int64_t slow = q / fast;
+    float* at = g.g + (int64_t)j * g.stride_g + slow * g.ldg + (q - slow * fast);
+    *at = (pieces ? g.scale[j] * sum : 0.0f) + (g.beta != 0.0f ? g.beta * *at : 0.0f);
+  }
+}
+
+template <typename T, int SRC, int RT> hipError_t launch_grad(const GradArgs& g, dim3 grid, hipStream_t s) {
+  if (g.trans) hipLaunchKernelGGL((lora_grad_kernel<T, SRC, RT, true>), grid, dim3(256), 0, s, g);
+  else hipLaunchKernelGGL((lora_grad_kernel<T, SRC, RT, false>), grid, dim3(256), 0, s, g);
+  return hipGetLastError();
+}
+template <typename T, int SRC> hipError_t launch_grad_rank(const GradArgs& g, dim3 grid, hipStream_t s) {
+  if (g.rank <= 16) return launch_grad<T, SRC, 1>(g, grid, s);
+  if (g.rank <= 32) return launch_grad<T, SRC, 2>(g, grid, s);
+  return launch_grad<T, SRC, 4>(g, grid, s);
+}
+
+}  // namespace
+
+hipError_t lora_plan_device(const int* ids, int64_t n, int64_t adapters, int* d_plan, hipStream_t s) {
+  hipLaunchKernelGGL(lora_plan_kernel, dim3((unsigned)(adapters / 4 + 1)), dim3(256), 0, s, ids, (int)n, (int)adapters, d_plan,
+                     d_plan + n, d_plan + 2 * n);
+  return hipGetLastError();
+}
+
+int64_t lora_work_bytes(int kind, bool w_trans, int64_t m, int64_t n, int64_t k) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  if (kind == F32) return std::min<int64_t>(16 * m * n * 4, (int64_t)256 << 20);
+  if (few(w_trans, n)) return 0;
+  int64_t piece;
+  const int splits = choose_pieces(tiles128(m, n), k, &piece);
+  return splits > 1 ? (int64_t)splits * m * n * 4 : 0;
+}
+
+hipError_t lora_device(const LoraArgs& c, hipStream_t s) {
+  hipError_t e = hipSuccess;
+  if (c.plan.adapters > 0) {
+    ProjectArgs g;
+    g.n = (int)c.n; g.k = (int)c.k; g.rank = (int)c.rank; g.none = c.plan.adapters;
+    g.x = c.x; g.ldx = c.ldx;
+    g.a = c.a;
+    g.a_row = c.a_trans ? c.lda : 1;
+    g.a_k = c.a_trans ? 1 : c.lda;
+    g.a_stride = c.stride_a;
+    g.order = c.plan.order; g.starts = c.plan.starts;
+    g.p = c.p; g.ldp = c.ldp;
+    e = c.kind == BF16 ? launch_project<Bf16>(g, s) : c.kind == F16K ? launch_project<F16>(g, s) : launch_project<Fp32>(g, s);
+    if (e != hipSuccess || c.m == 0) return e;
+  }
+  if (c.m == 0) return e;
+  if (c.kind == BF16) return launch_half<Bf16>(c, s);
+  if (c.kind == F16K) return launch_half<F16>(c, s);
+  GemmCall q;
+  q.kind = F32;
+  q.opa = c.w_trans ? OP_T : OP_N; q.opb = OP_N;
+  q.m = c.m; q.n = c.n; q.k = c.k;
+  q.alpha[0] = 1.0; q.alpha[1] = 0.0; q.beta[0] = 0.0; q.beta[1] = 0.0;
+  q.A = c.w; q.lda = c.ldw; q.B = c.x; q.ldb = c.ldx; q.C = c.y; q.ldc = c.ldy;
+  // (memory of the caller's, or none at all: either way the product allocates nothing and stays on this stream)
+  q.partials = c.work ? c.work : c.y;
+  q.partials_bytes = c.work ? (size_t)c.work_bytes : 0;
+  e = launch_gemm_f32(q, s);
+  if (e != hipSuccess || c.plan.adapters == 0) return e;
+  HalfGemm g;
+  g.m = (int)c.m; g.n = (int)c.n; g.k = (int)c.k;
+  g.c = c.y; g.ldc = c.ldy;
+  g.order = c.plan.order; g.seg = c.plan.seg; g.none = c.plan.adapters; g.rank = (int)c.rank;
+  g.up = c.b;
+  g.up_row = c.b_trans ? c.ldb : 1;
+  g.up_rank = c.b_trans ? 1 : c.ldb;
+  g.up_stride = c.stride_b;
+  g.p = c.p; g.ldp = c.ldp; g.scale = c.scale;
+  hipLaunchKernelGGL(lora_add_f32_kernel, dim3((unsigned)((c.n + 63) / 64), (unsigned)((c.m + 255) / 256)), dim3(256), 0, s, g);
+  return hipGetLastError();
+}
+
+int64_t lora_grad_work_bytes(int64_t rows, int64_t n, int64_t rank, int64_t adapters) {
+  const int chunk = grad_chunk(std::max<int64_t>(rows, 1), n);
+  return n > chunk ? (n / chunk + adapters + 1) * rows * rank * 4 : 0;
+}
+
+hipError_t lora_grad_device(const LoraGradArgs& c, hipStream_t s) {
+  GradArgs g;
+  g.rows = (int)c.rows; g.rank = (int)c.rank; g.n = (int)c.n; g.none = c.plan.adapters;
+  g.chunk = grad_chunk(c.rows, c.n);
+  g.trans = c.trans;
+  g.u = c.u; g.ldu = c.ldu; g.exponents = c.exponents; g.lde = c.lde;
+  g.p = c.p; g.ldp = c.ldp; g.scale = c.scale;
+  g.order = c.plan.order; g.starts = c.plan.starts;
+  g.beta = c.beta;
+  g.g = c.g; g.ldg = c.ldg; g.stride_g = c.stride_g;
+  g.partial = static_cast<float*>(c.work);
+  hipError_t e = hipSuccess;
+  if (c.n > 0) {
+    const dim3 grid((unsigned)((c.rows + kGradRows - 1) / kGradRows), (unsigned)(c.n / g.chunk + g.none + 1), (unsigned)((c.rank + 63) / 64));
+    const bool direct = (uintptr_t)c.u % 16 == 0 && c.ldu % 8 == 0 && c.rows % 8 == 0;
+    if (c.exponents) {
+      e = c.kind == BF16 ? launch_grad_rank<Bf16, QUANT>(g, grid, s)
+                         : c.kind == F16K ? launch_grad_rank<F16, QUANT>(g, grid, s) : launch_grad_rank<Fp32, QUANT>(g, grid, s);
+    } else if (c.kind == F32) {
+      e = launch_grad_rank<Fp32, STAGED>(g, grid, s);
+    } else if (direct) {
+      e = c.kind == BF16 ? launch_grad_rank<Bf16, DIRECT>(g, grid, s) : launch_grad_rank<F16, DIRECT>(g, grid, s);
+    } else {
+      e = c.kind == BF16 ? launch_grad_rank<Bf16, STAGED>(g, grid, s) : launch_grad_rank<F16, STAGED>(g, grid, s);
+    }
+    if (e != hipSuccess) return e;
+  }
+  const unsigned blocks = (unsigned)std::min<int64_t>((c.rows * c.rank + 255) / 256, 1024);
+  hipLaunchKernelGGL(lora_grad_join_kernel, dim3(blocks, (unsigned)g.none), dim3(256), 0, s, g);
+  return hipGetLastError();
+}
+
+}  // namespace eigamd

@@ -9,7 +9,7 @@ from . import _lib
 from ._lib import lib
 
 _TORCH_OF_KIND = {_lib.F32: torch.float32, _lib.F64: torch.float64, _lib.C32: torch.complex64,
-                  _lib.C64: torch.complex128}
+                  _lib.C64: torch.complex128, _lib.BF16: torch.bfloat16, _lib.F16: torch.float16}
 _NP_OF_KIND = {_lib.F32: np.float32, _lib.F64: np.float64, _lib.C32: np.complex64, _lib.C64: np.complex128}
 _KIND_OF_TORCH = {v: k for k, v in _TORCH_OF_KIND.items()}
 _OPCODE = {"N": _lib.OP_N, "T": _lib.OP_T, "C": _lib.OP_C, "J": _lib.OP_CONJ}

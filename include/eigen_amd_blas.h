@@ -13,8 +13,9 @@
 extern "C" {
 #endif
 
-/* Scalar kinds (argument `dtype`). */
-enum { EIGAMD_F32 = 0, EIGAMD_F64 = 1, EIGAMD_C32 = 2, EIGAMD_C64 = 3 };
+/* Scalar kinds (argument `dtype`).  The 16-bit kinds are taken by the adapter and checkpoint entries only
+ * (eigamd_lora_*, eigamd_ckpt8_*). */
+enum { EIGAMD_F32 = 0, EIGAMD_F64 = 1, EIGAMD_C32 = 2, EIGAMD_C64 = 3, EIGAMD_BF16 = 4, EIGAMD_F16 = 5 };
 
 /* Operand forms (arguments `opa`, `opb`).  N/T/C are the F77 'N','T','C'
  * (blas/common.h:47-50).  CONJ (conjugate without transposition) has no F77
@@ -408,6 +409,70 @@ int eigamd_symm_dev(int dtype, int side, int uplo, int hermitian, int64_t m, int
                     int64_t lda, const void* d_b, int64_t ldb, const void* beta, void* d_c, int64_t ldc, void* stream);
 int eigamd_trmm_dev(int dtype, int side, int uplo, int op, int diag, int64_t m, int64_t n, const void* alpha,
                     const void* d_a, int64_t lda, void* d_b, int64_t ldb, void* stream);
+
+/* ---- low-rank adapters of many requests beside a shared projection ---------------------
+ *
+ * No counterpart in the reference (its 16-bit scalars have no BLAS binding, and it has no batched low-rank product).
+ * A projection W (op(W) is m x k) is shared by all tokens; token i may have an adapter j, a product of two thin factors:
+ *
+ *   P(:,i) = op(A_j) X(:,i)                        op(A_j) is rank x k
+ *   Y(:,i) = op(W) X(:,i) + s_j op(B_j) P(:,i)     op(B_j) is m x rank
+ *
+ * X (k x n), Y (m x n) and P (rank x n) hold one token per column.  dtype (F32, BF16, F16) is that of W, X, A, B and Y; P and
+ * the scales s are float; sums are kept in float and rounded once, into Y.  A token without an adapter gets op(W) x_i and a
+ * zero column of P.  The factors lie `stride_a` / `stride_b` elements apart, adapter j at d_a + j * stride_a; op is N or T.
+ * P is an output: the backward pass reads it.
+ *
+ * eigamd_lora_plan_dev prepares a batch: d_adapter_of[i] (device memory) is token i's adapter, anything outside
+ * [0, n_adapters) means none; d_plan receives eigamd_lora_plan_ints(n, n_adapters) ints (tokens sorted by adapter).  The
+ * same plan serves every projection of every layer the batch passes through, forward and backward, and must have been made
+ * for the same n and n_adapters.  Tokens may come in any order; a column of Y and of P does not depend on it.
+ *
+ * dX is eigamd_lora_dev again with the factors transposed and their roles exchanged: dX = op(W)^T dY + s_j op(A_j)^T Q with
+ * Q = op(B_j)^T dY (pass the other op for W, B as `d_a` and A as `d_b`, each with the other op, Q as `d_p`).
+ *
+ * eigamd_lora_wgrad_dev is the gradient of a factor, G_j = beta G_j + s_j sum over j's tokens of u_i p_i^T (rows x rank, in
+ * float, stored as it is (opg N) or transposed (opg T)): dB_j from U = dY and P; dA_j^T from U = X and Q.  U is of kind dtype,
+ * or, with d_exponents, an 8-bit checkpoint (below; d_u then points to int8).  An adapter without tokens gets beta G_j; with
+ * beta = 0 G is not read.
+ *
+ * Limits: m, k, rows <= 2^22, n <= 2^24, rank 1..256, n_adapters <= 4096; n = 0 and n_adapters = 0 are allowed.  d_work is
+ * device memory of at least the bytes the matching query names (16-byte aligned; 0: may be NULL), free again behind the call;
+ * calls that may overlap need one each, so do captured graphs.  Everything is asynchronous on `stream`, allocates nothing, and
+ * gives the same bits every time.  Outputs must not overlap inputs.  The queries return -1 for arguments out of range. */
+int64_t eigamd_lora_plan_ints(int64_t n, int64_t n_adapters);
+int eigamd_lora_plan_dev(int64_t n, int64_t n_adapters, const int32_t* d_adapter_of, int32_t* d_plan, void* stream);
+int64_t eigamd_lora_work_bytes(int dtype, int opw, int64_t m, int64_t n, int64_t k);
+int eigamd_lora_dev(int dtype, int opw, int opa, int opb, int64_t m, int64_t n, int64_t k, int64_t rank, int64_t n_adapters,
+                    const void* d_w, int64_t ldw, const void* d_x, int64_t ldx, const void* d_a, int64_t lda, int64_t stride_a,
+                    const void* d_b, int64_t ldb, int64_t stride_b, const float* d_scale, const int32_t* d_plan, float* d_p,
+                    int64_t ldp, void* d_y, int64_t ldy, void* d_work, int64_t work_bytes, void* stream);
+int64_t eigamd_lora_wgrad_work_bytes(int64_t rows, int64_t n, int64_t rank, int64_t n_adapters);
+int eigamd_lora_wgrad_dev(int dtype, int opg, int64_t rows, int64_t n, int64_t rank, int64_t n_adapters, const void* d_u, int64_t ldu,
+                          const uint8_t* d_exponents, int64_t lde, const float* d_p, int64_t ldp, const float* d_scale,
+                          const int32_t* d_plan, const float* beta, float* d_g, int64_t ldg, int64_t stride_g, void* d_work,
+                          int64_t work_bytes, void* stream);
+
+/* ---- activations held in 8 bits for the backward pass --------------------------------------
+ *
+ * No counterpart in the reference.  X (k features x n tokens) becomes whole numbers Q (int8, k x n) and exponents E (bytes,
+ * ceil(k / 32) x n): X(f,i) stands for Q(f,i) * 2^(E(f / 32, i) - 127).  Per token and 32 consecutive features the exponent
+ * is the smallest with max|x| <= 127 * 2^e, not below the type's limit (-126; F16: -24), and Q is round(x / 2^e), ties to
+ * even -- at most half of 2^e off, except that the largest values of the type stop at 63 * 2^e where 64 * 2^e is no finite
+ * number of it (at most 2^e off).  Every stored value is exact in the type.  A block that holds an infinity or a NaN comes back as
+ * NaN throughout.
+ *
+ * eigamd_ckpt8_wgrad_dev is the weight gradient of Y = op(W) X from the checkpoint: dW = beta dW + dY X^T (opw N, m x k) or
+ * its transpose (opw T, k x m), in float; with beta = 0 dW is not read.  dtype is that of dY and of the matrix that was packed.
+ * d_work, limits and streams as above. */
+int eigamd_ckpt8_pack_dev(int dtype, int64_t k, int64_t n, const void* d_x, int64_t ldx, int8_t* d_q, int64_t ldq,
+                          uint8_t* d_exponents, int64_t lde, void* stream);
+int eigamd_ckpt8_unpack_dev(int dtype, int64_t k, int64_t n, const int8_t* d_q, int64_t ldq, const uint8_t* d_exponents, int64_t lde,
+                            void* d_x, int64_t ldx, void* stream);
+int64_t eigamd_ckpt8_wgrad_work_bytes(int dtype, int64_t m, int64_t n, int64_t k);
+int eigamd_ckpt8_wgrad_dev(int dtype, int opw, int64_t m, int64_t n, int64_t k, const void* d_dy, int64_t lddy, const int8_t* d_q,
+                           int64_t ldq, const uint8_t* d_exponents, int64_t lde, const float* beta, float* d_dw, int64_t lddw,
+                           void* d_work, int64_t work_bytes, void* stream);
 
 /* ---- misc --------------------------------------------------------------------- */
 const char* eigamd_last_error(void);  /* text of the last failure on this thread */
