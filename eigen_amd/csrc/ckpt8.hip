@@ -92,14 +92,7 @@ template <typename T> __global__ __launch_bounds__(256) void ckpt8_unpack_kernel
   if (!chunk_of(g, token, c)) return;
   const int n = g.k - c * 8;
   if (n <= 0) return;
-  const int8_t* from = g.q + token * g.ldq + c * 8;
-  uint64_t q = 0;
-  if (n >= 8) {
-    __builtin_memcpy(&q, from, 8);
-  } else {
-    for (int i = 0; i < 8; ++i)
-      if (i < n) q |= (uint64_t)(uint8_t)from[i] << (8 * i);
-  }
+  const uint64_t q = load_bytes(g.q + token * g.ldq + c * 8, n);
   const float scale = exponent_scale(g.e[token * g.lde + c / 4]);
   x8 v;
 #pragma unroll

@@ -93,6 +93,18 @@ template <typename E, typename V> __device__ __forceinline__ V load_up_to_8(cons
   return v;
 }
 
+// n <= 8 whole numbers of 8 bits from p (any alignment), the rest zero.
+__device__ __forceinline__ uint64_t load_bytes(const int8_t* p, int n) {
+  uint64_t v = 0;
+  if (n >= 8) {
+    __builtin_memcpy(&v, p, 8);
+  } else {
+    for (int i = 0; i < 8; ++i)
+      if (i < n) v |= (uint64_t)(uint8_t)p[i] << (8 * i);
+  }
+  return v;
+}
+
 // Which piece of which adapter workgroup-slot t stands for, when every adapter's run of the sorted batch is cut into pieces of
 // `size` tokens.  Adapter j's pieces take the slots from starts[j] / size + j on: the base of j + 1 is never below the base of
 // j plus j's pieces, so slots are unique without a prefix sum, and there are at most n / size + adapters + 1 of them.

@@ -8,6 +8,8 @@
 // LDS is filled in order of address (the direct loads can do nothing else), so bank conflicts are avoided by permuting
 // which 16-byte chunk of a line goes where: the lanes that read together then touch all 64 banks once.
 #pragma once
+#include <type_traits>
+
 #include "half.hpp"
 
 namespace eigamd {
@@ -44,19 +46,49 @@ struct HalfGemm {
 // 64 zero bytes that out-of-range chunks are loaded from.
 static __device__ __align__(64) unsigned char zero_page[64];
 
-// One operand's slice of R rows x 64 positions, loaded by NT threads in chunks of 8 elements; NT * N chunks in all.
-template <typename T, int LAY, int SRC, int R, int NT> struct SliceLoader {
-  static_assert(LAY == KC || R >= 128, "the permutation of a line needs 16 chunks");
+// Global memory to LDS without passing through registers: lane l's 16 bytes land at `to` + 16 l (`to` the same in every lane).
+// In assembly, because the compiler would wait for every such load before the next read of any LDS; it is waited for, with
+// everything else, in slice_barrier().  The second form takes a base that is the same in every lane.
+__device__ __forceinline__ void load_to_lds(const char* from, char* to) {
+  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)EIGAMD_LDS(char, to));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void load_to_lds(const char* base, unsigned off, char* to) {
+  const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)EIGAMD_LDS(char, to));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(base) : "memory", "m0");
+}
+// All of this wave's loads and LDS accesses are done, then those of the workgroup.
+__device__ __forceinline__ void slice_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x70);   // vmcnt(0) lgkmcnt(0), in a form the compiler's own counting sees
+  asm volatile("s_barrier" ::: "memory");
+}
+
+// One operand's slice of R rows x 64 positions, loaded by NT threads in chunks of 8 elements; NT * N chunks in all.  Slices are
+// taken one after the other: fetch() brings the next one into registers (nothing to do for DIRECT), commit() puts it into LDS.
+// Rows past the end are not cleared: whatever stands there meets only rows of C that are not stored.  Positions past the end of
+// the reduction are zero in both operands.
+// GATHER: row i is row order[i] of the matrix, and every chunk has an address of its own; otherwise they are 32-bit offsets from
+// a base that is the same in all lanes (256 rows or 64 lines of at most 2^22 elements).
+template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct SliceLoader {
+  static_assert(LAY == KC || (R >= 128 && !GATHER), "the permutation of a line needs 16 chunks");
   static constexpr int N = R * 8 / NT;
   static constexpr int bytes = R * 128;
+  static constexpr int es = SRC == QUANT ? 1 : 2;
+  static constexpr int NOFF = GATHER ? 1 : LAY == KC ? N : 1, NPTR = GATHER ? N : 1;
+  static constexpr int lines = NT / (R / 8);     // MC: lines from one chunk of a thread to the next
   using E = typename T::elem;
   using x8 = typename T::x8;
-  const char* ptr[N];      // this thread's chunks at position k0 = 0
-  int pos[N];              // KC: first position of the chunk inside the slice; MC: its line
-  int len[N];              // MC: elements of the chunk inside the matrix (0..8); KC: 8 inside, 0 outside
+  const char* base;        // first position of the next slice
   int64_t step;            // bytes from one slice to the next
-  const uint8_t* exps[N];
-  int64_t estep;
+  int64_t across;          // MC: bytes from one chunk of a thread to the next
+  unsigned off[NOFF];
+  const char* ptr[NPTR];
+  int len;                 // MC: elements of this thread's chunks inside the matrix (0..8)
+  int left;                // positions from the next slice's first to the end of the reduction
+  const uint8_t* ebase;
+  int64_t lde;
+  unsigned eoff;
   x8 reg[N];
   uint64_t qreg[N];
   unsigned ereg[N];
@@ -65,76 +97,125 @@ template <typename T, int LAY, int SRC, int R, int NT> struct SliceLoader {
     // KC: rows 0..7 of an 8-lane phase; MC: lines {0..3, 8..11} (+4, +16) of a half wave, 32 bytes each
     return LAY == KC ? (line & 7) : (((line & 3) | ((line >> 1) & 4)) << 1);
   }
+  // position inside the slice of chunk i: KC its first (the same for all i), MC its line
+  static __device__ __forceinline__ int position(int i) {
+    const int t = threadIdx.x;
+    return LAY == KC ? ((t % 8) ^ swizzle(t / 8)) * 8 : t / (R / 8) + i * lines;
+  }
 
-  __device__ __forceinline__ void init(const void* base, int64_t ld, int row0, int rows, int k0, const int* order, const uint8_t* e, int64_t lde) {
-    constexpr int es = SRC == QUANT ? 1 : 2;
+  __device__ __forceinline__ void init(const void* origin, int64_t ld, int row0, int rows, int k0, int count, const int* order,
+                                       const uint8_t* exponents, int64_t lde_) {
     step = (LAY == KC ? 64 : 64 * ld) * es;
-    estep = 64 * lde;
+    left = count;
+    base = static_cast<const char*>(origin);
+    if constexpr (LAY == KC) {
+      base += ((GATHER ? 0 : row0 * ld) + k0) * es;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int ch = threadIdx.x + i * NT;
-      if constexpr (LAY == KC) {
-        const int line = ch / 8, c = (ch % 8) ^ swizzle(line);
-        int row = row0 + line;
-        len[i] = row < rows ? 8 : 0;
-        row = row < rows ? row : rows - 1;
-        const int64_t at = order ? order[row] : row;
-        pos[i] = c * 8;
-        ptr[i] = static_cast<const char*>(base) + (at * ld + k0 + c * 8) * es;
-      } else {
-        const int line = ch / (R / 8), c = (ch % (R / 8)) ^ swizzle(line);
-        const int row = row0 + c * 8;
-        len[i] = rows - row < 0 ? 0 : (rows - row < 8 ? rows - row : 8);
-        pos[i] = line;
-        ptr[i] = static_cast<const char*>(base) + ((int64_t)(k0 + line) * ld + row) * es;
-        if constexpr (SRC == QUANT) exps[i] = e + (int64_t)(k0 + line) * lde + row / 32;
+      for (int i = 0; i < N; ++i) {
+        const int line = threadIdx.x / 8 + i * (NT / 8);
+        const int in = row0 + line < rows ? line : rows - 1 - row0;
+        if constexpr (GATHER) ptr[i] = base + ((int64_t)order[row0 + in] * ld + position(0)) * es;
+        else off[i] = (unsigned)((in * ld + position(0)) * es);
+      }
+    } else {
+      const int line = position(0), c = (threadIdx.x % (R / 8)) ^ swizzle(line);
+      const int row = row0 + c * 8;
+      len = rows - row < 0 ? 0 : (rows - row < 8 ? rows - row : 8);
+      base += (k0 * ld + row0) * es;
+      across = lines * ld * es;
+      off[0] = (unsigned)((line * ld + (len ? c * 8 : 0)) * es);
+      if constexpr (SRC == QUANT) {
+        lde = lde_;
+        ebase = exponents + (int64_t)k0 * lde + row0 / 32;
+        eoff = (unsigned)(line * lde + (len ? c / 4 : 0));
       }
     }
   }
-
-  // Chunks of the slice `s` slices further on, of which `left` positions are inside the reduction.
-  __device__ __forceinline__ void load(char* lds, int s, int left) {
+  __device__ __forceinline__ const char* at(int i) const {
+    if constexpr (GATHER) return ptr[i];
+    else return LAY == KC ? base + off[i] : base + i * across + off[0];
+  }
+  __device__ __forceinline__ const uint8_t* exponent_at(int i) const { return ebase + i * (lines * lde) + eoff; }
+  __device__ __forceinline__ int inside(int i) const { return LAY == KC ? left - position(0) : (position(i) < left ? len : 0); }
+  __device__ __forceinline__ void next() {
+    left -= 64;
+    base += step;
+    if constexpr (GATHER) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const char* q = ptr[i] + (int64_t)s * step;
-      const int n = LAY == KC ? (len[i] ? left - pos[i] : 0) : (pos[i] < left ? len[i] : 0);
-      if constexpr (SRC == DIRECT) {
-        // whole chunks only (the launcher checks extents); outside: zeros
-        const char* from = n > 0 ? q : reinterpret_cast<const char*>(zero_page);
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-        char* to = lds + (i * NT + wave * 64) * 16;
-        __builtin_amdgcn_global_load_lds(EIGAMD_GLOBAL(from), EIGAMD_LDS(void, to), 16, 0, 0);
-      } else if constexpr (SRC == STAGED) {
-        reg[i] = load_up_to_8<E, x8>(reinterpret_cast<const E*>(q), n);
-      } else {
-        uint64_t v = 0;
-        if (n >= 8) {
-          __builtin_memcpy(&v, q, 8);
-        } else {
-          for (int t = 0; t < 8; ++t)
-            if (t < n) v |= (uint64_t)(uint8_t)q[t] << (8 * t);
+      for (int i = 0; i < N; ++i) ptr[i] += step;
+    }
+    if constexpr (SRC == QUANT) ebase += 64 * lde;
+  }
+
+  __device__ __forceinline__ void fetch() {
+    if constexpr (SRC != DIRECT) {
+      if (left <= 0) return;
+      if (left >= 72) {
+        // Whole loads.  Past the end of a column they run into the next one (there are at least 8 more elements of columns
+        // behind this slice), and what they bring belongs to rows that are not stored.
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if constexpr (SRC == STAGED) {
+            reg[i] = load_8<E, x8>(reinterpret_cast<const E*>(at(i)));
+          } else {
+            __builtin_memcpy(&qreg[i], at(i), 8);
+            ereg[i] = *exponent_at(i);
+          }
         }
-        qreg[i] = v;
-        ereg[i] = n > 0 ? exps[i][(int64_t)s * estep] : 0u;
+      } else {
+        // element by element, those outside from the zero page
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int n = inside(i);
+          if constexpr (SRC == STAGED) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) reg[i][t] = *(t < n ? reinterpret_cast<const E*>(at(i)) + t : reinterpret_cast<const E*>(zero_page));
+          } else {
+            qreg[i] = 0;
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+              qreg[i] |= (uint64_t)*(t < n ? reinterpret_cast<const uint8_t*>(at(i)) + t : reinterpret_cast<const uint8_t*>(zero_page)) << (8 * t);
+            ereg[i] = *(n > 0 ? exponent_at(i) : reinterpret_cast<const uint8_t*>(zero_page));
+          }
+        }
       }
+      next();
     }
   }
 
-  // Second half of a load through registers.
-  __device__ __forceinline__ void store(char* lds) {
-    if constexpr (SRC == DIRECT) return;
+  __device__ __forceinline__ void commit(char* lds) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    if constexpr (SRC == DIRECT) {
+      if (left <= 0) return;
+      char* to = lds + wave * 1024;
+      if (left >= 64) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      x8 v;
-      if constexpr (SRC == STAGED) {
-        v = reg[i];
+        for (int i = 0; i < N; ++i) {
+          if constexpr (GATHER) load_to_lds(ptr[i], to + i * NT * 16);
+          else if constexpr (LAY == KC) load_to_lds(base, off[i], to + i * NT * 16);
+          else load_to_lds(base + i * across, off[0], to + i * NT * 16);
+        }
       } else {
-        // |q| <= 127 has 7 bits, so q * 2^e is exact in either type (the exponent is kept in the type's range by the packing)
-        const float sc = exponent_scale(ereg[i]);
+        // whole chunks only (the launcher checks extents); those outside: zeros
 #pragma unroll
-        for (int t = 0; t < 8; ++t) v[t] = (E)((float)(int8_t)(qreg[i] >> (8 * t)) * sc);
+        for (int i = 0; i < N; ++i)
+          load_to_lds((LAY == KC ? position(0) : position(i)) < left ? at(i) : reinterpret_cast<const char*>(zero_page), to + i * NT * 16);
       }
-      *reinterpret_cast<x8*>(lds + (threadIdx.x + i * NT) * 16) = v;
+      next();
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        x8 v;
+        if constexpr (SRC == STAGED) {
+          v = reg[i];
+        } else {
+          // |q| <= 127 has 7 bits, so q * 2^e is exact in either type (the packing keeps the exponent in the type's range)
+          const float sc = exponent_scale(ereg[i]);
+#pragma unroll
+          for (int t = 0; t < 8; ++t) v[t] = (E)((float)(int8_t)(qreg[i] >> (8 * t)) * sc);
+        }
+        *reinterpret_cast<x8*>(lds + (threadIdx.x + i * NT) * 16) = v;
+      }
     }
   }
 
@@ -260,8 +341,8 @@ enum { OUT_HALF = 0, OUT_F32 = 1, OUT_F32_SWAPPED = 2 };
 template <typename T, int LA, int SA, int LB, int SB, int OUT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
   constexpr int NT = WM * WN * 64, TM = BM / WM, TN = BN / WN, NI = TM / 16, NJ = TN / 16;
-  using LoadA = SliceLoader<T, LA, SA, BM, NT>;
-  using LoadB = SliceLoader<T, LB, SB, BN, NT>;
+  using LoadA = SliceLoader<T, LA, SA, BM, NT, false>;
+  using LoadB = SliceLoader<T, LB, SB, BN, NT, OUT == OUT_HALF>;
   constexpr int slice = LoadA::bytes + LoadB::bytes;
   __shared__ __align__(1024) char lds[2 * slice];
   const int tiles_m = (g.m + BM - 1) / BM, tiles_n = (g.n + BN - 1) / BN;
@@ -275,48 +356,86 @@ __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
 
   LoadA la;
   LoadB lb;
-  la.init(g.a, g.lda, tm * BM, g.m, k_begin, nullptr, g.exponents, g.lde);
-  lb.init(g.b, g.ldb, tn * BN, g.n, k_begin, g.order, g.exponents, g.lde);
+  la.init(g.a, g.lda, tm * BM, g.m, k_begin, k_count, nullptr, g.exponents, g.lde);
+  lb.init(g.b, g.ldb, tn * BN, g.n, k_begin, k_count, g.order, g.exponents, g.lde);
   f32x4 acc[NI][NJ] = {};
-  if (slices > 0) {
-    la.load(lds, 0, k_count);
-    lb.load(lds + LoadA::bytes, 0, k_count);
+  // Two slices in LDS.  Each half of a slice (32 positions) is multiplied in two steps, the upper and the lower half of this wave's
+  // rows; while one step's products run, the fragments of the next are read.  A slice's buffer is free once its last fragments are
+  // in registers: from the barrier in front of slice s's last step on, slice s + 2 is on its way there, and has to have arrived at
+  // the next slice's barrier.
+#pragma unroll 1
+  for (int z = 0; z < 2; ++z) {
+    la.fetch();
+    lb.fetch();
+    la.commit(lds + z * slice);
+    lb.commit(lds + z * slice + LoadA::bytes);
   }
+  la.fetch();
+  lb.fetch();
   if constexpr (OUT == OUT_HALF) {
     if (g.rank > 0 && blockIdx.y == 0) add_adapters<T, NI, NJ>(g, tm * BM + wr, tn * BN + wc, acc);
   }
-  if (slices > 0) {
-    la.store(lds);
-    lb.store(lds + LoadA::bytes);
-  }
-  __syncthreads();
+  slice_barrier();
+  constexpr int NH = NI / 2, RA = LA == KC ? 1 : 2, RB = LB == KC ? 1 : 2;
+  typename T::x8 fa[2][NH], fb[2][NJ];
+  auto read_a = [&](const char* from, int half, int kk) {
+#pragma unroll
+    for (int i = 0; i < NH; ++i) fa[half][i] = LoadA::fragment(from, wr + (half * NH + i) * 16, kk);
+  };
+  auto read_b = [&](const char* from, int set, int kk) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) fb[set][j] = LoadB::fragment(from + LoadA::bytes, wc + j * 16, kk);
+  };
+  auto multiply = [&](int half, int set) {
+#pragma unroll
+    for (int i = 0; i < NH; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        f32x4& c = acc[half * NH + i][j];
+        c = OUT == OUT_F32_SWAPPED ? T::mma(fb[set][j], fa[half][i], c) : T::mma(fa[half][i], fb[set][j], c);
+      }
+  };
+  // The compiler would put each read right in front of the product that needs it; here every read of the next step is followed
+  // by products of this one.
+  constexpr int products = NH * NJ;
+  auto interleave = [&](auto count) {
+    constexpr int reads = decltype(count)::value;
+#pragma unroll
+    for (int q = 0; q < reads; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, products / reads, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, products % reads, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  using ReadsA = std::integral_constant<int, NH * RA>;
+  using ReadsAB = std::integral_constant<int, NH * RA + NJ * RB>;
+  read_a(lds, 0, 0);
+  read_b(lds, 0, 0);
   for (int s = 0; s < slices; ++s) {
     char* here = lds + (s & 1) * slice;
-    char* next = lds + ((s & 1) ^ 1) * slice;
-    const bool more = s + 1 < slices;
-    if (more) {
-      la.load(next, s + 1, k_count - (s + 1) * 64);
-      lb.load(next + LoadA::bytes, s + 1, k_count - (s + 1) * 64);
-    }
-#pragma unroll
-    for (int kk = 0; kk < 64; kk += 32) {
-      typename T::x8 fa[NI], fb[NJ];
-#pragma unroll
-      for (int i = 0; i < NI; ++i) fa[i] = LoadA::fragment(here, wr + i * 16, kk);
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) fb[j] = LoadB::fragment(here + LoadA::bytes, wc + j * 16, kk);
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-          acc[i][j] = OUT == OUT_F32_SWAPPED ? T::mma(fb[j], fa[i], acc[i][j]) : T::mma(fa[i], fb[j], acc[i][j]);
-    }
-    if (more) {
-      la.store(next);
-      lb.store(next + LoadA::bytes);
-    }
-    __syncthreads();
+    char* other = lds + ((s & 1) ^ 1) * slice;
+    read_a(here, 1, 0);
+    multiply(0, 0);
+    interleave(ReadsA{});
+    read_a(here, 0, 32);
+    read_b(here, 1, 32);
+    multiply(1, 0);
+    interleave(ReadsAB{});
+    read_a(here, 1, 32);
+    multiply(0, 1);
+    interleave(ReadsA{});
+    slice_barrier();
+    la.commit(here);
+    lb.commit(here + LoadA::bytes);
+    la.fetch();
+    lb.fetch();
+    read_a(other, 0, 0);     // (behind the last slice: what was there before, not used)
+    read_b(other, 0, 0);
+    multiply(1, 1);
+    interleave(ReadsAB{});
   }
+  slice_barrier();
 
   const int row0 = tm * BM + wr, col0 = tn * BN + wc;
   if (g.splits > 1) {

@@ -339,14 +339,7 @@ template <typename T, int SRC> struct GradTile {
       } else if constexpr (SRC == STAGED) {
         reg[i] = load_up_to_8<E, x8>(static_cast<const E*>(g.u) + (int64_t)t * g.ldu + row, n);
       } else {
-        const int8_t* q = static_cast<const int8_t*>(g.u) + (int64_t)t * g.ldu + row;
-        uint64_t v = 0;
-        if (n >= 8) {
-          __builtin_memcpy(&v, q, 8);
-        } else {
-          for (int e = 0; e < 8; ++e)
-            if (e < n) v |= (uint64_t)(uint8_t)q[e] << (8 * e);
-        }
+        const uint64_t v = load_bytes(static_cast<const int8_t*>(g.u) + (int64_t)t * g.ldu + row, n);
         const float sc = exponent_scale(n > 0 ? g.exponents[(int64_t)t * g.lde + row / 32] : 0u);
 #pragma unroll
         for (int e = 0; e < 8; ++e) reg[i][e] = (E)((float)(int8_t)(v >> (8 * e)) * sc);
