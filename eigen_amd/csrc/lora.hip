@@ -60,55 +60,109 @@ struct ProjectArgs {
   float* p; int64_t ldp;
 };
 
-// P for up to 32 tokens of one adapter and 16 RT ranks.  Eight waves share the reduction, each straight from memory to the
-// matrix unit: a lane reads 32 consecutive positions of its token (64 bytes), so the order of the reduction is permuted the
-// same way for both operands.
-template <typename T, int RT> __global__ __launch_bounds__(512) void lora_project_kernel(ProjectArgs g) {
+// P for up to 32 tokens of one adapter and 16 RT ranks.  Eight waves share the reduction, 128 (64) positions a turn, each straight
+// from memory to the matrix unit: one load of a wave is 64 bytes of each of 16 tokens.  The next turn's loads are under way
+// while this one's are multiplied.
+//   A_K   the factor's reduction is contiguous: loaded like the tokens
+//   A_R   its ranks are (the backward pass): whole 16-byte chunks of ranks go through this wave's own LDS and come back
+//         transposed; one element at a time instead, the loads of a 64-rank factor took four times the rest (57 us of 4096 tokens
+//         x 4096, now 18)
+//   A_ANY element by element: ranks that are no multiple of 8, odd strides
+enum { A_K, A_R, A_ANY };
+template <typename T, int RT, int FORM> __global__ __launch_bounds__(512) void lora_project_kernel(ProjectArgs g) {
   using E = typename T::elem;
   using x8 = typename T::x8;
   Piece piece;
   if (!find_piece(g.starts, g.none + 1, kProjTokens, blockIdx.x, piece)) return;
   const int w = threadIdx.x / 64, l = threadIdx.x & 63, r0 = blockIdx.y * 64;
-  __shared__ f32x4 red[8][RT][2][64];
+  constexpr int line = RT * 32, turned_bytes = FORM == A_R ? 8 * 32 * line : 0;     // A_R: 32 positions x 16 RT ranks per wave
+  constexpr int red_bytes = 8 * RT * 2 * 64 * 16;
+  __shared__ __align__(1024) char lds[red_bytes > turned_bytes ? red_bytes : turned_bytes];
+  f32x4(&red)[8][RT][2][64] = *reinterpret_cast<f32x4(*)[8][RT][2][64]>(lds);
   const bool live = piece.adapter != g.none;
   if (live) {
     // lanes past the piece or the rank repeat the last one; what they compute is not stored
     f32x4 acc[RT][2] = {};
     const E* x[2];
     const E* a[RT];
+    const E* factor = static_cast<const E*>(g.a) + (int64_t)piece.adapter * g.a_stride;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int at = piece.begin + c * 16 + (l & 15);
       x[c] = static_cast<const E*>(g.x) + (int64_t)g.order[at < piece.end ? at : piece.end - 1] * g.ldx;
     }
+    constexpr int per = RT * 2;                              // A_R: 16-byte chunks of a line
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const int r = r0 + t * 16 + (l & 15);
-      a[t] = static_cast<const E*>(g.a) + (int64_t)piece.adapter * g.a_stride + (int64_t)(r < g.rank ? r : g.rank - 1) * g.a_row;
+      if constexpr (FORM == A_R) {
+        // chunk t * 64 + l of 32 lines
+        const int ch = t * 64 + l, r = r0 + (ch % per) * 8;
+        a[t] = factor + (int64_t)(ch / per) * g.a_k + (r < g.rank ? r : 0);
+      } else {
+        const int r = r0 + t * 16 + (l & 15);
+        a[t] = factor + (int64_t)(r < g.rank ? r : g.rank - 1) * g.a_row;
+      }
     }
-    for (int k0 = w * 128; k0 < g.k; k0 += 8 * 128) {
-      const bool whole = k0 + 128 <= g.k;
+    constexpr int S = RT == 4 ? 2 : 4, turn = 8 * 32 * S;      // products of a turn; positions all waves take in one
+    x8 fx[2][S][2], fa[2][S][RT];
+    auto load = [&](int k0, int set) {
+      const bool whole = k0 + 32 * S <= g.k;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int k = k0 + (l / 16) * 32 + s * 8, left = whole ? 8 : g.k - k;
-        x8 fx[2], fa[RT];
+      for (int s = 0; s < S; ++s) {
+        const int k = k0 + s * 32 + (l / 16) * 8, left = g.k - k;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) fx[c] = whole ? load_8<E, x8>(x[c] + k) : load_up_to_8<E, x8>(x[c] + k, left);
+        for (int c = 0; c < 2; ++c) fx[set][s][c] = whole ? load_8<E, x8>(x[c] + k) : load_up_to_8<E, x8>(x[c] + k, left);
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          if (g.a_k == 1) {
-            fa[t] = whole ? load_8<E, x8>(a[t] + k) : load_up_to_8<E, x8>(a[t] + k, left);
+          if constexpr (FORM == A_K) {
+            fa[set][s][t] = whole ? load_8<E, x8>(a[t] + k) : load_up_to_8<E, x8>(a[t] + k, left);
+          } else if constexpr (FORM == A_R) {
+            const int at = k0 + s * 32 + (t * 64 + l) / per;
+            fa[set][s][t] = load_up_to_8<E, x8>(a[t] + (int64_t)(k0 + s * 32) * g.a_k, at < g.k ? 8 : 0);
           } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) fa[t][e] = e < left ? a[t][(int64_t)(k + e) * g.a_k] : (E)0.0f;
+            for (int e = 0; e < 8; ++e) fa[set][s][t][e] = e < left ? a[t][(int64_t)(k + e) * g.a_k] : (E)0.0f;
           }
+        }
+      }
+    };
+    auto multiply = [&](int set) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        x8 f[RT];
+        if constexpr (FORM == A_R) {
+          char* mine = lds + w * 32 * line;
+          auto slot = [&](int ln, int ch) { return ln * line + ((ch ^ ((ln & 3) << 1)) & (per - 1)) * 16; };
+#pragma unroll
+          for (int t = 0; t < RT; ++t) *reinterpret_cast<x8*>(mine + slot((t * 64 + l) / per, (t * 64 + l) % per)) = fa[set][s][t];
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            union { x8 v; typename T::x4 h[2]; } u;
+            const int ln = (l / 16) * 8 + (l & 15) / 4, ch = t * 2 + (l & 3) / 2;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) u.h[h] = T::read_transposed(mine + slot(ln + 4 * h, ch) + (l & 1) * 8);
+            f[t] = u.v;
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < RT; ++t) f[t] = fa[set][s][t];
         }
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) acc[t][c] = T::mma(fa[t], fx[c], acc[t][c]);
+          for (int c = 0; c < 2; ++c) acc[t][c] = T::mma(f[t], fx[set][s][c], acc[t][c]);
       }
+    };
+    int k0 = w * 32 * S;
+    if (k0 < g.k) load(k0, 0);
+    for (; k0 < g.k; k0 += 2 * turn) {
+      if (k0 + turn < g.k) load(k0 + turn, 1);
+      multiply(0);
+      if (k0 + turn >= g.k) break;
+      if (k0 + 2 * turn < g.k) load(k0 + 2 * turn, 0);
+      multiply(1);
     }
+    if constexpr (FORM == A_R) __syncthreads();              // (the same LDS; `live` is the workgroup's)
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -128,12 +182,21 @@ template <typename T, int RT> __global__ __launch_bounds__(512) void lora_projec
   }
 }
 
-template <typename T> hipError_t launch_project(const ProjectArgs& g, hipStream_t s) {
+template <typename T, int RT> hipError_t launch_project_rank(const ProjectArgs& g, hipStream_t s) {
   const dim3 grid(g.n / kProjTokens + g.none + 1, (g.rank + 63) / 64);
-  if (g.rank <= 16) hipLaunchKernelGGL((lora_project_kernel<T, 1>), grid, dim3(512), 0, s, g);
-  else if (g.rank <= 32) hipLaunchKernelGGL((lora_project_kernel<T, 2>), grid, dim3(512), 0, s, g);
-  else hipLaunchKernelGGL((lora_project_kernel<T, 4>), grid, dim3(512), 0, s, g);
+  bool turned = false;
+  if constexpr (T::bytes == 2) {
+    turned = g.a_row == 1 && g.a_k % 8 == 0 && g.rank % 8 == 0 && g.a_stride % 8 == 0 && (uintptr_t)g.a % 16 == 0;
+    if (g.a_k != 1 && turned) hipLaunchKernelGGL((lora_project_kernel<T, RT, A_R>), grid, dim3(512), 0, s, g);
+  }
+  if (g.a_k == 1) hipLaunchKernelGGL((lora_project_kernel<T, RT, A_K>), grid, dim3(512), 0, s, g);
+  else if (!turned) hipLaunchKernelGGL((lora_project_kernel<T, RT, A_ANY>), grid, dim3(512), 0, s, g);
   return hipGetLastError();
+}
+template <typename T> hipError_t launch_project(const ProjectArgs& g, hipStream_t s) {
+  if (g.rank <= 16) return launch_project_rank<T, 1>(g, s);
+  if (g.rank <= 32) return launch_project_rank<T, 2>(g, s);
+  return launch_project_rank<T, 4>(g, s);
 }
 
 // ------------------------------------------------------------------------------------------------------ few tokens (KC)
@@ -152,40 +215,76 @@ template <typename T, int NG> __global__ __launch_bounds__(512) void lora_few_ke
     b[c] = static_cast<const E*>(g.b) + (int64_t)g.order[at < g.n ? at : g.n - 1] * g.ldb;
   }
   f32x4 acc[NG] = {};
-  for (int k0 = w * 128; k0 < g.k; k0 += 8 * 128) {
-    x8 fa[4], fb[4][NG];
+  x8 fa[2][4], fb[2][4][NG];
+  auto load = [&](int k0, int set) {
     const bool whole = k0 + 128 <= g.k;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const int k = k0 + (l / 16) * 32 + s * 8, left = g.k - k;
-      fa[s] = whole ? load_8<E, x8>(a + k) : load_up_to_8<E, x8>(a + k, left);
+      const int k = k0 + s * 32 + (l / 16) * 8, left = g.k - k;
+      fa[set][s] = whole ? load_8<E, x8>(a + k) : load_up_to_8<E, x8>(a + k, left);
 #pragma unroll
-      for (int c = 0; c < NG; ++c) fb[s][c] = whole ? load_8<E, x8>(b[c] + k) : load_up_to_8<E, x8>(b[c] + k, left);
+      for (int c = 0; c < NG; ++c) fb[set][s][c] = whole ? load_8<E, x8>(b[c] + k) : load_up_to_8<E, x8>(b[c] + k, left);
     }
+  };
+  auto multiply = [&](int set) {
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int c = 0; c < NG; ++c) acc[c] = T::mma(fa[s], fb[s][c], acc[c]);
+      for (int c = 0; c < NG; ++c) acc[c] = T::mma(fa[set][s], fb[set][s][c], acc[c]);
+  };
+  int k0 = w * 128;
+  if (k0 < g.k) load(k0, 0);
+  // The low-rank part of this thread's outputs (256 NG of them, one row of a token each; 16 rows are 16 neighbouring threads),
+  // while the first loads of W are under way.
+  constexpr int NOUT = (256 * NG + 511) / 512;
+  float extra[NOUT];
+  int64_t at[NOUT];
+#pragma unroll
+  for (int q = 0; q < NOUT; ++q) {
+    const int r = row0 + threadIdx.x % 16, col = threadIdx.x / 16 + q * 32;
+    at[q] = -1;
+    extra[q] = 0.0f;
+    if (col >= g.n || r >= g.m) continue;
+    const int token = g.order[col], who = g.seg[col];
+    at[q] = token * g.ldc + r;
+    if (who == g.none || g.rank == 0) continue;
+    using f32x8 = float __attribute__((ext_vector_type(8)));
+    const E* up = static_cast<const E*>(g.up) + (int64_t)who * g.up_stride + (int64_t)r * g.up_row;
+    const float* p = g.p + token * g.ldp;
+    float d = 0.0f;
+    for (int t = 0; t < g.rank; t += 8) {
+      const f32x8 pv = load_up_to_8<float, f32x8>(p + t, g.rank - t);
+      x8 u;
+      if (g.up_rank == 1) {
+        u = load_up_to_8<E, x8>(up + t, g.rank - t);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = t + e < g.rank ? up[(int64_t)(t + e) * g.up_rank] : (E)0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d += (float)u[e] * pv[e];
+    }
+    extra[q] = g.scale[who] * d;
+  }
+  for (; k0 < g.k; k0 += 2 * 1024) {
+    if (k0 + 1024 < g.k) load(k0 + 1024, 1);
+    multiply(0);
+    if (k0 + 1024 >= g.k) break;
+    if (k0 + 2048 < g.k) load(k0 + 2048, 0);
+    multiply(1);
   }
   __shared__ f32x4 red[8][NG][64];
 #pragma unroll
   for (int c = 0; c < NG; ++c) red[w][c][l] = acc[c];
   __syncthreads();
-  // one output per thread and turn: 16 rows of a token are 16 neighbouring threads
-  for (int q = threadIdx.x; q < 256 * NG; q += 512) {
-    const int r = q % 16, col = q / 16;
-    if (col >= g.n || row0 + r >= g.m) continue;
+#pragma unroll
+  for (int q = 0; q < NOUT; ++q) {
+    if (at[q] < 0) continue;
+    const int r = threadIdx.x % 16, col = threadIdx.x / 16 + q * 32;
     float sum = 0.0f;
+#pragma unroll
     for (int z = 0; z < 8; ++z) sum += red[z][col / 16][(r / 4) * 16 + col % 16][r % 4];
-    const int token = g.order[col], who = g.seg[col];
-    if (who != g.none && g.rank > 0) {
-      const E* up = static_cast<const E*>(g.up) + (int64_t)who * g.up_stride + (int64_t)(row0 + r) * g.up_row;
-      const float* p = g.p + (int64_t)token * g.ldp;
-      float d = 0.0f;
-      for (int t = 0; t < g.rank; ++t) d += (float)up[(int64_t)t * g.up_rank] * p[t];
-      sum += g.scale[who] * d;
-    }
-    static_cast<E*>(g.c)[(int64_t)token * g.ldc + row0 + r] = (E)sum;
+    static_cast<E*>(g.c)[at[q]] = (E)(sum + extra[q]);
   }
 }
 
@@ -402,45 +501,41 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
     nm = norm_of(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
   }
   Tile tile;
-  f32x4 acc[4][RT] = {};
+  // RT waves beside each other take 16 ranks each (every wave then makes the pieces of its own p only), 4 / RT one behind the
+  // other 64 RT rows each
+  constexpr int NI = 4 * RT;
+  const int wr = (w / RT) * 64 * RT, r = r0 + (w % RT) * 16 + (l & 15);
+  f32x4 acc[NI] = {};
   tile.load(lds, g, tok, row0);
   tile.store(lds);
   __syncthreads();
   for (int s = 0; s < turns; ++s) {
     char* here = lds + (s & 1) * Tile::bytes;
     char* next = lds + ((s & 1) ^ 1) * Tile::bytes;
-    float pv[RT][8];
+    float pv[8];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int r = r0 + t * 16 + (l & 15);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int token = tok[s * 32 + (l / 16) * 8 + e];
-        pv[t][e] = token >= 0 && r < g.rank ? g.p[(int64_t)token * g.ldp + r] : 0.0f;
-      }
+    for (int e = 0; e < 8; ++e) {
+      const int token = tok[s * 32 + (l / 16) * 8 + e];
+      pv[e] = token >= 0 && r < g.rank ? g.p[(int64_t)token * g.ldp + r] : 0.0f;
     }
     if (s + 1 < turns) tile.load(next, g, tok + (s + 1) * 32, row0);
-    x8 fu[4];
+    x8 fp[NP];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) fu[i] = Tile::fragment(here, w * 64 + i * 16);
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (NP == 1) {
+        fp[0][e] = pv[e];
+      } else {
+        E q[NP];
+        split<T, NP>(pv[e] * nm.down, q);
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      x8 fp[NP];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (NP == 1) {
-          fp[0][e] = pv[t][e];
-        } else {
-          E q[NP];
-          split<T, NP>(pv[t][e] * nm.down, q);
-#pragma unroll
-          for (int z = 0; z < NP; ++z) fp[z][e] = q[z];
-        }
+        for (int z = 0; z < NP; ++z) fp[z][e] = q[z];
       }
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NI; ++i) {
+      const x8 fu = Tile::fragment(here, wr + i * 16);
 #pragma unroll
-        for (int z = NP - 1; z >= 0; --z) acc[i][t] = TRANS ? T::mma(fp[z], fu[i], acc[i][t]) : T::mma(fu[i], fp[z], acc[i][t]);
+      for (int z = NP - 1; z >= 0; --z) acc[i] = TRANS ? T::mma(fp[z], fu, acc[i]) : T::mma(fu, fp[z], acc[i]);
     }
     if (s + 1 < turns) tile.store(next);
     __syncthreads();
@@ -451,16 +546,14 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
   const int64_t ld = whole ? g.ldg : (TRANS ? g.rank : g.rows);
   const float beta = whole ? g.beta : 0.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int fast = TRANS ? r0 + t * 16 + (l / 16) * 4 : row0 + w * 64 + i * 16 + (l / 16) * 4;
-      const int slow = TRANS ? row0 + w * 64 + i * 16 + (l & 15) : r0 + t * 16 + (l & 15);
-      if (slow >= (TRANS ? g.rows : g.rank)) continue;
-      float* at = out + (int64_t)slow * ld + fast;
-      for (int e = 0; e < 4; ++e)
-        if (fast + e < (TRANS ? g.rank : g.rows)) at[e] = acc[i][t][e] * nm.up * sj + (beta != 0.0f ? beta * at[e] : 0.0f);
-    }
+  for (int i = 0; i < NI; ++i) {
+    const int rank0 = r0 + (w % RT) * 16, top = row0 + wr + i * 16;
+    const int fast = (TRANS ? rank0 : top) + (l / 16) * 4, slow = (TRANS ? top : rank0) + (l & 15);
+    if (slow >= (TRANS ? g.rows : g.rank)) continue;
+    float* at = out + (int64_t)slow * ld + fast;
+    for (int e = 0; e < 4; ++e)
+      if (fast + e < (TRANS ? g.rank : g.rows)) at[e] = acc[i][e] * nm.up * sj + (beta != 0.0f ? beta * at[e] : 0.0f);
+  }
 }
 
 // G_j = beta G_j + s_j (sum of j's pieces, in the order of the batch); an adapter without tokens gets beta G_j.
@@ -472,7 +565,15 @@ __global__ __launch_bounds__(256) void lora_grad_join_kernel(GradArgs g) {
   const int fast = g.trans ? g.rank : g.rows;
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < size; q += (int64_t)gridDim.x * 256) {
     float sum = 0.0f;
-    for (int z = 0; z < pieces; ++z) sum += g.partial[(int64_t)(slot + z) * size + q];
+    int z = 0;
+    for (; z + 8 <= pieces; z += 8) {      // eight loads at a time under way, added in order
+      float v[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] = g.partial[(int64_t)(slot + z + t) * size + q];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) sum += v[t];
+    }
+    for (; z < pieces; ++z) sum += g.partial[(int64_t)(slot + z) * size + q];
     const int64_t slow = q / fast;
     float* at = g.g + (int64_t)j * g.stride_g + slow * g.ldg + (q - slow * fast);
     *at = (pieces ? g.scale[j] * sum : 0.0f) + (g.beta != 0.0f ? g.beta * *at : 0.0f);

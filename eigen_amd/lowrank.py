@@ -3,15 +3,13 @@ device-resident matrices (``eigamd_lora_*``, ``eigamd_ckpt8_*`` of ``include/eig
 
 Column-major, one token per column: a torch tensor of shape (tokens, features) is ``DeviceMatrix(features, tokens)`` on the
 same storage.  Every call is asynchronous on ``stream`` (default: torch's current stream of the operands' device)."""
-import contextlib
 import ctypes
 
-import numpy as np
 import torch
 
 from . import _lib
 from ._lib import lib
-from .device import DeviceMatrix, _OPCODE, _TORCH_OF_KIND
+from .device import DeviceMatrix, _TORCH_OF_KIND
 
 _KINDS = (_lib.F32, _lib.BF16, _lib.F16)
 
@@ -79,68 +77,71 @@ def _holds(storage, offset, ld, rows, cols, what):
         raise ValueError(f"{what}: the storage is too small for the matrix")
 
 
-def _check_matrix(m, kind, rows, cols, what):
+def _check_matrix(m, kind, rows, cols, what, count=1):
     if m.kind != kind:
         raise ValueError(f"{what} has the wrong scalar kind")
-    if (m.rows, m.cols) != (rows, cols):
+    if m.rows != rows or m.cols != cols:
         raise ValueError(f"{what} is {m.rows} x {m.cols}, expected {rows} x {cols}")
-    if m.storage.dtype != _TORCH_OF_KIND[kind] or not m.storage.is_contiguous():
+    storage = m.storage
+    if storage.dtype is not _TORCH_OF_KIND[kind] or not storage.is_contiguous():
         raise ValueError(f"{what}: the storage must be a contiguous tensor of the matrix's type")
-    _holds(m.storage, m.offset, m.ld, rows, cols, what)
+    _holds(storage, m.offset + (count - 1) * m.stride if count > 1 else m.offset, m.ld, rows, cols, what)
 
 
 def _check_stack(m, kind, rows, cols, count, what):
     if m.count != count:
         raise ValueError(f"{what} has {m.count} matrices, expected {count}")
-    _check_matrix(m, kind, rows, cols, what)
     if count:
-        _holds(m.storage, m.offset + (count - 1) * m.stride, m.ld, rows, cols, what)
+        _check_matrix(m, kind, rows, cols, what, count)
 
 
 def _check_vector(v, n, dtype, what):
-    if v.dtype != dtype or v.numel() != n or not v.is_contiguous():
+    if v.dtype is not dtype or v.numel() != n or not v.is_contiguous():
         raise ValueError(f"{what} must be {n} contiguous elements of {dtype}")
 
 
+_OPS = {"N": _lib.OP_N, "T": _lib.OP_T, "n": _lib.OP_N, "t": _lib.OP_T}
+
+
 def _op(op):
-    op = op.upper()
-    if op not in ("N", "T"):
+    code = _OPS.get(op)
+    if code is None:
         raise ValueError("op must be 'N' or 'T'")
-    return _OPCODE[op]
+    return code
 
 
 def _turned(op, rows, cols):
     return (cols, rows) if op == _lib.OP_T else (rows, cols)
 
 
-@contextlib.contextmanager
-def _on(stream, *tensors):
-    """The operands' device as the current one, and the stream (torch's current one there by default) with its handle."""
-    device = tensors[0].device
-    if device.type != "cuda":
+def _run(entry, stream, tensors, need, work, call):
+    """call(stream handle, address of the scratch memory, its bytes) with the operands' device as the current one; the scratch
+    memory is `work`, or allocated (and later used again) in the stream's own order."""
+    device = tensors[0].get_device()
+    if device < 0:
         raise ValueError("operands must be in device memory")
-    if any(t.device != device for t in tensors):
-        raise ValueError("operands lie on different devices")
-    with torch.cuda.device(device):
-        s = torch.cuda.current_stream(device) if stream is None else stream
-        if s.device != device:
-            raise ValueError("the stream belongs to another device than the operands")
-        with torch.cuda.stream(s):      # scratch memory is then allocated, and reused, in this stream's order
-            yield ctypes.c_void_p(s.cuda_stream)
-
-
-def _scratch(work, need, device):
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError("operands lie on different devices")
     if need < 0:
         raise ValueError("extent out of range")
-    if work is None:
-        work = torch.empty(max(need, 1), dtype=torch.uint8, device=device)
-    elif not work.is_contiguous() or work.numel() * work.element_size() < need:
-        raise ValueError(f"work needs {need} contiguous bytes")
-    return work, work.numel() * work.element_size()
-
-
-def _p(address):
-    return ctypes.c_void_p(address)
+    if work is not None and (work.get_device() != device or not work.is_contiguous() or work.numel() * work.element_size() < need):
+        raise ValueError(f"work needs {need} contiguous bytes on the operands' device")
+    if stream is None and torch.cuda.current_device() == device:
+        if work is None and need:
+            work = torch.empty(need, dtype=torch.uint8, device=tensors[0].device)
+        rc = call(torch._C._cuda_getCurrentRawStream(device), work.data_ptr() if need else 0, need)
+    else:
+        with torch.cuda.device(device):
+            s = torch.cuda.current_stream(device) if stream is None else stream
+            if s.device.index != device:
+                raise ValueError("the stream belongs to another device than the operands")
+            with torch.cuda.stream(s):
+                if work is None and need:
+                    work = torch.empty(need, dtype=torch.uint8, device=tensors[0].device)
+                rc = call(s.cuda_stream, work.data_ptr() if need else 0, need)
+    if rc != _lib.OK:
+        _lib.check(rc, entry)
 
 
 def lora_plan(adapter_of, n_adapters, stream=None):
@@ -151,10 +152,13 @@ def lora_plan(adapter_of, n_adapters, stream=None):
     ints = lib.eigamd_lora_plan_ints(n, n_adapters)
     if ints < 0:
         raise ValueError("number of tokens or adapters out of range")
-    with _on(stream, adapter_of) as s:
-        plan = torch.empty(ints, dtype=torch.int32, device=adapter_of.device)
-        _lib.check(lib.eigamd_lora_plan_dev(n, n_adapters, _p(adapter_of.data_ptr()), _p(plan.data_ptr()), s), "eigamd_lora_plan_dev")
-    return LoraPlan(n, n_adapters, plan)
+    plan = []
+
+    def call(s, work, have):
+        plan.append(torch.empty(ints, dtype=torch.int32, device=adapter_of.device))
+        return lib.eigamd_lora_plan_dev(n, n_adapters, adapter_of.data_ptr(), plan[0].data_ptr(), s)
+    _run("eigamd_lora_plan_dev", stream, (adapter_of,), 0, None, call)
+    return LoraPlan(n, n_adapters, plan[0])
 
 
 def lora_work_bytes(opw, w, x):
@@ -183,12 +187,12 @@ def lora_dev(opw, w, x, opa, a, opb, b, scale, plan, p, y, work=None, stream=Non
     _check_stack(a, kind, *_turned(oa, rank, k), plan.n_adapters, "a")
     _check_stack(b, kind, *_turned(ob, m, rank), plan.n_adapters, "b")
     _check_vector(scale, plan.n_adapters, torch.float32, "scale")
-    with _on(stream, x.storage, w.storage, a.storage, b.storage, scale, plan.storage, p.storage, y.storage) as s:
-        work, have = _scratch(work, lib.eigamd_lora_work_bytes(kind, ow, m, n, k), x.storage.device)
-        rc = lib.eigamd_lora_dev(kind, ow, oa, ob, m, n, k, rank, plan.n_adapters, _p(w.ptr), w.ld, _p(x.ptr), x.ld, _p(a.ptr), a.ld,
-                                 a.stride, _p(b.ptr), b.ld, b.stride, _p(scale.data_ptr()), _p(plan.storage.data_ptr()), _p(p.ptr),
-                                 p.ld, _p(y.ptr), y.ld, _p(work.data_ptr()), have, s)
-    _lib.check(rc, "eigamd_lora_dev")
+    count = plan.n_adapters
+    _run("eigamd_lora_dev", stream, (x.storage, w.storage, a.storage, b.storage, scale, plan.storage, p.storage, y.storage),
+         lib.eigamd_lora_work_bytes(kind, ow, m, n, k), work,
+         lambda s, at, have: lib.eigamd_lora_dev(kind, ow, oa, ob, m, n, k, rank, count, w.ptr, w.ld, x.ptr, x.ld, a.ptr, a.ld, a.stride,
+                                                 b.ptr, b.ld, b.stride, scale.data_ptr(), plan.storage.data_ptr(), p.ptr, p.ld, y.ptr, y.ld,
+                                                 at, have, s))
     return y
 
 
@@ -209,32 +213,31 @@ def lora_wgrad_dev(opg, u, p, scale, plan, beta, g, work=None, stream=None):
     _check_matrix(p, _lib.F32, rank, n, "p")
     _check_stack(g, _lib.F32, *_turned(og, rows, rank), plan.n_adapters, "g")
     _check_vector(scale, plan.n_adapters, torch.float32, "scale")
-    be = np.array([beta], dtype=np.float32)
-    with _on(stream, u.storage, p.storage, scale, plan.storage, g.storage, *([u.exponents] if packed else [])) as s:
-        work, have = _scratch(work, lib.eigamd_lora_wgrad_work_bytes(rows, n, rank, plan.n_adapters), u.storage.device)
-        rc = lib.eigamd_lora_wgrad_dev(u.kind, og, rows, n, rank, plan.n_adapters, _p(u.ptr), u.ld,
-                                       _p(u.exponents.data_ptr()) if packed else None, u.lde if packed else 0, _p(p.ptr), p.ld,
-                                       _p(scale.data_ptr()), _p(plan.storage.data_ptr()), _p(be.ctypes.data), _p(g.ptr), g.ld, g.stride,
-                                       _p(work.data_ptr()), have, s)
-    _lib.check(rc, "eigamd_lora_wgrad_dev")
+    be, count = ctypes.c_float(beta), plan.n_adapters
+    tensors = (u.storage, p.storage, scale, plan.storage, g.storage)
+    exps, lde = 0, 0
+    if packed:
+        tensors, exps, lde = tensors + (u.exponents,), u.exponents.data_ptr(), u.lde
+    _run("eigamd_lora_wgrad_dev", stream, tensors, lib.eigamd_lora_wgrad_work_bytes(rows, n, rank, count), work,
+         lambda s, at, have: lib.eigamd_lora_wgrad_dev(u.kind, og, rows, n, rank, count, u.ptr, u.ld, exps, lde, p.ptr, p.ld,
+                                                       scale.data_ptr(), plan.storage.data_ptr(), ctypes.byref(be), g.ptr, g.ld, g.stride,
+                                                       at, have, s))
     return g
 
 
 def ckpt8_pack_dev(x, c, stream=None):
     """The DeviceMatrix x (features x tokens) into the Checkpoint8 c of the same kind and shape."""
     _check_matrix(x, c.kind, c.rows, c.cols, "x")
-    with _on(stream, x.storage, c.storage, c.exponents) as s:
-        rc = lib.eigamd_ckpt8_pack_dev(x.kind, x.rows, x.cols, _p(x.ptr), x.ld, _p(c.ptr), c.ld, _p(c.exponents.data_ptr()), c.lde, s)
-    _lib.check(rc, "eigamd_ckpt8_pack_dev")
+    _run("eigamd_ckpt8_pack_dev", stream, (x.storage, c.storage, c.exponents), 0, None,
+         lambda s, at, have: lib.eigamd_ckpt8_pack_dev(x.kind, x.rows, x.cols, x.ptr, x.ld, c.ptr, c.ld, c.exponents.data_ptr(), c.lde, s))
     return c
 
 
 def ckpt8_unpack_dev(c, x, stream=None):
     """The values the Checkpoint8 c stands for into the DeviceMatrix x of the same kind and shape."""
     _check_matrix(x, c.kind, c.rows, c.cols, "x")
-    with _on(stream, x.storage, c.storage, c.exponents) as s:
-        rc = lib.eigamd_ckpt8_unpack_dev(x.kind, x.rows, x.cols, _p(c.ptr), c.ld, _p(c.exponents.data_ptr()), c.lde, _p(x.ptr), x.ld, s)
-    _lib.check(rc, "eigamd_ckpt8_unpack_dev")
+    _run("eigamd_ckpt8_unpack_dev", stream, (x.storage, c.storage, c.exponents), 0, None,
+         lambda s, at, have: lib.eigamd_ckpt8_unpack_dev(x.kind, x.rows, x.cols, c.ptr, c.ld, c.exponents.data_ptr(), c.lde, x.ptr, x.ld, s))
     return x
 
 
@@ -247,10 +250,8 @@ def ckpt8_wgrad_dev(opw, dy, c, beta, dw, work=None, stream=None):
         raise ValueError("the kind must be F32, BF16 or F16")
     _check_matrix(dy, c.kind, m, n, "dy")
     _check_matrix(dw, _lib.F32, *_turned(ow, m, k), "dw")
-    be = np.array([beta], dtype=np.float32)
-    with _on(stream, dy.storage, c.storage, c.exponents, dw.storage) as s:
-        work, have = _scratch(work, lib.eigamd_ckpt8_wgrad_work_bytes(c.kind, m, n, k), dy.storage.device)
-        rc = lib.eigamd_ckpt8_wgrad_dev(c.kind, ow, m, n, k, _p(dy.ptr), dy.ld, _p(c.ptr), c.ld, _p(c.exponents.data_ptr()), c.lde,
-                                        _p(be.ctypes.data), _p(dw.ptr), dw.ld, _p(work.data_ptr()), have, s)
-    _lib.check(rc, "eigamd_ckpt8_wgrad_dev")
+    be = ctypes.c_float(beta)
+    _run("eigamd_ckpt8_wgrad_dev", stream, (dy.storage, c.storage, c.exponents, dw.storage), lib.eigamd_ckpt8_wgrad_work_bytes(c.kind, m, n, k), work,
+         lambda s, at, have: lib.eigamd_ckpt8_wgrad_dev(c.kind, ow, m, n, k, dy.ptr, dy.ld, c.ptr, c.ld, c.exponents.data_ptr(), c.lde,
+                                                        ctypes.byref(be), dw.ptr, dw.ld, at, have, s))
     return dw
