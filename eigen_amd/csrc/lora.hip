@@ -10,9 +10,15 @@
 
 #include "gemm_launch.hpp"
 #include "half_gemm.hpp"
+#include "lora_project.hpp"
 #include "lowrank.hpp"
 
 namespace eigamd {
+
+// lora_few.hip
+bool lora_few(int64_t n);
+int64_t lora_few_work_bytes(int64_t m, int64_t n, int64_t k);
+hipError_t lora_few_device(int kind, bool w_trans, const HalfGemm& g, const ProjectArgs& q, hipStream_t s);
 
 namespace {
 
@@ -49,243 +55,25 @@ __global__ __launch_bounds__(256) void lora_plan_kernel(const int* __restrict__ 
   }
 }
 
-// ---------------------------------------------------------------------------------------------------------- projection
-constexpr int kProjTokens = 32;
-struct ProjectArgs {
-  int n, k, rank, none;
-  const void* x; int64_t ldx;
-  const void* a; int64_t a_row, a_k, a_stride;    // strides of op(A_j)(r, k) and of j
-  const int* order;
-  const int* starts;
-  float* p; int64_t ldp;
-};
-
-// P for up to 32 tokens of one adapter and 16 RT ranks.  Eight waves share the reduction, 128 (64) positions a turn, each straight
-// from memory to the matrix unit: one load of a wave is 64 bytes of each of 16 tokens.  The next turn's loads are under way
-// while this one's are multiplied.
-//   A_K   the factor's reduction is contiguous: loaded like the tokens
-//   A_R   its ranks are (the backward pass): whole 16-byte chunks of ranks go through this wave's own LDS and come back
-//         transposed; one element at a time instead, the loads of a 64-rank factor took four times the rest (57 us of 4096 tokens
-//         x 4096, now 18)
-//   A_ANY element by element: ranks that are no multiple of 8, odd strides
-enum { A_K, A_R, A_ANY };
 template <typename T, int RT, int FORM> __global__ __launch_bounds__(512) void lora_project_kernel(ProjectArgs g) {
-  using E = typename T::elem;
-  using x8 = typename T::x8;
-  Piece piece;
-  if (!find_piece(g.starts, g.none + 1, kProjTokens, blockIdx.x, piece)) return;
-  const int w = threadIdx.x / 64, l = threadIdx.x & 63, r0 = blockIdx.y * 64;
-  constexpr int line = RT * 32, turned_bytes = FORM == A_R ? 8 * 32 * line : 0;     // A_R: 32 positions x 16 RT ranks per wave
-  constexpr int red_bytes = 8 * RT * 2 * 64 * 16;
-  __shared__ __align__(1024) char lds[red_bytes > turned_bytes ? red_bytes : turned_bytes];
-  f32x4(&red)[8][RT][2][64] = *reinterpret_cast<f32x4(*)[8][RT][2][64]>(lds);
-  const bool live = piece.adapter != g.none;
-  if (live) {
-    // lanes past the piece or the rank repeat the last one; what they compute is not stored
-    f32x4 acc[RT][2] = {};
-    const E* x[2];
-    const E* a[RT];
-    const E* factor = static_cast<const E*>(g.a) + (int64_t)piece.adapter * g.a_stride;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int at = piece.begin + c * 16 + (l & 15);
-      x[c] = static_cast<const E*>(g.x) + (int64_t)g.order[at < piece.end ? at : piece.end - 1] * g.ldx;
-    }
-    constexpr int per = RT * 2;                              // A_R: 16-byte chunks of a line
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      if constexpr (FORM == A_R) {
-        // chunk t * 64 + l of 32 lines
-        const int ch = t * 64 + l, r = r0 + (ch % per) * 8;
-        a[t] = factor + (int64_t)(ch / per) * g.a_k + (r < g.rank ? r : 0);
-      } else {
-        const int r = r0 + t * 16 + (l & 15);
-        a[t] = factor + (int64_t)(r < g.rank ? r : g.rank - 1) * g.a_row;
-      }
-    }
-    constexpr int S = RT == 4 ? 2 : 4, turn = 8 * 32 * S;      // products of a turn; positions all waves take in one
-    x8 fx[2][S][2], fa[2][S][RT];
-    auto load = [&](int k0, int set) {
-      const bool whole = k0 + 32 * S <= g.k;
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const int k = k0 + s * 32 + (l / 16) * 8, left = g.k - k;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) fx[set][s][c] = whole ? load_8<E, x8>(x[c] + k) : load_up_to_8<E, x8>(x[c] + k, left);
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          if constexpr (FORM == A_K) {
-            fa[set][s][t] = whole ? load_8<E, x8>(a[t] + k) : load_up_to_8<E, x8>(a[t] + k, left);
-          } else if constexpr (FORM == A_R) {
-            const int at = k0 + s * 32 + (t * 64 + l) / per;
-            fa[set][s][t] = load_up_to_8<E, x8>(a[t] + (int64_t)(k0 + s * 32) * g.a_k, at < g.k ? 8 : 0);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) fa[set][s][t][e] = e < left ? a[t][(int64_t)(k + e) * g.a_k] : (E)0.0f;
-          }
-        }
-      }
-    };
-    auto multiply = [&](int set) {
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        x8 f[RT];
-        if constexpr (FORM == A_R) {
-          char* mine = lds + w * 32 * line;
-          auto slot = [&](int ln, int ch) { return ln * line + ((ch ^ ((ln & 3) << 1)) & (per - 1)) * 16; };
-#pragma unroll
-          for (int t = 0; t < RT; ++t) *reinterpret_cast<x8*>(mine + slot((t * 64 + l) / per, (t * 64 + l) % per)) = fa[set][s][t];
-#pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            union { x8 v; typename T::x4 h[2]; } u;
-            const int ln = (l / 16) * 8 + (l & 15) / 4, ch = t * 2 + (l & 3) / 2;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) u.h[h] = T::read_transposed(mine + slot(ln + 4 * h, ch) + (l & 1) * 8);
-            f[t] = u.v;
-          }
-        } else {
-#pragma unroll
-          for (int t = 0; t < RT; ++t) f[t] = fa[set][s][t];
-        }
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) acc[t][c] = T::mma(f[t], fx[set][s][c], acc[t][c]);
-      }
-    };
-    int k0 = w * 32 * S;
-    if (k0 < g.k) load(k0, 0);
-    for (; k0 < g.k; k0 += 2 * turn) {
-      if (k0 + turn < g.k) load(k0 + turn, 1);
-      multiply(0);
-      if (k0 + turn >= g.k) break;
-      if (k0 + 2 * turn < g.k) load(k0 + 2 * turn, 0);
-      multiply(1);
-    }
-    if constexpr (FORM == A_R) __syncthreads();              // (the same LDS; `live` is the workgroup's)
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) red[w][t][c][l] = acc[t][c];
-  }
-  __syncthreads();
-  for (int q = threadIdx.x; q < RT * 2 * 64; q += 512) {
-    const int t = q / 128, c = (q / 64) % 2, at = piece.begin + c * 16 + (l & 15);
-    if (at >= piece.end) continue;
-    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (live)
-      for (int z = 0; z < 8; ++z) sum += red[z][t][c][l];
-    const int r = r0 + t * 16 + (l / 16) * 4;
-    float* out = g.p + (int64_t)g.order[at] * g.ldp + r;
-    for (int e = 0; e < 4; ++e)
-      if (r + e < g.rank) out[e] = sum[e];
-  }
+  __shared__ __align__(1024) char lds[project_lds(RT)];
+  project_piece<T, RT, FORM>(g, blockIdx.x, blockIdx.y * 64, lds);
 }
-
 template <typename T, int RT> hipError_t launch_project_rank(const ProjectArgs& g, hipStream_t s) {
-  const dim3 grid(g.n / kProjTokens + g.none + 1, (g.rank + 63) / 64);
-  bool turned = false;
-  if constexpr (T::bytes == 2) {
-    turned = g.a_row == 1 && g.a_k % 8 == 0 && g.rank % 8 == 0 && g.a_stride % 8 == 0 && (uintptr_t)g.a % 16 == 0;
-    if (g.a_k != 1 && turned) hipLaunchKernelGGL((lora_project_kernel<T, RT, A_R>), grid, dim3(512), 0, s, g);
+  const dim3 grid((unsigned)project_slots(g), (g.rank + 63) / 64);
+  switch (project_form<T>(g)) {
+    case A_K: hipLaunchKernelGGL((lora_project_kernel<T, RT, A_K>), grid, dim3(512), 0, s, g); break;
+    case A_R:
+      if constexpr (T::bytes == 2) hipLaunchKernelGGL((lora_project_kernel<T, RT, A_R>), grid, dim3(512), 0, s, g);
+      break;
+    default: hipLaunchKernelGGL((lora_project_kernel<T, RT, A_ANY>), grid, dim3(512), 0, s, g);
   }
-  if (g.a_k == 1) hipLaunchKernelGGL((lora_project_kernel<T, RT, A_K>), grid, dim3(512), 0, s, g);
-  else if (!turned) hipLaunchKernelGGL((lora_project_kernel<T, RT, A_ANY>), grid, dim3(512), 0, s, g);
   return hipGetLastError();
 }
 template <typename T> hipError_t launch_project(const ProjectArgs& g, hipStream_t s) {
   if (g.rank <= 16) return launch_project_rank<T, 1>(g, s);
   if (g.rank <= 32) return launch_project_rank<T, 2>(g, s);
   return launch_project_rank<T, 4>(g, s);
-}
-
-// ------------------------------------------------------------------------------------------------------ few tokens (KC)
-// Y for at most 16 NG tokens, W's reduction contiguous: the time is that of reading W once, so nothing is staged.  A workgroup
-// owns 16 rows; its eight waves share the reduction (128 positions a turn) and feed the matrix unit straight from memory.
-template <typename T, int NG> __global__ __launch_bounds__(512) void lora_few_kernel(HalfGemm g) {
-  using E = typename T::elem;
-  using x8 = typename T::x8;
-  const int w = threadIdx.x / 64, l = threadIdx.x & 63, row0 = blockIdx.x * 16;
-  const int row = row0 + (l & 15);
-  const E* a = static_cast<const E*>(g.a) + (int64_t)(row < g.m ? row : g.m - 1) * g.lda;
-  const E* b[NG];                     // columns past the last repeat it and are not stored
-#pragma unroll
-  for (int c = 0; c < NG; ++c) {
-    const int at = c * 16 + (l & 15);
-    b[c] = static_cast<const E*>(g.b) + (int64_t)g.order[at < g.n ? at : g.n - 1] * g.ldb;
-  }
-  f32x4 acc[NG] = {};
-  x8 fa[2][4], fb[2][4][NG];
-  auto load = [&](int k0, int set) {
-    const bool whole = k0 + 128 <= g.k;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int k = k0 + s * 32 + (l / 16) * 8, left = g.k - k;
-      fa[set][s] = whole ? load_8<E, x8>(a + k) : load_up_to_8<E, x8>(a + k, left);
-#pragma unroll
-      for (int c = 0; c < NG; ++c) fb[set][s][c] = whole ? load_8<E, x8>(b[c] + k) : load_up_to_8<E, x8>(b[c] + k, left);
-    }
-  };
-  auto multiply = [&](int set) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int c = 0; c < NG; ++c) acc[c] = T::mma(fa[set][s], fb[set][s][c], acc[c]);
-  };
-  int k0 = w * 128;
-  if (k0 < g.k) load(k0, 0);
-  // The low-rank part of this thread's outputs (256 NG of them, one row of a token each; 16 rows are 16 neighbouring threads),
-  // while the first loads of W are under way.
-  constexpr int NOUT = (256 * NG + 511) / 512;
-  float extra[NOUT];
-  int64_t at[NOUT];
-#pragma unroll
-  for (int q = 0; q < NOUT; ++q) {
-    const int r = row0 + threadIdx.x % 16, col = threadIdx.x / 16 + q * 32;
-    at[q] = -1;
-    extra[q] = 0.0f;
-    if (col >= g.n || r >= g.m) continue;
-    const int token = g.order[col], who = g.seg[col];
-    at[q] = token * g.ldc + r;
-    if (who == g.none || g.rank == 0) continue;
-    using f32x8 = float __attribute__((ext_vector_type(8)));
-    const E* up = static_cast<const E*>(g.up) + (int64_t)who * g.up_stride + (int64_t)r * g.up_row;
-    const float* p = g.p + token * g.ldp;
-    float d = 0.0f;
-    for (int t = 0; t < g.rank; t += 8) {
-      const f32x8 pv = load_up_to_8<float, f32x8>(p + t, g.rank - t);
-      x8 u;
-      if (g.up_rank == 1) {
-        u = load_up_to_8<E, x8>(up + t, g.rank - t);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] = t + e < g.rank ? up[(int64_t)(t + e) * g.up_rank] : (E)0.0f;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) d += (float)u[e] * pv[e];
-    }
-    extra[q] = g.scale[who] * d;
-  }
-  for (; k0 < g.k; k0 += 2 * 1024) {
-    if (k0 + 1024 < g.k) load(k0 + 1024, 1);
-    multiply(0);
-    if (k0 + 1024 >= g.k) break;
-    if (k0 + 2048 < g.k) load(k0 + 2048, 0);
-    multiply(1);
-  }
-  __shared__ f32x4 red[8][NG][64];
-#pragma unroll
-  for (int c = 0; c < NG; ++c) red[w][c][l] = acc[c];
-  __syncthreads();
-#pragma unroll
-  for (int q = 0; q < NOUT; ++q) {
-    if (at[q] < 0) continue;
-    const int r = threadIdx.x % 16, col = threadIdx.x / 16 + q * 32;
-    float sum = 0.0f;
-#pragma unroll
-    for (int z = 0; z < 8; ++z) sum += red[z][col / 16][(r / 4) * 16 + col % 16][r % 4];
-    static_cast<E*>(g.c)[at[q]] = (E)(sum + extra[q]);
-  }
 }
 
 // Sums of a split reduction, in the order of the pieces.
@@ -331,7 +119,6 @@ int choose_pieces(int64_t tiles, int64_t k, int64_t* k_piece) {
 
 int64_t tiles128(int64_t m, int64_t n) { return ((m + 127) / 128) * ((n + 127) / 128); }
 int64_t tiles256(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256); }
-bool few(bool w_trans, int64_t n) { return w_trans && n <= 64; }
 
 template <typename T, int LA, int SRC, int B, int WM, int WN> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
   const dim3 grid((unsigned)(B == 256 ? tiles256(g.m, g.n) : tiles128(g.m, g.n)), g.splits);
@@ -339,7 +126,7 @@ template <typename T, int LA, int SRC, int B, int WM, int WN> hipError_t launch_
   return hipGetLastError();
 }
 
-template <typename T> hipError_t launch_half(const LoraArgs& c, hipStream_t s) {
+template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArgs& q, hipStream_t s) {
   HalfGemm g;
   g.m = (int)c.m; g.n = (int)c.n; g.k = (int)c.k;
   g.a = c.w; g.lda = c.ldw;
@@ -356,16 +143,14 @@ template <typename T> hipError_t launch_half(const LoraArgs& c, hipStream_t s) {
   g.p = c.p; g.ldp = c.ldp;
   g.scale = c.scale;
   g.k_piece = (int)std::max<int64_t>((c.k + 63) / 64 * 64, 64);
-  if (few(c.w_trans, c.n)) {
-    const dim3 grid((unsigned)((c.m + 15) / 16));
-    switch ((c.n + 15) / 16) {
-      case 1: hipLaunchKernelGGL((lora_few_kernel<T, 1>), grid, dim3(512), 0, s, g); break;
-      case 2: hipLaunchKernelGGL((lora_few_kernel<T, 2>), grid, dim3(512), 0, s, g); break;
-      case 3: hipLaunchKernelGGL((lora_few_kernel<T, 3>), grid, dim3(512), 0, s, g); break;
-      default: hipLaunchKernelGGL((lora_few_kernel<T, 4>), grid, dim3(512), 0, s, g); break;
-    }
-    return hipGetLastError();
+  hipError_t e;
+  // whole 16-byte chunks everywhere: the loads go to LDS without passing through registers
+  const bool w_chunks = (uintptr_t)c.w % 16 == 0 && c.ldw % 8 == 0 && (c.w_trans || c.m % 8 == 0);
+  if (lora_few(c.n) && (c.w_trans || w_chunks)) {
+    g.partial = static_cast<float*>(c.work);
+    return lora_few_device(c.kind, c.w_trans, g, q, s);
   }
+  if (q.none > 0 && (e = launch_project<T>(q, s)) != hipSuccess) return e;
   int64_t piece = g.k_piece;
   const int splits = choose_pieces(tiles128(c.m, c.n), c.k, &piece);
   if (splits > 1 && c.work && c.work_bytes >= (int64_t)splits * c.m * c.n * 4) {
@@ -373,10 +158,7 @@ template <typename T> hipError_t launch_half(const LoraArgs& c, hipStream_t s) {
     g.k_piece = (int)piece;
     g.partial = static_cast<float*>(c.work);
   }
-  // whole 16-byte chunks everywhere: the loads go to LDS without passing through registers
-  const bool direct = ((uintptr_t)c.w | (uintptr_t)c.x) % 16 == 0 && c.ldw % 8 == 0 && c.ldx % 8 == 0 && c.k % 8 == 0 &&
-                      (c.w_trans || c.m % 8 == 0);
-  hipError_t e;
+  const bool direct = w_chunks && (uintptr_t)c.x % 16 == 0 && c.ldx % 8 == 0 && c.k % 8 == 0;
   if (direct && g.splits == 1 && tiles256(c.m, c.n) >= 200)
     e = c.w_trans ? launch_tiles<T, KC, DIRECT, 256, 2, 4>(g, s) : launch_tiles<T, MC, DIRECT, 256, 2, 4>(g, s);
   else if (direct)
@@ -593,6 +375,10 @@ template <typename T, int SRC> hipError_t launch_grad_rank(const GradArgs& g, di
 
 }  // namespace
 
+hipError_t lora_project_device(int kind, const ProjectArgs& g, hipStream_t s) {
+  return kind == BF16 ? launch_project<Bf16>(g, s) : kind == F16K ? launch_project<F16>(g, s) : launch_project<Fp32>(g, s);
+}
+
 hipError_t lora_plan_device(const int* ids, int64_t n, int64_t adapters, int* d_plan, hipStream_t s) {
   hipLaunchKernelGGL(lora_plan_kernel, dim3((unsigned)(adapters / 4 + 1)), dim3(256), 0, s, ids, (int)n, (int)adapters, d_plan,
                      d_plan + n, d_plan + 2 * n);
@@ -600,32 +386,29 @@ hipError_t lora_plan_device(const int* ids, int64_t n, int64_t adapters, int* d_
 }
 
 int64_t lora_work_bytes(int kind, bool w_trans, int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  if (m <= 0 || n <= 0) return 0;
   if (kind == F32) return std::min<int64_t>(16 * m * n * 4, (int64_t)256 << 20);
-  if (few(w_trans, n)) return 0;
   int64_t piece;
   const int splits = choose_pieces(tiles128(m, n), k, &piece);
-  return splits > 1 ? (int64_t)splits * m * n * 4 : 0;
+  const int64_t tiles = splits > 1 ? (int64_t)splits * m * n * 4 : 0;
+  return lora_few(n) ? std::max<int64_t>(tiles, lora_few_work_bytes(m, n, k)) : tiles;
 }
 
 hipError_t lora_device(const LoraArgs& c, hipStream_t s) {
+  ProjectArgs p;
+  p.n = (int)c.n; p.k = (int)c.k; p.rank = (int)c.rank; p.none = c.plan.adapters;
+  p.x = c.x; p.ldx = c.ldx;
+  p.a = c.a;
+  p.a_row = c.a_trans ? c.lda : 1;
+  p.a_k = c.a_trans ? 1 : c.lda;
+  p.a_stride = c.stride_a;
+  p.order = c.plan.order; p.starts = c.plan.starts;
+  p.p = c.p; p.ldp = c.ldp;
+  if (c.m > 0 && c.kind == BF16) return launch_half<Bf16>(c, p, s);
+  if (c.m > 0 && c.kind == F16K) return launch_half<F16>(c, p, s);
   hipError_t e = hipSuccess;
-  if (c.plan.adapters > 0) {
-    ProjectArgs g;
-    g.n = (int)c.n; g.k = (int)c.k; g.rank = (int)c.rank; g.none = c.plan.adapters;
-    g.x = c.x; g.ldx = c.ldx;
-    g.a = c.a;
-    g.a_row = c.a_trans ? c.lda : 1;
-    g.a_k = c.a_trans ? 1 : c.lda;
-    g.a_stride = c.stride_a;
-    g.order = c.plan.order; g.starts = c.plan.starts;
-    g.p = c.p; g.ldp = c.ldp;
-    e = c.kind == BF16 ? launch_project<Bf16>(g, s) : c.kind == F16K ? launch_project<F16>(g, s) : launch_project<Fp32>(g, s);
-    if (e != hipSuccess || c.m == 0) return e;
-  }
-  if (c.m == 0) return e;
-  if (c.kind == BF16) return launch_half<Bf16>(c, s);
-  if (c.kind == F16K) return launch_half<F16>(c, s);
+  if (p.none > 0) e = lora_project_device(c.kind, p, s);
+  if (e != hipSuccess || c.m == 0) return e;
   GemmCall q;
   q.kind = F32;
   q.opa = c.w_trans ? OP_T : OP_N; q.opb = OP_N;

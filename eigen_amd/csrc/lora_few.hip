@@ -1,0 +1,233 @@
+// The adapter product for few tokens (one a request while answering): one launch over W and the projection, one that joins.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "half_gemm.hpp"
+#include "lora_project.hpp"
+#include "lowrank.hpp"
+
+namespace eigamd {
+
+hipError_t lora_project_device(int kind, const ProjectArgs& g, hipStream_t s);   // lora.hip
+
+namespace {
+
+// Y for at most 64 tokens (16 NG of them): the time is that of reading W once, from as many compute units as there are.  A
+// workgroup owns 64 rows and one piece of the reduction, so that X, which every workgroup reads its piece of, costs little beside
+// W (with 16 rows and the whole reduction X was four times the traffic: 64 tokens x 4096 x 4096 took 22 us, now 12).  Its eight
+// waves share the piece, 64 (32) positions a turn, from memory to the matrix unit directly (W's reduction contiguous) or through the
+// wave's own LDS and back transposed (its rows contiguous).  The sums go to memory in 32 bits; the second kernel adds the
+// pieces up and the low-rank part to them.
+// The projection needs nothing of this, so its workgroups (16 ranks each) are the first ones of the same launch.
+template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512) void lora_few_kernel(HalfGemm g, ProjectArgs q, int project, int slots) {
+  using E = typename T::elem;
+  using x8 = typename T::x8;
+  constexpr int red_bytes = 8 * 4 * NG * 64 * 16, lds_bytes = red_bytes > project_lds(1) ? red_bytes : project_lds(1);
+  __shared__ __align__(1024) char lds[lds_bytes];
+  if ((int)blockIdx.x < project) {
+    project_piece<T, 1, FORM>(q, blockIdx.x % slots, blockIdx.x / slots * 16, lds);
+    return;
+  }
+  const int id = blockIdx.x - project, row_blocks = (g.m + 63) / 64;
+  const int row0 = id % row_blocks * 64, z = id / row_blocks;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63;
+  const int k_begin = z * g.k_piece, k_end = k_begin + g.k_piece < g.k ? k_begin + g.k_piece : g.k;
+  const E* a[4];                      // KC: rows of the four row blocks; MC: chunks of 8 lines
+  const E* b[NG];                     // rows and columns past the end repeat the last one and are not stored
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if constexpr (LA == KC) {
+      const int row = row0 + t * 16 + (l & 15);
+      a[t] = static_cast<const E*>(g.a) + (int64_t)(row < g.m ? row : g.m - 1) * g.lda;
+    } else {
+      const int row = row0 + (l % 8) * 8;
+      a[t] = static_cast<const E*>(g.a) + (int64_t)(t * 8 + l / 8) * g.lda + (row < g.m ? row : 0);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < NG; ++c) {
+    const int at = c * 16 + (l & 15);
+    b[c] = static_cast<const E*>(g.b) + (int64_t)g.order[at < g.n ? at : g.n - 1] * g.ldb;
+  }
+  f32x4 acc[4][NG] = {};
+  constexpr int S = NG == 4 ? 1 : 2, turn = 8 * 32 * S;
+  x8 fa[2][S][4], fb[2][S][NG];
+  auto load = [&](int k0, int set) {
+    const bool whole = k0 + 32 * S <= k_end;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int k = k0 + s * 32 + (l / 16) * 8, left = k_end - k;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if constexpr (LA == KC) fa[set][s][t] = whole ? load_8<E, x8>(a[t] + k) : load_up_to_8<E, x8>(a[t] + k, left);
+        else {
+          const int line = k0 + s * 32 + t * 8 + l / 8;
+          fa[set][s][t] = load_up_to_8<E, x8>(a[t] + (int64_t)(k0 + s * 32) * g.lda, whole || line < k_end ? 8 : 0);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < NG; ++c) fb[set][s][c] = whole ? load_8<E, x8>(b[c] + k) : load_up_to_8<E, x8>(b[c] + k, left);
+    }
+  };
+  auto multiply = [&](int set) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      x8 f[4];
+      if constexpr (LA == MC) {
+        // lines of 64 rows, 128 bytes; chunks permuted so that the 8 lines a half wave reads meet all banks once
+        char* mine = lds + w * 4096;
+        auto slot = [](int line, int ch) { return line * 128 + (ch ^ (((line >> 1) & 1) | ((line >> 2) & 2)) << 1) * 16; };
+#pragma unroll
+        for (int t = 0; t < 4; ++t) *reinterpret_cast<x8*>(mine + slot(t * 8 + l / 8, l % 8)) = fa[set][s][t];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          union { x8 v; typename T::x4 h[2]; } u;
+          const int line = (l / 16) * 8 + (l & 15) / 4, ch = t * 2 + (l & 3) / 2;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) u.h[h] = T::read_transposed(mine + slot(line + 4 * h, ch) + (l & 1) * 8);
+          f[t] = u.v;
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) f[t] = fa[set][s][t];
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int c = 0; c < NG; ++c) acc[t][c] = T::mma(f[t], fb[set][s][c], acc[t][c]);
+    }
+  };
+  int k0 = k_begin + w * 32 * S;
+  if (k0 < k_end) load(k0, 0);
+  for (; k0 < k_end; k0 += 2 * turn) {
+    if (k0 + turn < k_end) load(k0 + turn, 1);
+    multiply(0);
+    if (k0 + turn >= k_end) break;
+    if (k0 + 2 * turn < k_end) load(k0 + 2 * turn, 0);
+    multiply(1);
+  }
+  if constexpr (LA == MC) __syncthreads();
+  f32x4(&red)[8][4][NG][64] = *reinterpret_cast<f32x4(*)[8][4][NG][64]>(lds);
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int c = 0; c < NG; ++c) red[w][t][c][l] = acc[t][c];
+  __syncthreads();
+  float* out = g.partial + (int64_t)z * g.m * g.n;
+#pragma unroll
+  for (int v = threadIdx.x; v < 4 * NG * 64; v += 512) {
+    // 16 neighbouring threads hold the 64 rows of a column
+    const int part = v % 16, col = v / 16, t = part / 4;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int y = 0; y < 8; ++y) sum += red[y][t][col / 16][(part % 4) * 16 + col % 16];
+    const int row = row0 + part * 4;
+    if (col >= g.n) continue;
+    float* at = out + (int64_t)col * g.m + row;
+    if (g.m % 4 == 0 && row < g.m) *reinterpret_cast<f32x4*>(at) = sum;
+    else
+      for (int e = 0; e < 4; ++e)
+        if (row + e < g.m) at[e] = sum[e];
+  }
+}
+
+// Sums of a split reduction in the order of the pieces, and the low-rank part: one output per thread, neighbouring rows side by
+// side, 8 ranks at a time.
+template <typename T> __global__ __launch_bounds__(256) void lora_few_join_kernel(HalfGemm g) {
+  using E = typename T::elem;
+  using x8 = typename T::x8;
+  using f32x8 = float __attribute__((ext_vector_type(8)));
+  const int row = blockIdx.x * 256 + threadIdx.x, col = blockIdx.y;
+  if (row >= g.m) return;
+  const int token = g.order[col], who = g.seg[col];
+  const int64_t total = (int64_t)g.m * g.n;
+  const float* from = g.partial + (int64_t)col * g.m + row;
+  float sum = 0.0f;
+  int z = 0;
+  for (; z + 4 <= g.splits; z += 4) {
+    float v[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) v[t] = from[(z + t) * total];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) sum += v[t];
+  }
+  for (; z < g.splits; ++z) sum += from[z * total];
+  if (who != g.none && g.rank > 0) {
+    const E* up = static_cast<const E*>(g.up) + (int64_t)who * g.up_stride + (int64_t)row * g.up_row;
+    const float* p = g.p + token * g.ldp;
+    float d = 0.0f;
+    for (int t = 0; t < g.rank; t += 8) {
+      const f32x8 pv = load_up_to_8<float, f32x8>(p + t, g.rank - t);
+      x8 u;
+      if (g.up_rank == 1) {
+        u = load_up_to_8<E, x8>(up + t, g.rank - t);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = t + e < g.rank ? up[(int64_t)(t + e) * g.up_rank] : (E)0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d += (float)u[e] * pv[e];
+    }
+    sum += g.scale[who] * d;
+  }
+  static_cast<E*>(g.c)[token * g.ldc + row] = (E)sum;
+}
+
+// At most 64 tokens: pieces of the reduction, none shorter than 512 (eight waves, 64 positions each), at most 512 workgroups.
+bool piece_allowed(int64_t blocks, int64_t k, int64_t pieces) {
+  return pieces == 1 || (pieces <= 16 && k / pieces >= 512 && blocks * pieces <= 512);
+}
+// A compute unit runs one of these workgroups at a time, so the 64-row blocks times the pieces and the projection's workgroups
+// should fill whole rounds of 256; a round costs what its piece does plus the latencies at both ends, about as much as 600
+// positions (64 tokens x 4096 x 4096: 512 workgroups 16.8 us, 256 12.6).
+int few_pieces(int64_t m, int64_t k, int64_t project, int64_t* k_piece) {
+  const int64_t blocks = (m + 63) / 64;
+  int64_t best = 1, best_cost = INT64_MAX;
+  for (int64_t pieces = 1; piece_allowed(blocks, k, pieces); ++pieces) {
+    const int64_t piece = (k + pieces - 1) / pieces, cost = (blocks * pieces + project + 255) / 256 * (piece + 600);
+    if (cost < best_cost) { best = pieces; best_cost = cost; }
+  }
+  *k_piece = std::max<int64_t>(((k + best - 1) / best + 63) / 64 * 64, 64);
+  return (int)std::max<int64_t>((k + *k_piece - 1) / *k_piece, 1);
+}
+template <typename T, int LA, int NG> hipError_t launch_few_tokens(const HalfGemm& g, const ProjectArgs& q, int form, hipStream_t s) {
+  const int slots = q.none && form != A_ANY ? (int)project_slots(q) : 0, project = slots * ((q.rank + 15) / 16);
+  const dim3 grid((unsigned)(project + (g.m + 63) / 64 * g.splits));
+  if (form == A_R) hipLaunchKernelGGL((lora_few_kernel<T, LA, NG, A_R>), grid, dim3(512), 0, s, g, q, project, slots);
+  else hipLaunchKernelGGL((lora_few_kernel<T, LA, NG, A_K>), grid, dim3(512), 0, s, g, q, project, slots);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(lora_few_join_kernel<T>, dim3((unsigned)((g.m + 255) / 256), (unsigned)g.n), dim3(256), 0, s, g);
+  return hipGetLastError();
+}
+template <typename T, int LA> hipError_t launch_few(HalfGemm g, const ProjectArgs& q, hipStream_t s) {
+  // factors that are read element by element keep the projection in a launch of its own
+  const int form = project_form<T>(q);
+  if (q.none && form == A_ANY) {
+    hipError_t e = lora_project_device(__is_same(T, Bf16) ? (int)BF16 : (int)F16K, q, s);
+    if (e != hipSuccess) return e;
+  }
+  int64_t piece;
+  g.splits = few_pieces(g.m, g.k, q.none && form != A_ANY ? project_slots(q) * ((q.rank + 15) / 16) : 0, &piece);
+  g.k_piece = (int)piece;
+  return g.n <= 16 ? launch_few_tokens<T, LA, 1>(g, q, form, s) : g.n <= 32 ? launch_few_tokens<T, LA, 2>(g, q, form, s)
+                                                                         : launch_few_tokens<T, LA, 4>(g, q, form, s);
+}
+
+}  // namespace
+
+bool lora_few(int64_t n) { return n <= 64; }
+int64_t lora_few_work_bytes(int64_t m, int64_t n, int64_t k) {
+  int64_t pieces = 1;
+  while (piece_allowed((m + 63) / 64, k, pieces + 1)) ++pieces;
+  return pieces * m * n * 4;
+}
+
+hipError_t lora_few_device(int kind, bool w_trans, const HalfGemm& g, const ProjectArgs& q, hipStream_t s) {
+  if (kind == BF16) return w_trans ? launch_few<Bf16, KC>(g, q, s) : launch_few<Bf16, MC>(g, q, s);
+  return w_trans ? launch_few<F16, KC>(g, q, s) : launch_few<F16, MC>(g, q, s);
+}
+
+}  // namespace eigamd
