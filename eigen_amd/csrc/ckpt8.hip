@@ -114,33 +114,16 @@ PackArgs pack_args(int64_t k, int64_t n) {
   return g;
 }
 
-// C = beta C + the pieces of a split reduction, in their order; C is rows x cols.
-__global__ __launch_bounds__(256) void ckpt8_join_kernel(const float* __restrict__ partial, int splits, int rows, int64_t total, float beta,
-                                                         float* __restrict__ c, int64_t ldc) {
-  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
-    float sum = 0.0f;
-    for (int z = 0; z < splits; ++z) sum += partial[(int64_t)z * total + q];
-    const int64_t col = q / rows;
-    float* at = c + col * ldc + (q - col * rows);
-    *at = sum + (beta != 0.0f ? beta * *at : 0.0f);
-  }
-}
-
-int choose_pieces(int64_t m, int64_t k, int64_t n, int64_t* n_piece) {
-  const int64_t tiles = ((m + 127) / 128) * ((k + 127) / 128);
-  const int64_t want = std::min<int64_t>(std::max<int64_t>(512 / std::max<int64_t>(tiles, 1), 1), std::max<int64_t>(n / 512, 1));
-  *n_piece = std::max<int64_t>(((n + want - 1) / want + 63) / 64 * 64, 64);
-  return (int)std::max<int64_t>((n + *n_piece - 1) / *n_piece, 1);
-}
-
 template <typename T, int SRC, int OUT, int B, int WM, int WN> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
   const dim3 grid((unsigned)(((g.m + B - 1) / B) * ((g.n + B - 1) / B)), g.splits);
-  hipLaunchKernelGGL((half_gemm_kernel<T, MC, QUANT, MC, SRC, OUT, B, B, WM, WN>), grid, dim3(WM * WN * 64), 0, s, g);
+  hipLaunchKernelGGL((half_gemm_kernel<T, MC, QUANT, MC, SRC, OUT, B, B, WM, WN, 2>), grid, dim3(WM * WN * 64), 0, s, g);
   return hipGetLastError();
 }
-template <typename T, int OUT> hipError_t launch_out(const HalfGemm& g, bool direct, bool large, hipStream_t s) {
+template <typename T, int OUT> hipError_t launch_out(const HalfGemm& g, bool direct, int tile, hipStream_t s) {
   if (!direct) return launch_tiles<T, STAGED, OUT, 128, 2, 2>(g, s);
-  return large ? launch_tiles<T, DIRECT, OUT, 256, 2, 4>(g, s) : launch_tiles<T, DIRECT, OUT, 128, 2, 2>(g, s);
+  return tile == TILE_256   ? launch_tiles<T, DIRECT, OUT, 256, 2, 4>(g, s)
+         : tile == TILE_128 ? launch_tiles<T, DIRECT, OUT, 128, 2, 2>(g, s)
+                            : launch_tiles<T, DIRECT, OUT, 128, 2, 4>(g, s);
 }
 
 }  // namespace
@@ -170,8 +153,7 @@ hipError_t ckpt8_unpack_device(int kind, int64_t k, int64_t n, const int8_t* q, 
 int64_t ckpt8_grad_work_bytes(int kind, int64_t m, int64_t n, int64_t k) {
   if (m <= 0 || n <= 0 || k <= 0) return 0;
   if (kind == F32) return (k * n * 4 + 255) / 256 * 256 + std::min<int64_t>(16 * m * k * 4, (int64_t)256 << 20);
-  int64_t piece;
-  const int splits = choose_pieces(m, k, n, &piece);
+  const int splits = plan_tiles(k, m, n).splits;
   return splits > 1 ? splits * m * k * 4 : 0;
 }
 
@@ -201,24 +183,16 @@ hipError_t ckpt8_grad_device(const Ckpt8GradArgs& c, hipStream_t s) {
   g.b = c.dy; g.ldb = c.lddy;
   g.c = c.dw; g.ldc = c.lddw;
   g.beta = c.beta;
-  int64_t piece;
-  const int splits = choose_pieces(c.m, c.k, c.n, &piece);
-  g.k_piece = (int)std::max<int64_t>((c.n + 63) / 64 * 64, 64);
-  if (splits > 1 && c.work && c.work_bytes >= splits * c.m * c.k * 4) {
-    g.splits = splits;
-    g.k_piece = (int)piece;
-    g.partial = static_cast<float*>(c.work);
-  }
+  const TilePlan plan = plan_tiles(c.k, c.m, c.n);
+  g.splits = plan.splits;
+  g.k_piece = (int)plan.k_piece;
+  g.partial = static_cast<float*>(c.work);
   const bool direct = (uintptr_t)c.dy % 16 == 0 && c.lddy % 8 == 0 && c.m % 8 == 0;
-  const bool large = g.splits == 1 && ((c.m + 255) / 256) * ((c.k + 255) / 256) >= 200;
   hipError_t e;
-  if (c.kind == BF16) e = c.trans ? launch_out<Bf16, OUT_F32>(g, direct, large, s) : launch_out<Bf16, OUT_F32_SWAPPED>(g, direct, large, s);
-  else e = c.trans ? launch_out<F16, OUT_F32>(g, direct, large, s) : launch_out<F16, OUT_F32_SWAPPED>(g, direct, large, s);
+  if (c.kind == BF16) e = c.trans ? launch_out<Bf16, OUT_F32>(g, direct, plan.tile, s) : launch_out<Bf16, OUT_F32_SWAPPED>(g, direct, plan.tile, s);
+  else e = c.trans ? launch_out<F16, OUT_F32>(g, direct, plan.tile, s) : launch_out<F16, OUT_F32_SWAPPED>(g, direct, plan.tile, s);
   if (e != hipSuccess || g.splits == 1) return e;
-  const int64_t total = c.m * c.k;
-  hipLaunchKernelGGL(ckpt8_join_kernel, dim3((unsigned)std::min<int64_t>((total + 255) / 256, 4096)), dim3(256), 0, s, g.partial, g.splits,
-                     (int)(c.trans ? c.k : c.m), total, c.beta, c.dw, c.lddw);
-  return hipGetLastError();
+  return launch_half_join(g.partial, g.splits, (int)(c.trans ? c.k : c.m), c.m * c.k, c.beta, c.dw, c.lddw, (const int*)nullptr, s);
 }
 
 }  // namespace eigamd

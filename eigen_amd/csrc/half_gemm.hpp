@@ -58,10 +58,12 @@ __device__ __forceinline__ void load_to_lds(const char* base, unsigned off, char
   const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)EIGAMD_LDS(char, to));
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(base) : "memory");
 }
-// All of this wave's loads and LDS accesses are done, then those of the workgroup.
-__device__ __forceinline__ void slice_barrier() {
+// This wave's LDS accesses and all but its newest KEEP loads are done, then those of the workgroup.
+template <int KEEP> __device__ __forceinline__ void slice_barrier() {
+  static_assert(KEEP < 64, "six bits of vmcnt");
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x70);   // vmcnt(0) lgkmcnt(0), in a form the compiler's own counting sees
+  // vmcnt(KEEP) lgkmcnt(0), in a form the compiler's own counting sees
+  __builtin_amdgcn_s_waitcnt(0x70 | (KEEP & 15) | (KEEP >> 4) << 14);
   asm volatile("s_barrier" ::: "memory");
 }
 
@@ -339,13 +341,14 @@ enum { OUT_HALF = 0, OUT_F32 = 1, OUT_F32_SWAPPED = 2 };
 
 // OUT_HALF: C in the operands' type, columns scattered by `order`, adapters added.
 // OUT_F32: C = beta C + A B in 32 bits.  OUT_F32_SWAPPED: the same with C stored transposed (N x M column-major).
-template <typename T, int LA, int SA, int LB, int SB, int OUT, int BM, int BN, int WM, int WN>
+template <typename T, int LA, int SA, int LB, int SB, int OUT, int BM, int BN, int WM, int WN, int D>
 __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
   constexpr int NT = WM * WN * 64, TM = BM / WM, TN = BN / WN, NI = TM / 16, NJ = TN / 16;
   using LoadA = SliceLoader<T, LA, SA, BM, NT, false>;
   using LoadB = SliceLoader<T, LB, SB, BN, NT, OUT == OUT_HALF>;
   constexpr int slice = LoadA::bytes + LoadB::bytes;
-  __shared__ __align__(1024) char lds[2 * slice];
+  static_assert(D == 2 || (SA == DIRECT && SB == DIRECT), "what passes through registers is one slice ahead of LDS");
+  __shared__ __align__(1024) char lds[D * slice];
   const int tiles_m = (g.m + BM - 1) / BM, tiles_n = (g.n + BN - 1) / BN;
   int tm, tn;
   tile_of<4>(blockIdx.x, tiles_m, tiles_n, tm, tn);
@@ -360,12 +363,12 @@ __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
   la.init(g.a, g.lda, tm * BM, g.m, k_begin, k_count, nullptr, g.exponents, g.lde);
   lb.init(g.b, g.ldb, tn * BN, g.n, k_begin, k_count, g.order, g.exponents, g.lde);
   f32x4 acc[NI][NJ] = {};
-  // Two slices in LDS.  Each half of a slice (32 positions) is multiplied in two steps, the upper and the lower half of this wave's
-  // rows; while one step's products run, the fragments of the next are read.  A slice's buffer is free once its last fragments are
-  // in registers: from the barrier in front of slice s's last step on, slice s + 2 is on its way there, and has to have arrived at
-  // the next slice's barrier.
+  // D slices in LDS.  Each half of a slice (32 positions) is multiplied in P steps of 16 rows each x 4 (all rows of this wave, or the
+  // upper and the lower half); while one step's products run, the fragments of the next are read.  A slice's buffer is free once
+  // its last fragments are in registers: from the barrier in front of slice s's last step on, slice s + D is on its way there;
+  // slice s + 1 has to have arrived at that barrier, those behind it may still be under way.
 #pragma unroll 1
-  for (int z = 0; z < 2; ++z) {
+  for (int z = 0; z < D; ++z) {
     la.fetch();
     lb.fetch();
     la.commit(lds + z * slice);
@@ -376,67 +379,68 @@ __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
   if constexpr (OUT == OUT_HALF) {
     if (g.rank > 0 && blockIdx.y == 0) add_adapters<T, NI, NJ>(g, tm * BM + wr, tn * BN + wc, acc);
   }
-  slice_barrier();
-  constexpr int NH = NI / 2, RA = LA == KC ? 1 : 2, RB = LB == KC ? 1 : 2;
+  slice_barrier<0>();
+  constexpr int P = NI > 4 ? 2 : 1, NH = NI / P, RA = LA == KC ? 1 : 2, RB = LB == KC ? 1 : 2;
   typename T::x8 fa[2][NH], fb[2][NJ];
-  auto read_a = [&](const char* from, int half, int kk) {
+  // fragments of step q of the slice at `from`
+  auto read = [&](const char* from, int q) {
+    const int half = q / P, part = q % P;
 #pragma unroll
-    for (int i = 0; i < NH; ++i) fa[half][i] = LoadA::fragment(from, wr + (half * NH + i) * 16, kk);
-  };
-  auto read_b = [&](const char* from, int set, int kk) {
+    for (int i = 0; i < NH; ++i) fa[q & 1][i] = LoadA::fragment(from, wr + (part * NH + i) * 16, half * 32);
+    if (part == 0) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) fb[set][j] = LoadB::fragment(from + LoadA::bytes, wc + j * 16, kk);
+      for (int j = 0; j < NJ; ++j) fb[half][j] = LoadB::fragment(from + LoadA::bytes, wc + j * 16, half * 32);
+    }
   };
-  auto multiply = [&](int half, int set) {
+  auto multiply = [&](int q) {
+    const int half = q / P, part = q % P;
 #pragma unroll
     for (int i = 0; i < NH; ++i)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        f32x4& c = acc[half * NH + i][j];
-        c = OUT == OUT_F32_SWAPPED ? T::mma(fb[set][j], fa[half][i], c) : T::mma(fa[half][i], fb[set][j], c);
+        f32x4& c = acc[part * NH + i][j];
+        c = OUT == OUT_F32_SWAPPED ? T::mma(fb[half][j], fa[q & 1][i], c) : T::mma(fa[q & 1][i], fb[half][j], c);
       }
   };
   // The compiler would put each read right in front of the product that needs it; here every read of the next step is followed
   // by products of this one.
   constexpr int products = NH * NJ;
   auto interleave = [&](auto count) {
-    constexpr int reads = decltype(count)::value;
+    constexpr int reads = decltype(count)::value, per = products >= 2 * reads ? products / reads / 2 : products >= reads ? 1 : 0;
 #pragma unroll
     for (int q = 0; q < reads; ++q) {
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, products / reads, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, per, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, products % reads, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, products - reads * per, 0);
     __builtin_amdgcn_sched_barrier(0);
   };
   using ReadsA = std::integral_constant<int, NH * RA>;
   using ReadsAB = std::integral_constant<int, NH * RA + NJ * RB>;
-  read_a(lds, 0, 0);
-  read_b(lds, 0, 0);
+  read(lds, 0);
+  constexpr int keep = (D - 2) * (LoadA::N + LoadB::N);
+  char* here = lds;
   for (int s = 0; s < slices; ++s) {
-    char* here = lds + (s & 1) * slice;
-    char* other = lds + ((s & 1) ^ 1) * slice;
-    read_a(here, 1, 0);
-    multiply(0, 0);
-    interleave(ReadsA{});
-    read_a(here, 0, 32);
-    read_b(here, 1, 32);
-    multiply(1, 0);
-    interleave(ReadsAB{});
-    read_a(here, 1, 32);
-    multiply(0, 1);
-    interleave(ReadsA{});
-    slice_barrier();
+    char* other = here + slice == lds + D * slice ? lds : here + slice;
+#pragma unroll
+    for (int q = 0; q + 1 < 2 * P; ++q) {
+      read(here, q + 1);
+      multiply(q);
+      if ((q + 1) % P == 0) interleave(ReadsAB{});
+      else interleave(ReadsA{});
+    }
+    if (D == 2 || s + D > slices) slice_barrier<0>();
+    else slice_barrier<keep>();
     la.commit(here);
     lb.commit(here + LoadA::bytes);
     la.fetch();
     lb.fetch();
-    read_a(other, 0, 0);     // (behind the last slice: what was there before, not used)
-    read_b(other, 0, 0);
-    multiply(1, 1);
+    read(other, 0);     // (behind the last slice: what was there before, not used)
+    multiply(2 * P - 1);
     interleave(ReadsAB{});
+    here = other;
   }
-  slice_barrier();
+  slice_barrier<0>();
 
   const int row0 = tm * BM + wr, col0 = tn * BN + wc;
   if (g.splits > 1) {
@@ -464,7 +468,7 @@ __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
     // through LDS (the slices are done with; every wave stays in its own part): whole lines of C per store
     using E = typename T::elem;
     constexpr int line = TM * 2 + 16;
-    static_assert(16 * line * WM * WN <= 2 * slice, "the epilogue's part of LDS");
+    static_assert(16 * line * WM * WN <= D * slice, "the epilogue's part of LDS");
     char* mine = lds + w * 16 * line;
     E* C = static_cast<E*>(g.c);
     const bool wide = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && g.ldc % 8 == 0;
@@ -514,6 +518,72 @@ __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
         }
       }
   }
+}
+
+// Sums of a split reduction in the order of the pieces, four rows a thread: C = beta C + sum (C in the operands' type: beta is 0).
+// `rows` is C's contiguous extent, `order` its columns' (nullptr: as they are).
+template <typename E> __global__ __launch_bounds__(256) void half_join_kernel(const float* __restrict__ partial, int splits, int rows, int64_t total,
+                                                                           float beta, E* __restrict__ c, int64_t ldc, const int* __restrict__ order) {
+  const bool wide = rows % 4 == 0;
+  const int per = wide ? 4 : 1;
+  for (int64_t q = ((int64_t)blockIdx.x * 256 + threadIdx.x) * per; q < total; q += (int64_t)gridDim.x * 256 * per) {
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (wide) {
+      int z = 0;
+      for (; z + 4 <= splits; z += 4) {
+        f32x4 v[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[t] = *reinterpret_cast<const f32x4*>(partial + (int64_t)(z + t) * total + q);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sum += v[t];
+      }
+      for (; z < splits; ++z) sum += *reinterpret_cast<const f32x4*>(partial + (int64_t)z * total + q);
+    } else {
+      for (int z = 0; z < splits; ++z) sum[0] += partial[(int64_t)z * total + q];
+    }
+    const int64_t col = q / rows;
+    E* at = c + (order ? order[col] : col) * ldc + (q - col * rows);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if (t < per) at[t] = (E)(sum[t] + (beta != 0.0f ? beta * (float)at[t] : 0.0f));
+  }
+}
+template <typename E>
+inline hipError_t launch_half_join(const float* partial, int splits, int rows, int64_t total, float beta, E* c, int64_t ldc, const int* order, hipStream_t s) {
+  const int64_t blocks = rows % 4 == 0 ? (total + 1023) / 1024 : (total + 255) / 256;
+  hipLaunchKernelGGL(half_join_kernel<E>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, partial, splits, rows, total, beta, c, ldc, order);
+  return hipGetLastError();
+}
+
+// Which tile, and how many pieces of the reduction.  Measured at k = 4096 (bf16), a round of the 256 compute units takes 90 us with
+// 256 x 256 tiles; 57 us with 128 x 128 tiles two to a unit, 48 us where each has its unit to itself; 39 us in the form for that
+// (eight waves, four slices in LDS).  A reduction is split where the tiles leave units idle: a piece costs about 0.55 us per 64
+// positions, the join a launch and the traffic of its sums.
+enum { TILE_256, TILE_128, TILE_128_ALONE };
+struct TilePlan {
+  int tile, splits;
+  int64_t k_piece;
+};
+inline TilePlan plan_tiles(int64_t m, int64_t n, int64_t k) {
+  const int64_t t128 = ((m + 127) / 128) * ((n + 127) / 128), t256 = ((m + 255) / 256) * ((n + 255) / 256);
+  TilePlan plan = {TILE_128_ALONE, 1, k > 0 ? (k + 63) / 64 * 64 : 64};
+  if (t128 <= 256) {
+    double best = 1e30;
+    for (int64_t s = 1; s * t128 <= 256 && (s == 1 || k / s >= 128) && s <= 32; ++s) {
+      const int64_t piece = ((k + s - 1) / s + 63) / 64 * 64;
+      const double cost = 0.55 * (double)(piece / 64) + (s > 1 ? 2.5 + (double)s * (double)m * (double)n * 8.0 / 4.0e6 : 0.0);
+      if (cost < 0.9 * best) {
+        best = cost;
+        plan.k_piece = piece > 64 ? piece : 64;
+        plan.splits = (int)(k > 0 ? (k + plan.k_piece - 1) / plan.k_piece : 1);
+      }
+    }
+    return plan;
+  }
+  const int64_t full = t128 / 512, rest = t128 % 512;
+  const double small = 57.0 * (double)full + (rest == 0 ? 0.0 : rest <= 256 ? 48.0 : 57.0), large = 90.0 * (double)((t256 + 255) / 256);
+  plan.tile = large <= small ? TILE_256 : TILE_128;
+  return plan;
 }
 
 }  // namespace eigamd

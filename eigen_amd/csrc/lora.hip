@@ -76,17 +76,6 @@ template <typename T> hipError_t launch_project(const ProjectArgs& g, hipStream_
   return launch_project_rank<T, 4>(g, s);
 }
 
-// Sums of a split reduction, in the order of the pieces.
-template <typename E> __global__ __launch_bounds__(256) void lora_join_kernel(HalfGemm g) {
-  const int64_t total = (int64_t)g.m * g.n;
-  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
-    float sum = 0.0f;
-    for (int z = 0; z < g.splits; ++z) sum += g.partial[(int64_t)z * total + q];
-    const int col = (int)(q / g.m), row = (int)(q - (int64_t)col * g.m);
-    static_cast<E*>(g.c)[(int64_t)g.order[col] * g.ldc + row] = (E)sum;
-  }
-}
-
 // Y += s_j op(B_j) P in single precision, behind the plain product.
 __global__ __launch_bounds__(256) void lora_add_f32_kernel(HalfGemm g) {
   const int w = threadIdx.x / 64, l = threadIdx.x & 63;
@@ -108,22 +97,16 @@ __global__ __launch_bounds__(256) void lora_add_f32_kernel(HalfGemm g) {
   }
 }
 
-// Pieces of the reduction for a grid of `tiles` workgroups: enough to fill the 256 compute units about twice, none shorter
-// than 256 positions.
-int choose_pieces(int64_t tiles, int64_t k, int64_t* k_piece) {
-  int64_t want = std::min<int64_t>(std::max<int64_t>(512 / std::max<int64_t>(tiles, 1), 1), std::max<int64_t>(k / 256, 1));
-  const int64_t piece = ((k + want - 1) / want + 63) / 64 * 64;
-  *k_piece = std::max<int64_t>(piece, 64);
-  return (int)std::max<int64_t>((k + *k_piece - 1) / *k_piece, 1);
-}
-
-int64_t tiles128(int64_t m, int64_t n) { return ((m + 127) / 128) * ((n + 127) / 128); }
-int64_t tiles256(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256); }
-
-template <typename T, int LA, int SRC, int B, int WM, int WN> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
-  const dim3 grid((unsigned)(B == 256 ? tiles256(g.m, g.n) : tiles128(g.m, g.n)), g.splits);
-  hipLaunchKernelGGL((half_gemm_kernel<T, LA, SRC, KC, SRC, OUT_HALF, B, B, WM, WN>), grid, dim3(WM * WN * 64), 0, s, g);
+template <typename T, int LA, int SRC, int B, int WM, int WN, int D> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
+  const dim3 grid((unsigned)(((g.m + B - 1) / B) * (((int64_t)g.n + B - 1) / B)), g.splits);
+  hipLaunchKernelGGL((half_gemm_kernel<T, LA, SRC, KC, SRC, OUT_HALF, B, B, WM, WN, D>), grid, dim3(WM * WN * 64), 0, s, g);
   return hipGetLastError();
+}
+template <typename T, int LA> hipError_t launch_form(const HalfGemm& g, bool direct, int tile, hipStream_t s) {
+  if (!direct) return launch_tiles<T, LA, STAGED, 128, 2, 2, 2>(g, s);
+  return tile == TILE_256   ? launch_tiles<T, LA, DIRECT, 256, 2, 4, 2>(g, s)
+         : tile == TILE_128 ? launch_tiles<T, LA, DIRECT, 128, 2, 2, 2>(g, s)
+                            : launch_tiles<T, LA, DIRECT, 128, 2, 4, 4>(g, s);
 }
 
 template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArgs& q, hipStream_t s) {
@@ -142,7 +125,6 @@ template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArg
   g.up_stride = c.stride_b;
   g.p = c.p; g.ldp = c.ldp;
   g.scale = c.scale;
-  g.k_piece = (int)std::max<int64_t>((c.k + 63) / 64 * 64, 64);
   hipError_t e;
   // whole 16-byte chunks everywhere: the loads go to LDS without passing through registers
   const bool w_chunks = (uintptr_t)c.w % 16 == 0 && c.ldw % 8 == 0 && (c.w_trans || c.m % 8 == 0);
@@ -151,26 +133,14 @@ template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArg
     return lora_few_device(c.kind, c.w_trans, g, q, s);
   }
   if (q.none > 0 && (e = launch_project<T>(q, s)) != hipSuccess) return e;
-  int64_t piece = g.k_piece;
-  const int splits = choose_pieces(tiles128(c.m, c.n), c.k, &piece);
-  if (splits > 1 && c.work && c.work_bytes >= (int64_t)splits * c.m * c.n * 4) {
-    g.splits = splits;
-    g.k_piece = (int)piece;
-    g.partial = static_cast<float*>(c.work);
-  }
+  const TilePlan plan = plan_tiles(c.m, c.n, c.k);
+  g.splits = plan.splits;
+  g.k_piece = (int)plan.k_piece;
+  g.partial = static_cast<float*>(c.work);
   const bool direct = w_chunks && (uintptr_t)c.x % 16 == 0 && c.ldx % 8 == 0 && c.k % 8 == 0;
-  if (direct && g.splits == 1 && tiles256(c.m, c.n) >= 200)
-    e = c.w_trans ? launch_tiles<T, KC, DIRECT, 256, 2, 4>(g, s) : launch_tiles<T, MC, DIRECT, 256, 2, 4>(g, s);
-  else if (direct)
-    e = c.w_trans ? launch_tiles<T, KC, DIRECT, 128, 2, 2>(g, s) : launch_tiles<T, MC, DIRECT, 128, 2, 2>(g, s);
-  else
-    e = c.w_trans ? launch_tiles<T, KC, STAGED, 128, 2, 2>(g, s) : launch_tiles<T, MC, STAGED, 128, 2, 2>(g, s);
-  if (e == hipSuccess && g.splits > 1) {
-    const unsigned blocks = (unsigned)std::min<int64_t>((c.m * c.n + 255) / 256, 4096);
-    hipLaunchKernelGGL((lora_join_kernel<typename T::elem>), dim3(blocks), dim3(256), 0, s, g);
-    e = hipGetLastError();
-  }
-  return e;
+  e = c.w_trans ? launch_form<T, KC>(g, direct, plan.tile, s) : launch_form<T, MC>(g, direct, plan.tile, s);
+  if (e != hipSuccess || g.splits == 1) return e;
+  return launch_half_join(g.partial, g.splits, g.m, c.m * c.n, 0.0f, static_cast<typename T::elem*>(g.c), g.ldc, g.order, s);
 }
 
 // ------------------------------------------------------------------------------------------------ gradients of the factors
@@ -388,8 +358,7 @@ hipError_t lora_plan_device(const int* ids, int64_t n, int64_t adapters, int* d_
 int64_t lora_work_bytes(int kind, bool w_trans, int64_t m, int64_t n, int64_t k) {
   if (m <= 0 || n <= 0) return 0;
   if (kind == F32) return std::min<int64_t>(16 * m * n * 4, (int64_t)256 << 20);
-  int64_t piece;
-  const int splits = choose_pieces(tiles128(m, n), k, &piece);
+  const int splits = plan_tiles(m, n, k).splits;
   const int64_t tiles = splits > 1 ? (int64_t)splits * m * n * 4 : 0;
   return lora_few(n) ? std::max<int64_t>(tiles, lora_few_work_bytes(m, n, k)) : tiles;
 }

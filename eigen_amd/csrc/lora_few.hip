@@ -52,7 +52,7 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
     b[c] = static_cast<const E*>(g.b) + (int64_t)g.order[at < g.n ? at : g.n - 1] * g.ldb;
   }
   f32x4 acc[4][NG] = {};
-  constexpr int S = NG == 4 ? 1 : 2, turn = 8 * 32 * S;
+  constexpr int S = NG == 4 ? 1 : NG == 2 || LA == MC ? 2 : 4, turn = 8 * 32 * S;
   x8 fa[2][S][4], fb[2][S][NG];
   auto load = [&](int k0, int set) {
     const bool whole = k0 + 32 * S <= k_end;
