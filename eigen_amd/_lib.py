@@ -124,14 +124,14 @@ _int = ctypes.c_int
 for _name, _res, _args in (
         ("lora_plan_ints", _i64, [_i64] * 2),
         ("lora_plan_dev", _int, [_i64] * 2 + [_vp] * 3),
-        ("lora_work_bytes", _i64, [_int] * 2 + [_i64] * 3),
+        ("lora_work_bytes", _i64, [_int] * 2 + [_i64] * 3 + [_vp, _i64] * 2),
         ("lora_dev", _int, [_int] * 4 + [_i64] * 5 + [_vp, _i64, _vp, _i64] + [_vp, _i64, _i64] * 2 + [_vp, _vp, _vp, _i64, _vp, _i64,
                                                                                                _vp, _i64, _vp]),
         ("lora_wgrad_work_bytes", _i64, [_i64] * 4),
         ("lora_wgrad_dev", _int, [_int] * 2 + [_i64] * 4 + [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp]),
         ("ckpt8_pack_dev", _int, [_int] + [_i64] * 2 + [_vp, _i64] * 3 + [_vp]),
         ("ckpt8_unpack_dev", _int, [_int] + [_i64] * 2 + [_vp, _i64] * 3 + [_vp]),
-        ("ckpt8_wgrad_work_bytes", _i64, [_int] + [_i64] * 3),
+        ("ckpt8_wgrad_work_bytes", _i64, [_int] + [_i64] * 3 + [_vp, _i64]),
         ("ckpt8_wgrad_dev", _int, [_int] * 2 + [_i64] * 3 + [_vp, _i64] * 3 + [_vp, _vp, _i64, _vp, _i64, _vp])):
     _f = getattr(lib, "eigamd_" + _name)
     _f.restype = _res

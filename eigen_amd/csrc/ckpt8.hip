@@ -114,16 +114,19 @@ PackArgs pack_args(int64_t k, int64_t n) {
   return g;
 }
 
-template <typename T, int SRC, int OUT, int B, int WM, int WN> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
-  const dim3 grid((unsigned)(((g.m + B - 1) / B) * ((g.n + B - 1) / B)), g.splits);
-  hipLaunchKernelGGL((half_gemm_kernel<T, MC, QUANT, MC, SRC, OUT, B, B, WM, WN, 2>), grid, dim3(WM * WN * 64), 0, s, g);
+template <typename T, int OUT, int B, int WM, int WN> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
+  const dim3 grid((unsigned)(((g.m + B - 1) / B) * (((int64_t)g.n + B - 1) / B)), g.splits);
+  hipLaunchKernelGGL((half_gemm_kernel<T, MC, QUANT, MC, DIRECT, OUT, B, B, WM, WN, 2>), grid, dim3(WM * WN * 64), 0, s, g);
   return hipGetLastError();
 }
-template <typename T, int OUT> hipError_t launch_out(const HalfGemm& g, bool direct, int tile, hipStream_t s) {
-  if (!direct) return launch_tiles<T, STAGED, OUT, 128, 2, 2>(g, s);
-  return tile == TILE_256   ? launch_tiles<T, DIRECT, OUT, 256, 2, 4>(g, s)
-         : tile == TILE_128 ? launch_tiles<T, DIRECT, OUT, 128, 2, 2>(g, s)
-                            : launch_tiles<T, DIRECT, OUT, 128, 2, 4>(g, s);
+template <typename T, int OUT> hipError_t launch_out(const HalfGemm& g, int tile, hipStream_t s) {
+  return tile == TILE_256   ? launch_tiles<T, OUT, 256, 2, 4>(g, s)
+         : tile == TILE_128 ? launch_tiles<T, OUT, 128, 2, 2>(g, s)
+                            : launch_tiles<T, OUT, 128, 2, 4>(g, s);
+}
+int64_t sums_bytes(int64_t m, int64_t n, int64_t k) {
+  const int splits = plan_tiles(k, m, n).splits;
+  return splits > 1 ? (splits * m * k * 4 + 255) / 256 * 256 : 0;
 }
 
 }  // namespace
@@ -150,11 +153,10 @@ hipError_t ckpt8_unpack_device(int kind, int64_t k, int64_t n, const int8_t* q, 
   return hipGetLastError();
 }
 
-int64_t ckpt8_grad_work_bytes(int kind, int64_t m, int64_t n, int64_t k) {
+int64_t ckpt8_grad_work_bytes(int kind, int64_t m, int64_t n, int64_t k, const void* dy, int64_t lddy) {
   if (m <= 0 || n <= 0 || k <= 0) return 0;
   if (kind == F32) return (k * n * 4 + 255) / 256 * 256 + std::min<int64_t>(16 * m * k * 4, (int64_t)256 << 20);
-  const int splits = plan_tiles(k, m, n).splits;
-  return splits > 1 ? splits * m * k * 4 : 0;
+  return sums_bytes(m, n, k) + (whole_chunks(dy, lddy, m) ? 0 : padded_bytes(m, n));
 }
 
 hipError_t ckpt8_grad_device(const Ckpt8GradArgs& c, hipStream_t s) {
@@ -187,10 +189,15 @@ hipError_t ckpt8_grad_device(const Ckpt8GradArgs& c, hipStream_t s) {
   g.splits = plan.splits;
   g.k_piece = (int)plan.k_piece;
   g.partial = static_cast<float*>(c.work);
-  const bool direct = (uintptr_t)c.dy % 16 == 0 && c.lddy % 8 == 0 && c.m % 8 == 0;
   hipError_t e;
-  if (c.kind == BF16) e = c.trans ? launch_out<Bf16, OUT_F32>(g, direct, plan.tile, s) : launch_out<Bf16, OUT_F32_SWAPPED>(g, direct, plan.tile, s);
-  else e = c.trans ? launch_out<F16, OUT_F32>(g, direct, plan.tile, s) : launch_out<F16, OUT_F32_SWAPPED>(g, direct, plan.tile, s);
+  if (c.n > 0 && !whole_chunks(c.dy, c.lddy, c.m)) {
+    const PadCopy copy = pad_copy(c.dy, c.lddy, c.m, c.n, static_cast<char*>(c.work) + sums_bytes(c.m, c.n, c.k));
+    g.b = copy.to;
+    g.ldb = padded(c.m);
+    if ((e = launch_pad_copy(copy, {}, s)) != hipSuccess) return e;
+  }
+  if (c.kind == BF16) e = c.trans ? launch_out<Bf16, OUT_F32>(g, plan.tile, s) : launch_out<Bf16, OUT_F32_SWAPPED>(g, plan.tile, s);
+  else e = c.trans ? launch_out<F16, OUT_F32>(g, plan.tile, s) : launch_out<F16, OUT_F32_SWAPPED>(g, plan.tile, s);
   if (e != hipSuccess || g.splits == 1) return e;
   return launch_half_join(g.partial, g.splits, (int)(c.trans ? c.k : c.m), c.m * c.k, c.beta, c.dw, c.lddw, (const int*)nullptr, s);
 }

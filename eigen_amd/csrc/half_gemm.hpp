@@ -15,7 +15,7 @@
 namespace eigamd {
 
 enum { KC = 0, MC = 1 };                       // orientation
-enum { DIRECT = 0, STAGED = 1, QUANT = 2 };    // global -> LDS by hardware / through registers, any alignment / from 8 bits
+enum { DIRECT = 0, STAGED = 1, QUANT = 2 };    // global -> LDS by hardware / (factor gradients only) through registers / from 8 bits
 
 struct HalfGemm {
   int m, n, k;
@@ -75,6 +75,7 @@ template <int KEEP> __device__ __forceinline__ void slice_barrier() {
 // a base that is the same in all lanes (256 rows or 64 lines of at most 2^22 elements).
 template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct SliceLoader {
   static_assert(LAY == KC || (R >= 128 && !GATHER), "the permutation of a line needs 16 chunks");
+  static_assert(SRC == DIRECT || (SRC == QUANT && LAY == MC), "what the operators need");
   static constexpr int N = R * 8 / NT;
   static constexpr int bytes = R * 128;
   static constexpr int es = SRC == QUANT ? 1 : 2;
@@ -92,7 +93,6 @@ template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct Slice
   const uint8_t* ebase;
   int64_t lde;
   unsigned eoff;
-  x8 reg[N];
   uint64_t qreg[N];
   unsigned ereg[N];
 
@@ -139,7 +139,6 @@ template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct Slice
     else return LAY == KC ? base + off[i] : base + i * across + off[0];
   }
   __device__ __forceinline__ const uint8_t* exponent_at(int i) const { return ebase + i * (lines * lde) + eoff; }
-  __device__ __forceinline__ int inside(int i) const { return LAY == KC ? left - position(0) : (position(i) < left ? len : 0); }
   __device__ __forceinline__ void next() {
     left -= 64;
     base += step;
@@ -151,35 +150,26 @@ template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct Slice
   }
 
   __device__ __forceinline__ void fetch() {
-    if constexpr (SRC != DIRECT) {
+    if constexpr (SRC == QUANT) {
       if (left <= 0) return;
       if (left >= 72) {
         // Whole loads.  Past the end of a column they run into the next one (there are at least 8 more elements of columns
         // behind this slice), and what they bring belongs to rows that are not stored.
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          if constexpr (SRC == STAGED) {
-            reg[i] = load_8<E, x8>(reinterpret_cast<const E*>(at(i)));
-          } else {
-            __builtin_memcpy(&qreg[i], at(i), 8);
-            ereg[i] = *exponent_at(i);
-          }
+          __builtin_memcpy(&qreg[i], at(i), 8);
+          ereg[i] = *exponent_at(i);
         }
       } else {
-        // element by element, those outside from the zero page
+        // byte by byte, those outside from the zero page
+        const uint8_t* zero = reinterpret_cast<const uint8_t*>(zero_page);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int n = inside(i);
-          if constexpr (SRC == STAGED) {
+          const int n = position(i) < left ? len : 0;
+          qreg[i] = 0;
 #pragma unroll
-            for (int t = 0; t < 8; ++t) reg[i][t] = *(t < n ? reinterpret_cast<const E*>(at(i)) + t : reinterpret_cast<const E*>(zero_page));
-          } else {
-            qreg[i] = 0;
-#pragma unroll
-            for (int t = 0; t < 8; ++t)
-              qreg[i] |= (uint64_t)*(t < n ? reinterpret_cast<const uint8_t*>(at(i)) + t : reinterpret_cast<const uint8_t*>(zero_page)) << (8 * t);
-            ereg[i] = *(n > 0 ? exponent_at(i) : reinterpret_cast<const uint8_t*>(zero_page));
-          }
+          for (int t = 0; t < 8; ++t) qreg[i] |= (uint64_t)*(t < n ? reinterpret_cast<const uint8_t*>(at(i)) + t : zero) << (8 * t);
+          ereg[i] = *(n > 0 ? exponent_at(i) : zero);
         }
       }
       next();
@@ -199,7 +189,7 @@ template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct Slice
           else load_to_lds(base + i * across, off[0], to + i * NT * 16);
         }
       } else {
-        // whole chunks only (the launcher checks extents); those outside: zeros
+        // Whole chunks (the launcher sees to that; one that the reduction ends in has zeros behind its end); those outside: zeros.
 #pragma unroll
         for (int i = 0; i < N; ++i)
           load_to_lds((LAY == KC ? position(0) : position(i)) < left ? at(i) : reinterpret_cast<const char*>(zero_page), to + i * NT * 16);
@@ -208,15 +198,11 @@ template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct Slice
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
+        // |q| <= 127 has 7 bits, so q * 2^e is exact in either type (the packing keeps the exponent in the type's range)
         x8 v;
-        if constexpr (SRC == STAGED) {
-          v = reg[i];
-        } else {
-          // |q| <= 127 has 7 bits, so q * 2^e is exact in either type (the packing keeps the exponent in the type's range)
-          const float sc = exponent_scale(ereg[i]);
+        const float sc = exponent_scale(ereg[i]);
 #pragma unroll
-          for (int t = 0; t < 8; ++t) v[t] = (E)((float)(int8_t)(qreg[i] >> (8 * t)) * sc);
-        }
+        for (int t = 0; t < 8; ++t) v[t] = (E)((float)(int8_t)(qreg[i] >> (8 * t)) * sc);
         *reinterpret_cast<x8*>(lds + (threadIdx.x + i * NT) * 16) = v;
       }
     }
@@ -295,30 +281,36 @@ __device__ __forceinline__ void add_adapters(const HalfGemm& g, int row0, int co
           }
         }
       }
+      // four row blocks' factors under way together
+      constexpr int GI = NI < 4 ? NI : 4;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        int row = row0 + i * 16 + (l & 15);
-        asm("" : "+v"(row));   // addresses are made here, not kept for every row block across the loops
-        x8 u;
-        const E* at = up + (int64_t)row * g.up_row + (int64_t)r * g.up_rank;
-        const int n = row < g.m ? rn : 0;
-        if (g.up_rank == 1) {
-          u = load_up_to_8<E, x8>(at, n);
-        } else {
+      for (int i0 = 0; i0 < NI; i0 += GI) {
+        x8 u[GI];
 #pragma unroll
-          for (int t = 0; t < 8; ++t) u[t] = t < n ? at[(int64_t)t * g.up_rank] : (E)0.0f;
+        for (int i = 0; i < GI; ++i) {
+          int row = row0 + (i0 + i) * 16 + (l & 15);
+          asm("" : "+v"(row));   // addresses are made here, not kept for every row block across the loops
+          const E* at = up + (int64_t)row * g.up_row + (int64_t)r * g.up_rank;
+          const int n = row < g.m ? rn : 0;
+          if (g.up_rank == 1) {
+            u[i] = load_up_to_8<E, x8>(at, n);
+          } else {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) u[i][t] = t < n ? at[(int64_t)t * g.up_rank] : (E)0.0f;
+          }
         }
+#pragma unroll
+        for (int i = 0; i < GI; ++i)
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           if (!((mask >> (j * 16)) & 0xffff)) continue;
           f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
-          if constexpr (T::bytes == 2) d = T::mma(u, lo[j], d);
-          d = T::mma(u, hi[j], d);
+          if constexpr (T::bytes == 2) d = T::mma(u[i], lo[j], d);
+          d = T::mma(u[i], hi[j], d);
           const bool on = (mask >> (j * 16 + (l & 15))) & 1;
 #pragma unroll
-          for (int t = 0; t < 4; ++t) acc[i][j][t] += on ? d[t] * back[j] : 0.0f;
+          for (int t = 0; t < 4; ++t) acc[i0 + i][j][t] += on ? d[t] * back[j] : 0.0f;
         }
-        __builtin_amdgcn_sched_barrier(0);   // one row block's factors in registers at a time
       }
     }
   }
@@ -518,6 +510,48 @@ __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
         }
       }
   }
+}
+
+// The direct loads take whole, aligned 16-byte chunks.  A matrix that has others (an odd leading dimension, an extent that is no
+// multiple of 8) is copied into scratch memory first, columns padded with zeros: reading it in place through registers took
+// 378 us for 4096 tokens x 4095 x 4093, copies and product take 190 (4096 x 4096: 126).
+inline bool whole_chunks(const void* p, int64_t ld, int64_t rows) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && rows % 8 == 0; }
+inline int64_t padded(int64_t rows) { return (rows + 7) / 8 * 8; }
+inline int64_t padded_bytes(int64_t rows, int64_t cols) { return (padded(rows) * cols * 2 + 255) / 256 * 256; }
+struct PadCopy {
+  const uint16_t* from;
+  int64_t ld;
+  int rows;
+  int64_t chunks;        // of 8 elements, in all; 0: nothing to copy
+  uint16_t* to;
+};
+inline PadCopy pad_copy(const void* from, int64_t ld, int64_t rows, int64_t cols, void* to) {
+  return {static_cast<const uint16_t*>(from), ld, (int)rows, padded(rows) / 8 * cols, static_cast<uint16_t*>(to)};
+}
+static __global__ __launch_bounds__(256) void pad_copy_kernel(PadCopy a, PadCopy b) {
+  using u16x8 = uint16_t __attribute__((ext_vector_type(8)));
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < a.chunks + b.chunks; q += (int64_t)gridDim.x * 256) {
+    const PadCopy& m = q < a.chunks ? a : b;
+    const int64_t ch = q < a.chunks ? q : q - a.chunks;
+    const int per = (m.rows + 7) / 8;
+    const int64_t col = ch / per;
+    const int row = (int)(ch - col * per) * 8;
+    const uint16_t* from = m.from + col * m.ld + row;
+    u16x8 v;
+    if (row + 8 <= m.rows) {
+      __builtin_memcpy(&v, from, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = row + i < m.rows ? from[i] : 0;
+    }
+    *reinterpret_cast<u16x8*>(m.to + ch * 8) = v;
+  }
+}
+inline hipError_t launch_pad_copy(const PadCopy& a, const PadCopy& b, hipStream_t s) {
+  const int64_t blocks = (a.chunks + b.chunks + 255) / 256;
+  if (blocks == 0) return hipSuccess;
+  hipLaunchKernelGGL(pad_copy_kernel, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, a, b);
+  return hipGetLastError();
 }
 
 // Sums of a split reduction in the order of the pieces, four rows a thread: C = beta C + sum (C in the operands' type: beta is 0).

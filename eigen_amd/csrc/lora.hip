@@ -97,16 +97,35 @@ __global__ __launch_bounds__(256) void lora_add_f32_kernel(HalfGemm g) {
   }
 }
 
-template <typename T, int LA, int SRC, int B, int WM, int WN, int D> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
+template <typename T, int LA, int B, int WM, int WN, int D> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
   const dim3 grid((unsigned)(((g.m + B - 1) / B) * (((int64_t)g.n + B - 1) / B)), g.splits);
-  hipLaunchKernelGGL((half_gemm_kernel<T, LA, SRC, KC, SRC, OUT_HALF, B, B, WM, WN, D>), grid, dim3(WM * WN * 64), 0, s, g);
+  hipLaunchKernelGGL((half_gemm_kernel<T, LA, DIRECT, KC, DIRECT, OUT_HALF, B, B, WM, WN, D>), grid, dim3(WM * WN * 64), 0, s, g);
   return hipGetLastError();
 }
-template <typename T, int LA> hipError_t launch_form(const HalfGemm& g, bool direct, int tile, hipStream_t s) {
-  if (!direct) return launch_tiles<T, LA, STAGED, 128, 2, 2, 2>(g, s);
-  return tile == TILE_256   ? launch_tiles<T, LA, DIRECT, 256, 2, 4, 2>(g, s)
-         : tile == TILE_128 ? launch_tiles<T, LA, DIRECT, 128, 2, 2, 2>(g, s)
-                            : launch_tiles<T, LA, DIRECT, 128, 2, 4, 4>(g, s);
+template <typename T, int LA> hipError_t launch_form(const HalfGemm& g, int tile, hipStream_t s) {
+  return tile == TILE_256   ? launch_tiles<T, LA, 256, 2, 4, 2>(g, s)
+         : tile == TILE_128 ? launch_tiles<T, LA, 128, 2, 2, 2>(g, s)
+                            : launch_tiles<T, LA, 128, 2, 4, 4>(g, s);
+}
+
+// What a call keeps in its scratch memory: sums of a split reduction, then copies of W and of X with whole chunks (launch_half).
+struct HalfWork {
+  int64_t sums, w_copy, x_copy;
+};
+HalfWork half_work(bool w_trans, int64_t m, int64_t n, int64_t k, const void* w, int64_t ldw, const void* x, int64_t ldx) {
+  HalfWork need = {0, 0, 0};
+  const bool w_whole = whole_chunks(w, ldw, w_trans ? k : m);
+  if (lora_few(n)) {
+    need.sums = lora_few_work_bytes(m, n, k);      // (W's reduction contiguous: read where it is, whatever its alignment)
+    if (!w_trans && !w_whole) need.w_copy = padded_bytes(m, k);
+  } else {
+    const int splits = plan_tiles(m, n, k).splits;
+    if (splits > 1) need.sums = (int64_t)splits * m * n * 4;
+    if (!w_whole) need.w_copy = w_trans ? padded_bytes(k, m) : padded_bytes(m, k);
+    if (!whole_chunks(x, ldx, k)) need.x_copy = padded_bytes(k, n);
+  }
+  need.sums = (need.sums + 255) / 256 * 256;
+  return need;
 }
 
 template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArgs& q, hipStream_t s) {
@@ -125,20 +144,28 @@ template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArg
   g.up_stride = c.stride_b;
   g.p = c.p; g.ldp = c.ldp;
   g.scale = c.scale;
-  hipError_t e;
-  // whole 16-byte chunks everywhere: the loads go to LDS without passing through registers
-  const bool w_chunks = (uintptr_t)c.w % 16 == 0 && c.ldw % 8 == 0 && (c.w_trans || c.m % 8 == 0);
-  if (lora_few(c.n) && (c.w_trans || w_chunks)) {
-    g.partial = static_cast<float*>(c.work);
-    return lora_few_device(c.kind, c.w_trans, g, q, s);
+  const HalfWork need = half_work(c.w_trans, c.m, c.n, c.k, c.w, c.ldw, c.x, c.ldx);
+  char* work = static_cast<char*>(c.work);
+  g.partial = reinterpret_cast<float*>(work);
+  PadCopy w_copy = {}, x_copy = {};
+  if (need.w_copy) {
+    w_copy = pad_copy(c.w, c.ldw, c.w_trans ? c.k : c.m, c.w_trans ? c.m : c.k, work + need.sums);
+    g.a = w_copy.to;
+    g.lda = padded(c.w_trans ? c.k : c.m);
   }
+  if (need.x_copy) {
+    x_copy = pad_copy(c.x, c.ldx, c.k, c.n, work + need.sums + need.w_copy);
+    g.b = x_copy.to;
+    g.ldb = padded(c.k);
+  }
+  hipError_t e = launch_pad_copy(w_copy, x_copy, s);
+  if (e != hipSuccess) return e;
+  if (lora_few(c.n)) return lora_few_device(c.kind, c.w_trans, g, q, s);
   if (q.none > 0 && (e = launch_project<T>(q, s)) != hipSuccess) return e;
   const TilePlan plan = plan_tiles(c.m, c.n, c.k);
   g.splits = plan.splits;
   g.k_piece = (int)plan.k_piece;
-  g.partial = static_cast<float*>(c.work);
-  const bool direct = w_chunks && (uintptr_t)c.x % 16 == 0 && c.ldx % 8 == 0 && c.k % 8 == 0;
-  e = c.w_trans ? launch_form<T, KC>(g, direct, plan.tile, s) : launch_form<T, MC>(g, direct, plan.tile, s);
+  e = c.w_trans ? launch_form<T, KC>(g, plan.tile, s) : launch_form<T, MC>(g, plan.tile, s);
   if (e != hipSuccess || g.splits == 1) return e;
   return launch_half_join(g.partial, g.splits, g.m, c.m * c.n, 0.0f, static_cast<typename T::elem*>(g.c), g.ldc, g.order, s);
 }
@@ -355,12 +382,11 @@ hipError_t lora_plan_device(const int* ids, int64_t n, int64_t adapters, int* d_
   return hipGetLastError();
 }
 
-int64_t lora_work_bytes(int kind, bool w_trans, int64_t m, int64_t n, int64_t k) {
+int64_t lora_work_bytes(int kind, bool w_trans, int64_t m, int64_t n, int64_t k, const void* w, int64_t ldw, const void* x, int64_t ldx) {
   if (m <= 0 || n <= 0) return 0;
   if (kind == F32) return std::min<int64_t>(16 * m * n * 4, (int64_t)256 << 20);
-  const int splits = plan_tiles(m, n, k).splits;
-  const int64_t tiles = splits > 1 ? (int64_t)splits * m * n * 4 : 0;
-  return lora_few(n) ? std::max<int64_t>(tiles, lora_few_work_bytes(m, n, k)) : tiles;
+  const HalfWork need = half_work(w_trans, m, n, k, w, ldw, x, ldx);
+  return need.sums + need.w_copy + need.x_copy;
 }
 
 hipError_t lora_device(const LoraArgs& c, hipStream_t s) {

@@ -36,7 +36,7 @@ struct LoraArgs {
 };
 
 hipError_t lora_plan_device(const int* ids, int64_t n, int64_t adapters, int* d_plan, hipStream_t s);
-int64_t lora_work_bytes(int kind, bool w_trans, int64_t m, int64_t n, int64_t k);
+int64_t lora_work_bytes(int kind, bool w_trans, int64_t m, int64_t n, int64_t k, const void* w, int64_t ldw, const void* x, int64_t ldx);
 hipError_t lora_device(const LoraArgs& c, hipStream_t s);
 
 struct LoraGradArgs {
@@ -71,7 +71,7 @@ struct Ckpt8GradArgs {
   float* dw; int64_t lddw;
   void* work; int64_t work_bytes;
 };
-int64_t ckpt8_grad_work_bytes(int kind, int64_t m, int64_t n, int64_t k);
+int64_t ckpt8_grad_work_bytes(int kind, int64_t m, int64_t n, int64_t k, const void* dy, int64_t lddy);
 hipError_t ckpt8_grad_device(const Ckpt8GradArgs& c, hipStream_t s);
 
 }  // namespace eigamd

@@ -57,10 +57,11 @@ int eigamd_lora_plan_dev(int64_t n, int64_t n_adapters, const int32_t* d_adapter
   return done(me, lora_plan_device(d_adapter_of, n, n_adapters, d_plan, static_cast<hipStream_t>(stream)));
 }
 
-int64_t eigamd_lora_work_bytes(int dtype, int opw, int64_t m, int64_t n, int64_t k) {
+int64_t eigamd_lora_work_bytes(int dtype, int opw, int64_t m, int64_t n, int64_t k, const void* d_w, int64_t ldw, const void* d_x,
+                               int64_t ldx) {
   if (!kind_ok(dtype) || !op_ok(opw) || !extent_ok(m, kMaxFeatures) || !extent_ok(n, kMaxTokens) || !extent_ok(k, kMaxFeatures))
     return -1;
-  return lora_work_bytes(dtype, opw == EIGAMD_OP_T, m, n, k);
+  return lora_work_bytes(dtype, opw == EIGAMD_OP_T, m, n, k, d_w, ldw, d_x, ldx);
 }
 
 int eigamd_lora_dev(int dtype, int opw, int opa, int opb, int64_t m, int64_t n, int64_t k, int64_t rank, int64_t n_adapters,
@@ -87,7 +88,7 @@ int eigamd_lora_dev(int dtype, int opw, int opa, int opb, int64_t m, int64_t n, 
   if (n == 0 || (m == 0 && n_adapters == 0)) return EIGAMD_OK;
   if (!d_plan) return bad(me, "plan is null");
   if (d_y == d_x || (m > 0 && k > 0 && d_y == d_w)) return bad(me, "Y overlaps an input");
-  if (!work_ok(d_work, work_bytes, lora_work_bytes(dtype, wt, m, n, k))) return bad(me, "work is smaller than eigamd_lora_work_bytes or not 16-byte aligned");
+  if (!work_ok(d_work, work_bytes, lora_work_bytes(dtype, wt, m, n, k, d_w, ldw, d_x, ldx))) return bad(me, "work is smaller than eigamd_lora_work_bytes or not 16-byte aligned");
   int rc = abi_ensure_device();
   if (rc != EIGAMD_OK) return rc;
   LoraArgs c;
@@ -178,9 +179,9 @@ int eigamd_ckpt8_unpack_dev(int dtype, int64_t k, int64_t n, const int8_t* d_q, 
   return done(me, ckpt8_unpack_device(dtype, k, n, d_q, ldq, d_exponents, lde, d_x, ldx, static_cast<hipStream_t>(stream)));
 }
 
-int64_t eigamd_ckpt8_wgrad_work_bytes(int dtype, int64_t m, int64_t n, int64_t k) {
+int64_t eigamd_ckpt8_wgrad_work_bytes(int dtype, int64_t m, int64_t n, int64_t k, const void* d_dy, int64_t lddy) {
   if (!kind_ok(dtype) || !extent_ok(m, kMaxFeatures) || !extent_ok(n, kMaxTokens) || !extent_ok(k, kMaxFeatures)) return -1;
-  return ckpt8_grad_work_bytes(dtype, m, n, k);
+  return ckpt8_grad_work_bytes(dtype, m, n, k, d_dy, lddy);
 }
 
 int eigamd_ckpt8_wgrad_dev(int dtype, int opw, int64_t m, int64_t n, int64_t k, const void* d_dy, int64_t lddy, const int8_t* d_q,
@@ -197,7 +198,7 @@ int eigamd_ckpt8_wgrad_dev(int dtype, int opw, int64_t m, int64_t n, int64_t k, 
   if (!matrix_ok(d_dw, wt ? k : m, wt ? m : k, lddw, 4)) return bad(me, "dW: pointer, alignment or leading dimension");
   if (!beta) return bad(me, "beta is null");
   if (m == 0 || k == 0) return EIGAMD_OK;
-  if (!work_ok(d_work, work_bytes, ckpt8_grad_work_bytes(dtype, m, n, k)))
+  if (!work_ok(d_work, work_bytes, ckpt8_grad_work_bytes(dtype, m, n, k, d_dy, lddy)))
     return bad(me, "work is smaller than eigamd_ckpt8_wgrad_work_bytes or not 16-byte aligned");
   int rc = abi_ensure_device();
   if (rc != EIGAMD_OK) return rc;

@@ -164,7 +164,7 @@ def lora_plan(adapter_of, n_adapters, stream=None):
 def lora_work_bytes(opw, w, x):
     """Bytes of ``work`` that ``lora_dev`` needs for these operands."""
     o = _op(opw)
-    return lib.eigamd_lora_work_bytes(w.kind, o, _turned(o, w.rows, w.cols)[0], x.cols, x.rows)
+    return lib.eigamd_lora_work_bytes(w.kind, o, _turned(o, w.rows, w.cols)[0], x.cols, x.rows, w.ptr, w.ld, x.ptr, x.ld)
 
 
 def lora_dev(opw, w, x, opa, a, opb, b, scale, plan, p, y, work=None, stream=None):
@@ -189,7 +189,7 @@ def lora_dev(opw, w, x, opa, a, opb, b, scale, plan, p, y, work=None, stream=Non
     _check_vector(scale, plan.n_adapters, torch.float32, "scale")
     count = plan.n_adapters
     _run("eigamd_lora_dev", stream, (x.storage, w.storage, a.storage, b.storage, scale, plan.storage, p.storage, y.storage),
-         lib.eigamd_lora_work_bytes(kind, ow, m, n, k), work,
+         lib.eigamd_lora_work_bytes(kind, ow, m, n, k, w.ptr, w.ld, x.ptr, x.ld), work,
          lambda s, at, have: lib.eigamd_lora_dev(kind, ow, oa, ob, m, n, k, rank, count, w.ptr, w.ld, x.ptr, x.ld, a.ptr, a.ld, a.stride,
                                                  b.ptr, b.ld, b.stride, scale.data_ptr(), plan.storage.data_ptr(), p.ptr, p.ld, y.ptr, y.ld,
                                                  at, have, s))
@@ -251,7 +251,7 @@ def ckpt8_wgrad_dev(opw, dy, c, beta, dw, work=None, stream=None):
     _check_matrix(dy, c.kind, m, n, "dy")
     _check_matrix(dw, _lib.F32, *_turned(ow, m, k), "dw")
     be = ctypes.c_float(beta)
-    _run("eigamd_ckpt8_wgrad_dev", stream, (dy.storage, c.storage, c.exponents, dw.storage), lib.eigamd_ckpt8_wgrad_work_bytes(c.kind, m, n, k), work,
+    _run("eigamd_ckpt8_wgrad_dev", stream, (dy.storage, c.storage, c.exponents, dw.storage), lib.eigamd_ckpt8_wgrad_work_bytes(c.kind, m, n, k, dy.ptr, dy.ld), work,
          lambda s, at, have: lib.eigamd_ckpt8_wgrad_dev(c.kind, ow, m, n, k, dy.ptr, dy.ld, c.ptr, c.ld, c.exponents.data_ptr(), c.lde,
                                                         ctypes.byref(be), dw.ptr, dw.ld, at, have, s))
     return dw

@@ -437,12 +437,14 @@ int eigamd_trmm_dev(int dtype, int side, int uplo, int op, int diag, int64_t m, 
  * beta = 0 G is not read.
  *
  * Limits: m, k, rows <= 2^22, n <= 2^24, rank 1..256, n_adapters <= 4096; n = 0 and n_adapters = 0 are allowed.  d_work is
- * device memory of at least the bytes the matching query names (16-byte aligned; 0: may be NULL), free again behind the call;
+ * device memory of at least the bytes the matching query names (16-byte aligned; 0: may be NULL; it depends on the operands'
+ * alignment: one without whole aligned 16-byte chunks along its columns may be copied there), free again behind the call;
  * calls that may overlap need one each, so do captured graphs.  Everything is asynchronous on `stream`, allocates nothing, and
  * gives the same bits every time.  Outputs must not overlap inputs.  The queries return -1 for arguments out of range. */
 int64_t eigamd_lora_plan_ints(int64_t n, int64_t n_adapters);
 int eigamd_lora_plan_dev(int64_t n, int64_t n_adapters, const int32_t* d_adapter_of, int32_t* d_plan, void* stream);
-int64_t eigamd_lora_work_bytes(int dtype, int opw, int64_t m, int64_t n, int64_t k);
+int64_t eigamd_lora_work_bytes(int dtype, int opw, int64_t m, int64_t n, int64_t k, const void* d_w, int64_t ldw, const void* d_x,
+                               int64_t ldx);
 int eigamd_lora_dev(int dtype, int opw, int opa, int opb, int64_t m, int64_t n, int64_t k, int64_t rank, int64_t n_adapters,
                     const void* d_w, int64_t ldw, const void* d_x, int64_t ldx, const void* d_a, int64_t lda, int64_t stride_a,
                     const void* d_b, int64_t ldb, int64_t stride_b, const float* d_scale, const int32_t* d_plan, float* d_p,
@@ -469,7 +471,7 @@ int eigamd_ckpt8_pack_dev(int dtype, int64_t k, int64_t n, const void* d_x, int6
                           uint8_t* d_exponents, int64_t lde, void* stream);
 int eigamd_ckpt8_unpack_dev(int dtype, int64_t k, int64_t n, const int8_t* d_q, int64_t ldq, const uint8_t* d_exponents, int64_t lde,
                             void* d_x, int64_t ldx, void* stream);
-int64_t eigamd_ckpt8_wgrad_work_bytes(int dtype, int64_t m, int64_t n, int64_t k);
+int64_t eigamd_ckpt8_wgrad_work_bytes(int dtype, int64_t m, int64_t n, int64_t k, const void* d_dy, int64_t lddy);
 int eigamd_ckpt8_wgrad_dev(int dtype, int opw, int64_t m, int64_t n, int64_t k, const void* d_dy, int64_t lddy, const int8_t* d_q,
                            int64_t ldq, const uint8_t* d_exponents, int64_t lde, const float* beta, float* d_dw, int64_t lddw,
                            void* d_work, int64_t work_bytes, void* stream);

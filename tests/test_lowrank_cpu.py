@@ -18,10 +18,10 @@ ONE = np.ones(1, dtype=np.float32)
 BETA = ctypes.c_void_p(ONE.ctypes.data)
 # m, n, k, rank, adapters = 4, 3, 5, 2, 2 everywhere
 LORA = dict(dtype=_lib.BF16, opw=0, opa=0, opb=0, m=4, n=3, k=5, rank=2, count=2, w=P, ldw=4, x=P, ldx=5, a=P, lda=2, sa=10, b=P, ldb=4, sb=8,
-            scale=P, plan=P, p=P, ldp=2, y=Q, ldy=4, work=NULL, bytes=0, stream=NULL)
+            scale=P, plan=P, p=P, ldp=2, y=Q, ldy=4, work=P, bytes=8192, stream=NULL)
 GRAD = dict(dtype=_lib.F16, opg=0, rows=4, n=3, rank=2, count=2, u=P, ldu=4, e=NULL, lde=0, p=P, ldp=2, scale=P, plan=P, beta=BETA, g=Q, ldg=4,
             sg=8, work=NULL, bytes=0, stream=NULL)
-WGRAD = dict(dtype=_lib.BF16, opw=0, m=4, n=3, k=5, dy=P, lddy=4, q=P, ldq=5, e=P, lde=1, beta=BETA, dw=Q, lddw=4, work=NULL, bytes=0, stream=NULL)
+WGRAD = dict(dtype=_lib.BF16, opw=0, m=4, n=3, k=5, dy=P, lddy=4, q=P, ldq=5, e=P, lde=1, beta=BETA, dw=Q, lddw=4, work=P, bytes=8192, stream=NULL)
 
 
 def call(fn, base, **change):
@@ -35,7 +35,8 @@ def call(fn, base, **change):
     dict(m=2 ** 22 + 1), dict(n=2 ** 24 + 1), dict(rank=0), dict(rank=257), dict(count=-1), dict(count=4097), dict(ldw=3), dict(opw=1, ldw=4),
     dict(ldx=4), dict(ldy=3), dict(lda=1), dict(opa=1, lda=4), dict(ldb=3), dict(opb=1, ldb=1), dict(ldp=1), dict(sa=-1), dict(sb=-1),
     dict(w=NULL), dict(x=NULL), dict(y=NULL), dict(a=NULL), dict(b=NULL), dict(p=NULL), dict(scale=NULL), dict(plan=NULL),
-    dict(x=ctypes.c_void_p(P.value + 1)), dict(p=ctypes.c_void_p(P.value + 2)), dict(y=P), dict(dtype=_lib.F32, work=NULL)])
+    dict(x=ctypes.c_void_p(P.value + 1)), dict(p=ctypes.c_void_p(P.value + 2)), dict(y=P), dict(work=NULL), dict(bytes=511),
+    dict(work=ctypes.c_void_p(P.value + 4)), dict(dtype=_lib.F32, work=NULL)])
 def test_lora_refuses(change):
     assert call(lib.eigamd_lora_dev, LORA, **change) == _lib.ERR_ARG
     assert b"eigamd_lora_dev" in lib.eigamd_last_error()
@@ -52,7 +53,7 @@ def test_lora_wgrad_refuses(change):
 
 @pytest.mark.parametrize("change", [
     dict(dtype=_lib.F64), dict(opw=2), dict(m=-1), dict(n=-1), dict(k=2 ** 23), dict(lddy=3), dict(ldq=4), dict(lde=0), dict(lddw=3),
-    dict(opw=1, lddw=4), dict(dy=NULL), dict(q=NULL), dict(e=NULL), dict(dw=NULL), dict(beta=NULL), dict(dtype=_lib.F32, work=NULL),
+    dict(opw=1, lddw=4), dict(dy=NULL), dict(q=NULL), dict(e=NULL), dict(dw=NULL), dict(beta=NULL), dict(dtype=_lib.F32, work=NULL), dict(work=NULL),
     dict(dw=ctypes.c_void_p(Q.value + 1))])
 def test_ckpt8_wgrad_refuses(change):
     assert call(lib.eigamd_ckpt8_wgrad_dev, WGRAD, **change) == _lib.ERR_ARG
@@ -77,10 +78,10 @@ def test_plan_checks_and_sizes():
     assert lib.eigamd_lora_plan_ints(-1, 3) == -1 and lib.eigamd_lora_plan_ints(3, 4097) == -1
     assert lib.eigamd_lora_plan_dev(3, 2, NULL, P, NULL) == _lib.ERR_ARG
     assert lib.eigamd_lora_plan_dev(3, 2, P, NULL, NULL) == _lib.ERR_ARG
-    assert lib.eigamd_lora_work_bytes(_lib.F64, 0, 4, 4, 4) == -1
-    assert lib.eigamd_lora_work_bytes(_lib.BF16, 0, 0, 4, 4) == 0
+    assert lib.eigamd_lora_work_bytes(_lib.F64, 0, 4, 4, 4, P, 4, P, 4) == -1
+    assert lib.eigamd_lora_work_bytes(_lib.BF16, 0, 0, 4, 4, P, 4, P, 4) == 0
     assert lib.eigamd_lora_wgrad_work_bytes(4, 4, 0, 1) == -1
-    assert lib.eigamd_ckpt8_wgrad_work_bytes(_lib.BF16, -1, 4, 4) == -1
+    assert lib.eigamd_ckpt8_wgrad_work_bytes(_lib.BF16, -1, 4, 4, P, 4) == -1
 
 
 def test_nothing_to_do_needs_no_device():
