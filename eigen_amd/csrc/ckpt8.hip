@@ -19,8 +19,33 @@ namespace {
 
 // Limits of a type: smallest exponent of a scale (f16: its subnormals are whole multiples of 2^-24), and the exponent of its
 // largest values, above which 127 2^e would leave the type and q stops at 63.
-template <typename T> struct Range { static constexpr int low = -126, top = 127; };
-template <> struct Range<F16> { static constexpr int low = -24, top = 15; };
+template <typename T> struct Range { static constexpr int low = -126, top = 127; static constexpr unsigned infinity = 0x7f80; };
+template <> struct Range<F16> { static constexpr int low = -24, top = 15; static constexpr unsigned infinity = 0x7c00; };
+template <> struct Range<Fp32> { static constexpr int low = -126, top = 127; static constexpr unsigned infinity = 0x7f800000; };
+
+// Largest magnitude of 8 values, as the type's bits without the sign: their order is that of the magnitudes, and everything that
+// is not finite is at or above infinity's.
+template <typename T> __device__ __forceinline__ unsigned largest_bits(typename T::x8 v) {
+  if constexpr (T::bytes == 2) {
+    using u16x2 = uint16_t __attribute__((ext_vector_type(2)));
+    using u16x8 = uint16_t __attribute__((ext_vector_type(8)));
+    const u16x8 b = __builtin_bit_cast(u16x8, v) & (uint16_t)0x7fff;
+    u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(b.s01, b.s23), __builtin_elementwise_max(b.s45, b.s67));
+    return m.x > m.y ? m.x : m.y;
+  } else {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned b = __float_as_uint(v[i]) & 0x7fffffff;
+      m = m > b ? m : b;
+    }
+    return m;
+  }
+}
+template <typename T> __device__ __forceinline__ float value_of_bits(unsigned b) {
+  if constexpr (T::bytes == 4) return __uint_as_float(b);
+  else return (float)__builtin_bit_cast(typename T::elem, (uint16_t)b);
+}
 
 struct PackArgs {
   int k, chunks;          // features; chunks of 8 features a token takes (whole blocks of 32)
@@ -31,8 +56,8 @@ struct PackArgs {
   void* out;
 };
 
-__device__ __forceinline__ bool chunk_of(const PackArgs& g, int64_t& token, int& c) {
-  const int64_t first = (int64_t)blockIdx.x * 256;         // one 64-bit division per workgroup
+// Chunk `first` + this thread of the whole matrix; first is the workgroup's, so the 64-bit division is done once.
+__device__ __forceinline__ bool chunk_of(const PackArgs& g, int64_t first, int64_t& token, int& c) {
   const int64_t t0 = first / g.chunks;
   const unsigned in = (unsigned)(first - t0 * g.chunks) + threadIdx.x;
   token = t0 + in / (unsigned)g.chunks;
@@ -40,70 +65,91 @@ __device__ __forceinline__ bool chunk_of(const PackArgs& g, int64_t& token, int&
   return first + threadIdx.x < g.total;
 }
 
-// A thread takes 8 features, four neighbours a block (`chunks` is a multiple of 4, so a block never leaves its wave).
-template <typename T> __global__ __launch_bounds__(256) void ckpt8_pack_kernel(PackArgs g) {
+// A thread takes 8 features, four neighbours a block (`chunks` is a multiple of 4, so a block never leaves its wave), and U such
+// chunks with all their loads under way at once: 4 from 2^20 chunks on, 1 below, where every chunk is wanted at once.
+template <typename T, int U> __global__ __launch_bounds__(256) void ckpt8_pack_kernel(PackArgs g) {
   using E = typename T::elem;
   using x8 = typename T::x8;
-  int64_t token;
-  int c;
-  const bool on = chunk_of(g, token, c);
-  const int n = on ? g.k - c * 8 : 0;
-  const x8 v = load_up_to_8<E, x8>(static_cast<const E*>(g.x) + token * g.ldx + c * 8, n);
-  float top = 0.0f;
-  bool bad = false;
+  int64_t token[U];
+  int c[U], n[U];
+  x8 v[U];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = __builtin_fabsf((float)v[i]);
-    bad |= !(a < __builtin_inff());
-    top = fmaxf(top, a);
+  for (int u = 0; u < U; ++u) {
+    n[u] = chunk_of(g, ((int64_t)blockIdx.x * U + u) * 256, token[u], c[u]) ? g.k - c[u] * 8 : 0;
+    v[u] = load_up_to_8<E, x8>(static_cast<const E*>(g.x) + token[u] * g.ldx + c[u] * 8, n[u]);
   }
-  top = fmaxf(top, __shfl_xor(top, 1));
-  top = fmaxf(top, __shfl_xor(top, 2));
-  int flag = bad;
-  flag |= __shfl_xor(flag, 1);
-  flag |= __shfl_xor(flag, 2);
-  if (!on) return;
-  const int bits = __float_as_int(top);
-  int e = (bits >> 23) - 127 - ((bits & 0x7fffff) > 0x7e0000 ? 5 : 6);     // 127 = 1.984375 * 2^6
-  e = e < Range<T>::low ? Range<T>::low : e;
-  const float most = e > Range<T>::top - 6 ? 63.0f : 127.0f, inverse = __int_as_float((127 - e) << 23);
-  uint64_t q = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float r = rintf((float)v[i] * inverse);
-    r = fminf(fmaxf(r, -most), most);
-    q |= (uint64_t)(uint8_t)(int8_t)(int)(flag ? 0.0f : r) << (8 * i);
+  for (int u = 0; u < U; ++u) {
+    unsigned top = largest_bits<T>(v[u]);
+    unsigned other = __shfl_xor(top, 1);
+    top = top > other ? top : other;
+    other = __shfl_xor(top, 2);
+    top = top > other ? top : other;
+    const bool flag = top >= Range<T>::infinity;
+    const int bits = __float_as_int(value_of_bits<T>(top));
+    int e = (bits >> 23) - 127 - ((bits & 0x7fffff) > 0x7e0000 ? 5 : 6);     // 127 = 1.984375 * 2^6
+    e = e < Range<T>::low ? Range<T>::low : e;
+    const float inverse = __int_as_float((127 - e) << 23);
+    // x / 2^e + 1.5 * 2^23 in one rounding: its low byte is the nearest whole number, ties to even, in two's complement
+    unsigned r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(__builtin_fmaf((float)v[u][i], inverse, 12582912.0f));
+    if (e > Range<T>::top - 6) {      // 64 * 2^e is no finite number of the type
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(fminf(fmaxf(__uint_as_float(r[i]), 12582912.0f - 63.0f), 12582912.0f + 63.0f));
+    }
+    // bytes 0 of four words into one
+    auto pack = [](unsigned a, unsigned b, unsigned cc, unsigned d) {
+      return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, cc, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
+    };
+    const uint64_t q = flag ? 0ull : (uint64_t)pack(r[4], r[5], r[6], r[7]) << 32 | pack(r[0], r[1], r[2], r[3]);
+    int8_t* to = g.q + token[u] * g.ldq + c[u] * 8;
+    if (n[u] >= 8) {
+      __builtin_memcpy(to, &q, 8);
+    } else {
+      for (int i = 0; i < 8; ++i)
+        if (i < n[u]) to[i] = (int8_t)(q >> (8 * i));
+    }
+    if (n[u] > 0 && c[u] % 4 == 0) g.e[token[u] * g.lde + c[u] / 4] = (uint8_t)(flag ? 255 : e + 127);
   }
-  int8_t* to = g.q + token * g.ldq + c * 8;
-  if (n >= 8) {
-    __builtin_memcpy(to, &q, 8);
-  } else {
-    for (int i = 0; i < 8; ++i)
-      if (i < n) to[i] = (int8_t)(q >> (8 * i));
-  }
-  if (c % 4 == 0) g.e[token * g.lde + c / 4] = (uint8_t)(flag ? 255 : e + 127);
 }
 
-template <typename T> __global__ __launch_bounds__(256) void ckpt8_unpack_kernel(PackArgs g) {
+template <typename T, int U> __global__ __launch_bounds__(256) void ckpt8_unpack_kernel(PackArgs g) {
   using E = typename T::elem;
   using x8 = typename T::x8;
-  int64_t token;
-  int c;
-  if (!chunk_of(g, token, c)) return;
-  const int n = g.k - c * 8;
-  if (n <= 0) return;
-  const uint64_t q = load_bytes(g.q + token * g.ldq + c * 8, n);
-  const float scale = exponent_scale(g.e[token * g.lde + c / 4]);
-  x8 v;
+  int64_t token[U];
+  int c[U], n[U];
+  uint64_t q[U];
+  unsigned e[U];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (E)((float)(int8_t)(q >> (8 * i)) * scale);
-  E* to = static_cast<E*>(g.out) + token * g.ldx + c * 8;
-  if (n >= 8) {
-    __builtin_memcpy(to, &v, sizeof v);
-  } else {
-    for (int i = 0; i < 8; ++i)
-      if (i < n) to[i] = v[i];
+  for (int u = 0; u < U; ++u) {
+    n[u] = chunk_of(g, ((int64_t)blockIdx.x * U + u) * 256, token[u], c[u]) ? g.k - c[u] * 8 : 0;
+    q[u] = load_bytes(g.q + token[u] * g.ldq + c[u] * 8, n[u]);
+    e[u] = n[u] > 0 ? g.e[token[u] * g.lde + c[u] / 4] : 0u;
   }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float scale = exponent_scale(e[u]);
+    x8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (E)((float)(int8_t)(q[u] >> (8 * i)) * scale);
+    E* to = static_cast<E*>(g.out) + token[u] * g.ldx + c[u] * 8;
+    if (n[u] >= 8) {
+      __builtin_memcpy(to, &v, sizeof v);
+    } else {
+      for (int i = 0; i < 8; ++i)
+        if (i < n[u]) to[i] = v[i];
+    }
+  }
+}
+
+template <typename T> void launch_pack(const PackArgs& g, hipStream_t s) {
+  if (g.total >= 1 << 20) hipLaunchKernelGGL((ckpt8_pack_kernel<T, 4>), dim3((unsigned)((g.total + 1023) / 1024)), dim3(256), 0, s, g);
+  else hipLaunchKernelGGL((ckpt8_pack_kernel<T, 1>), dim3((unsigned)((g.total + 255) / 256)), dim3(256), 0, s, g);
+}
+template <typename T> void launch_unpack(const PackArgs& g, hipStream_t s) {
+  if (g.total >= 1 << 20) hipLaunchKernelGGL((ckpt8_unpack_kernel<T, 4>), dim3((unsigned)((g.total + 1023) / 1024)), dim3(256), 0, s, g);
+  else hipLaunchKernelGGL((ckpt8_unpack_kernel<T, 1>), dim3((unsigned)((g.total + 255) / 256)), dim3(256), 0, s, g);
 }
 
 PackArgs pack_args(int64_t k, int64_t n) {
@@ -135,10 +181,9 @@ hipError_t ckpt8_pack_device(int kind, int64_t k, int64_t n, const void* x, int6
                              int64_t lde, hipStream_t s) {
   PackArgs g = pack_args(k, n);
   g.x = x; g.ldx = ldx; g.q = q; g.ldq = ldq; g.e = e; g.lde = lde;
-  const dim3 grid((unsigned)((g.total + 255) / 256));
-  if (kind == BF16) hipLaunchKernelGGL(ckpt8_pack_kernel<Bf16>, grid, dim3(256), 0, s, g);
-  else if (kind == F16K) hipLaunchKernelGGL(ckpt8_pack_kernel<F16>, grid, dim3(256), 0, s, g);
-  else hipLaunchKernelGGL(ckpt8_pack_kernel<Fp32>, grid, dim3(256), 0, s, g);
+  if (kind == BF16) launch_pack<Bf16>(g, s);
+  else if (kind == F16K) launch_pack<F16>(g, s);
+  else launch_pack<Fp32>(g, s);
   return hipGetLastError();
 }
 
@@ -146,10 +191,9 @@ hipError_t ckpt8_unpack_device(int kind, int64_t k, int64_t n, const int8_t* q, 
                                void* x, int64_t ldx, hipStream_t s) {
   PackArgs g = pack_args(k, n);
   g.out = x; g.ldx = ldx; g.q = const_cast<int8_t*>(q); g.ldq = ldq; g.e = const_cast<uint8_t*>(e); g.lde = lde;
-  const dim3 grid((unsigned)((g.total + 255) / 256));
-  if (kind == BF16) hipLaunchKernelGGL(ckpt8_unpack_kernel<Bf16>, grid, dim3(256), 0, s, g);
-  else if (kind == F16K) hipLaunchKernelGGL(ckpt8_unpack_kernel<F16>, grid, dim3(256), 0, s, g);
-  else hipLaunchKernelGGL(ckpt8_unpack_kernel<Fp32>, grid, dim3(256), 0, s, g);
+  if (kind == BF16) launch_unpack<Bf16>(g, s);
+  else if (kind == F16K) launch_unpack<F16>(g, s);
+  else launch_unpack<Fp32>(g, s);
   return hipGetLastError();
 }
 

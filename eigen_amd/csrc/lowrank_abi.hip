@@ -17,7 +17,7 @@ using namespace eigamd;
 namespace {
 
 // Extents the kernels' 32-bit indices and grids are good for.
-constexpr int64_t kMaxFeatures = (int64_t)1 << 22, kMaxTokens = (int64_t)1 << 24, kMaxRank = 256, kMaxAdapters = 4096;
+constexpr int64_t kMaxFeatures = (int64_t)1 << 21, kMaxTokens = (int64_t)1 << 24, kMaxRank = 256, kMaxAdapters = 4096;
 
 int bad(const char* entry, const char* what) { return abi_fail(EIGAMD_ERR_ARG, std::string(entry) + ": " + what); }
 int done(const char* entry, hipError_t e) {

@@ -32,7 +32,7 @@ def call(fn, base, **change):
 
 @pytest.mark.parametrize("change", [
     dict(dtype=_lib.F64), dict(dtype=_lib.C32), dict(dtype=9), dict(opw=2), dict(opa=3), dict(opb=-1), dict(m=-1), dict(n=-1), dict(k=-1),
-    dict(m=2 ** 22 + 1), dict(n=2 ** 24 + 1), dict(rank=0), dict(rank=257), dict(count=-1), dict(count=4097), dict(ldw=3), dict(opw=1, ldw=4),
+    dict(m=2 ** 21 + 1), dict(n=2 ** 24 + 1), dict(rank=0), dict(rank=257), dict(count=-1), dict(count=4097), dict(ldw=3), dict(opw=1, ldw=4),
     dict(ldx=4), dict(ldy=3), dict(lda=1), dict(opa=1, lda=4), dict(ldb=3), dict(opb=1, ldb=1), dict(ldp=1), dict(sa=-1), dict(sb=-1),
     dict(w=NULL), dict(x=NULL), dict(y=NULL), dict(a=NULL), dict(b=NULL), dict(p=NULL), dict(scale=NULL), dict(plan=NULL),
     dict(x=ctypes.c_void_p(P.value + 1)), dict(p=ctypes.c_void_p(P.value + 2)), dict(y=P), dict(work=NULL), dict(bytes=511),
