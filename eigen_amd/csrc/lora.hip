@@ -201,6 +201,8 @@ template <typename T, int SRC> struct GradTile {
   using x8 = typename T::x8;
   static constexpr int bytes = 32 * kGradRows * T::bytes;
   x8 reg[4];
+  uint64_t qreg[4];
+  unsigned ereg[4];
   static __device__ __forceinline__ int swizzle(int line) { return T::bytes == 4 ? 0 : ((line & 3) | ((line >> 1) & 4)) << 1; }
   // token of line i: tok[i], -1 past the end
   __device__ __forceinline__ void load(char* lds, const GradArgs& g, const int* tok, int row0) {
@@ -216,17 +218,22 @@ template <typename T, int SRC> struct GradTile {
       } else if constexpr (SRC == STAGED) {
         reg[i] = load_up_to_8<E, x8>(static_cast<const E*>(g.u) + (int64_t)t * g.ldu + row, n);
       } else {
-        const uint64_t v = load_bytes(static_cast<const int8_t*>(g.u) + (int64_t)t * g.ldu + row, n);
-        const float sc = exponent_scale(n > 0 ? g.exponents[(int64_t)t * g.lde + row / 32] : 0u);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) reg[i][e] = (E)((float)(int8_t)(v >> (8 * e)) * sc);
+        qreg[i] = load_bytes(static_cast<const int8_t*>(g.u) + (int64_t)t * g.ldu + row, n);
+        ereg[i] = n > 0 ? g.exponents[(int64_t)t * g.lde + row / 32] : 0u;
       }
     }
   }
   __device__ __forceinline__ void store(char* lds) {
     if constexpr (SRC == DIRECT) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<x8*>(lds + (threadIdx.x + i * 256) * 8 * T::bytes) = reg[i];
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (SRC == QUANT) {
+        const float sc = exponent_scale(ereg[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) reg[i][e] = (E)((float)(int8_t)(qreg[i] >> (8 * e)) * sc);
+      }
+      *reinterpret_cast<x8*>(lds + (threadIdx.x + i * 256) * 8 * T::bytes) = reg[i];
+    }
   }
   static __device__ __forceinline__ x8 fragment(const char* lds, int row) {
     const int l = threadIdx.x & 63;
@@ -284,19 +291,26 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
   constexpr int NI = 4 * RT;
   const int wr = (w / RT) * 64 * RT, r = r0 + (w % RT) * 16 + (l & 15);
   f32x4 acc[NI] = {};
+  // p of a turn, loaded a turn early like u
+  float pv[8], pn[8];
+  auto load_p = [&](float(&v)[8], int s) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int token = tok[s * 32 + (l / 16) * 8 + e];
+      v[e] = token >= 0 && r < g.rank ? g.p[(int64_t)token * g.ldp + r] : 0.0f;
+    }
+  };
+  load_p(pv, 0);
   tile.load(lds, g, tok, row0);
   tile.store(lds);
   __syncthreads();
   for (int s = 0; s < turns; ++s) {
     char* here = lds + (s & 1) * Tile::bytes;
     char* next = lds + ((s & 1) ^ 1) * Tile::bytes;
-    float pv[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int token = tok[s * 32 + (l / 16) * 8 + e];
-      pv[e] = token >= 0 && r < g.rank ? g.p[(int64_t)token * g.ldp + r] : 0.0f;
+    if (s + 1 < turns) {
+      load_p(pn, s + 1);
+      tile.load(next, g, tok + (s + 1) * 32, row0);
     }
-    if (s + 1 < turns) tile.load(next, g, tok + (s + 1) * 32, row0);
     x8 fp[NP];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -317,6 +331,8 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
     }
     if (s + 1 < turns) tile.store(next);
     __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pv[e] = pn[e];
   }
   const bool whole = piece.run_end - piece.run_begin <= g.chunk;
   const float sj = whole ? g.scale[piece.adapter] : 1.0f;
