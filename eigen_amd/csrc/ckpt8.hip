@@ -129,10 +129,7 @@ template <typename T, int U> __global__ __launch_bounds__(256) void ckpt8_unpack
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const float scale = exponent_scale(e[u]);
-    x8 v;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (E)((float)(int8_t)(q[u] >> (8 * i)) * scale);
+    const x8 v = unpack_8<T>(q[u], exponent_scale(e[u]));
     E* to = static_cast<E*>(g.out) + token[u] * g.ldx + c[u] * 8;
     if (n[u] >= 8) {
       __builtin_memcpy(to, &v, sizeof v);

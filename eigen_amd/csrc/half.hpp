@@ -77,6 +77,15 @@ __device__ __forceinline__ Norm norm_of(float largest) {
 // exponent 255 and comes back as 0 * inf = NaN.
 __device__ __forceinline__ float exponent_scale(unsigned e) { return __int_as_float((int)(e << 23)); }
 
+// The 8 values q * scale of one chunk: |q| <= 127 has 7 bits, so they are exact in every type (the packing keeps the exponent in
+// the type's range).
+template <typename T> __device__ __forceinline__ typename T::x8 unpack_8(uint64_t q, float scale) {
+  typename T::x8 v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (typename T::elem)((float)(int8_t)(q >> (8 * i)) * scale);
+  return v;
+}
+
 template <typename E, typename V> __device__ __forceinline__ V load_8(const E* p) {
   V v;
   __builtin_memcpy(&v, p, 8 * sizeof(E));

@@ -176,6 +176,13 @@ template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct Slice
     }
   }
 
+  // DIRECT: chunk i of a slice that is whole; next() behind the last one.
+  __device__ __forceinline__ void send(char* lds, int i) {
+    char* to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 1024 + i * NT * 16;
+    if constexpr (GATHER) load_to_lds(ptr[i], to);
+    else if constexpr (LAY == KC) load_to_lds(base, off[i], to);
+    else load_to_lds(base + i * across, off[0], to);
+  }
   __device__ __forceinline__ void commit(char* lds) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     if constexpr (SRC == DIRECT) {
@@ -183,11 +190,7 @@ template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct Slice
       char* to = lds + wave * 1024;
       if (left >= 64) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if constexpr (GATHER) load_to_lds(ptr[i], to + i * NT * 16);
-          else if constexpr (LAY == KC) load_to_lds(base, off[i], to + i * NT * 16);
-          else load_to_lds(base + i * across, off[0], to + i * NT * 16);
-        }
+        for (int i = 0; i < N; ++i) send(lds, i);
       } else {
         // Whole chunks (the launcher sees to that; one that the reduction ends in has zeros behind its end); those outside: zeros.
 #pragma unroll
@@ -198,12 +201,7 @@ template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct Slice
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        // |q| <= 127 has 7 bits, so q * 2^e is exact in either type (the packing keeps the exponent in the type's range)
-        x8 v;
-        const float sc = exponent_scale(ereg[i]);
-#pragma unroll
-        for (int t = 0; t < 8; ++t) v[t] = (E)((float)(int8_t)(qreg[i] >> (8 * t)) * sc);
-        *reinterpret_cast<x8*>(lds + (threadIdx.x + i * NT) * 16) = v;
+        *reinterpret_cast<x8*>(lds + (threadIdx.x + i * NT) * 16) = unpack_8<T>(qreg[i], exponent_scale(ereg[i]));
       }
     }
   }
@@ -412,7 +410,47 @@ __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
   read(lds, 0);
   constexpr int keep = (D - 2) * (LoadA::N + LoadB::N);
   char* here = lds;
-  for (int s = 0; s < slices; ++s) {
+  int s = 0;
+  if constexpr (SA == DIRECT && SB == DIRECT) {
+    // As long as slice s + D is whole its loads need no looking at: they go out between the products of the last step, one of
+    // each operand behind every group.
+    for (; la.left >= 64; ++s) {
+      char* other = here + slice == lds + D * slice ? lds : here + slice;
+#pragma unroll
+      for (int q = 0; q + 1 < 2 * P; ++q) {
+        read(here, q + 1);
+        multiply(q);
+        if ((q + 1) % P == 0) interleave(ReadsAB{});
+        else interleave(ReadsA{});
+      }
+      slice_barrier<keep>();
+      constexpr int G = LoadA::N > LoadB::N ? LoadA::N : LoadB::N;
+#pragma unroll
+      for (int q = 0; q < G; ++q) {
+        if (q < LoadA::N) la.send(here, q);
+        if (q < LoadB::N) lb.send(here + LoadA::bytes, q);
+#pragma unroll
+        for (int i = 0; i < NH; ++i)
+          if (i * G / NH == q) fa[0][i] = LoadA::fragment(other, wr + i * 16, 0);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          if (j * G / NJ == q) fb[0][j] = LoadB::fragment(other + LoadA::bytes, wc + j * 16, 0);
+#pragma unroll
+        for (int i = 0; i < NH; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            if ((i * NJ + j) * G / products == q) {
+              f32x4& c = acc[(P - 1) * NH + i][j];
+              c = T::mma(fa[1][i], fb[1][j], c);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      la.next();
+      lb.next();
+      here = other;
+    }
+  }
+  for (; s < slices; ++s) {
     char* other = here + slice == lds + D * slice ? lds : here + slice;
 #pragma unroll
     for (int q = 0; q + 1 < 2 * P; ++q) {

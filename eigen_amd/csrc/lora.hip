@@ -227,11 +227,7 @@ template <typename T, int SRC> struct GradTile {
     if constexpr (SRC == DIRECT) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (SRC == QUANT) {
-        const float sc = exponent_scale(ereg[i]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) reg[i][e] = (E)((float)(int8_t)(qreg[i] >> (8 * e)) * sc);
-      }
+      if constexpr (SRC == QUANT) reg[i] = unpack_8<T>(qreg[i], exponent_scale(ereg[i]));
       *reinterpret_cast<x8*>(lds + (threadIdx.x + i * 256) * 8 * T::bytes) = reg[i];
     }
   }
