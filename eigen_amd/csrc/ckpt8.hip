@@ -157,15 +157,15 @@ PackArgs pack_args(int64_t k, int64_t n) {
   return g;
 }
 
-template <typename T, int OUT, int B, int WM, int WN> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
+template <typename T, int OUT, int B, int WM, int WN, int D> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
   const dim3 grid((unsigned)(((g.m + B - 1) / B) * (((int64_t)g.n + B - 1) / B)), g.splits);
-  hipLaunchKernelGGL((half_gemm_kernel<T, MC, QUANT, MC, DIRECT, OUT, B, B, WM, WN, 2>), grid, dim3(WM * WN * 64), 0, s, g);
+  hipLaunchKernelGGL((half_gemm_kernel<T, MC, MC, OUT, B, B, WM, WN, D>), grid, dim3(WM * WN * 64), 0, s, g);
   return hipGetLastError();
 }
 template <typename T, int OUT> hipError_t launch_out(const HalfGemm& g, int tile, hipStream_t s) {
-  return tile == TILE_256   ? launch_tiles<T, OUT, 256, 2, 4>(g, s)
-         : tile == TILE_128 ? launch_tiles<T, OUT, 128, 2, 2>(g, s)
-                            : launch_tiles<T, OUT, 128, 2, 4>(g, s);
+  return tile == TILE_256   ? launch_tiles<T, OUT, 256, 2, 4, 2>(g, s)
+         : tile == TILE_128 ? launch_tiles<T, OUT, 128, 2, 2, 2>(g, s)
+                            : launch_tiles<T, OUT, 128, 2, 4, 4>(g, s);
 }
 int64_t sums_bytes(int64_t m, int64_t n, int64_t k) {
   const int splits = plan_tiles(k, m, n).splits;
@@ -197,7 +197,7 @@ hipError_t ckpt8_unpack_device(int kind, int64_t k, int64_t n, const int8_t* q, 
 int64_t ckpt8_grad_work_bytes(int kind, int64_t m, int64_t n, int64_t k, const void* dy, int64_t lddy) {
   if (m <= 0 || n <= 0 || k <= 0) return 0;
   if (kind == F32) return (k * n * 4 + 255) / 256 * 256 + std::min<int64_t>(16 * m * k * 4, (int64_t)256 << 20);
-  return sums_bytes(m, n, k) + (whole_chunks(dy, lddy, m) ? 0 : padded_bytes(m, n));
+  return sums_bytes(m, n, k) + padded_bytes(k, n) + (whole_chunks(dy, lddy, m) ? 0 : padded_bytes(m, n));
 }
 
 hipError_t ckpt8_grad_device(const Ckpt8GradArgs& c, hipStream_t s) {
@@ -219,23 +219,30 @@ hipError_t ckpt8_grad_device(const Ckpt8GradArgs& c, hipStream_t s) {
     q.partials_bytes = c.work && c.work_bytes > used ? (size_t)(c.work_bytes - used) : 0;
     return launch_gemm_f32(q, s);
   }
+  // The checkpoint is unpacked into scratch memory once, and the product reads that.  Unpacking inside the product (every tile's
+  // chunks through registers) kept its loads from going to LDS directly and cost more than the extra pass: 16384 tokens x 4096 x
+  // 4096 took 520 us so, 465 now, 34 of them unpacking.
+  char* work = static_cast<char*>(c.work);
+  const int64_t sums = sums_bytes(c.m, c.n, c.k);
   HalfGemm g;
   g.m = (int)c.k; g.n = (int)c.m; g.k = (int)c.n;
-  g.a = c.q; g.lda = c.ldq;
-  g.exponents = c.e; g.lde = c.lde;
+  g.a = work + sums; g.lda = padded(c.k);
   g.b = c.dy; g.ldb = c.lddy;
   g.c = c.dw; g.ldc = c.lddw;
   g.beta = c.beta;
+  g.partial = reinterpret_cast<float*>(work);
   const TilePlan plan = plan_tiles(c.k, c.m, c.n);
   g.splits = plan.splits;
   g.k_piece = (int)plan.k_piece;
-  g.partial = static_cast<float*>(c.work);
   hipError_t e;
-  if (c.n > 0 && !whole_chunks(c.dy, c.lddy, c.m)) {
-    const PadCopy copy = pad_copy(c.dy, c.lddy, c.m, c.n, static_cast<char*>(c.work) + sums_bytes(c.m, c.n, c.k));
-    g.b = copy.to;
-    g.ldb = padded(c.m);
-    if ((e = launch_pad_copy(copy, {}, s)) != hipSuccess) return e;
+  if (c.n > 0) {
+    if ((e = ckpt8_unpack_device(c.kind, c.k, c.n, c.q, c.ldq, c.e, c.lde, work + sums, g.lda, s)) != hipSuccess) return e;
+    if (!whole_chunks(c.dy, c.lddy, c.m)) {
+      const PadCopy copy = pad_copy(c.dy, c.lddy, c.m, c.n, work + sums + padded_bytes(c.k, c.n));
+      g.b = copy.to;
+      g.ldb = padded(c.m);
+      if ((e = launch_pad_copy(copy, {}, s)) != hipSuccess) return e;
+    }
   }
   if (c.kind == BF16) e = c.trans ? launch_out<Bf16, OUT_F32>(g, plan.tile, s) : launch_out<Bf16, OUT_F32_SWAPPED>(g, plan.tile, s);
   else e = c.trans ? launch_out<F16, OUT_F32>(g, plan.tile, s) : launch_out<F16, OUT_F32_SWAPPED>(g, plan.tile, s);

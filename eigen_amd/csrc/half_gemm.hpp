@@ -15,7 +15,6 @@
 namespace eigamd {
 
 enum { KC = 0, MC = 1 };                       // orientation
-enum { DIRECT = 0, STAGED = 1, QUANT = 2 };    // global -> LDS by hardware / (factor gradients only) through registers / from 8 bits
 
 struct HalfGemm {
   int m, n, k;
@@ -26,9 +25,6 @@ struct HalfGemm {
   void* c;
   int64_t ldc;
   const int* order = nullptr;   // column j of B and C is column order[j] of the stored matrices
-  // exponents of an 8-bit operand, one per 32 features (its contiguous direction)
-  const uint8_t* exponents = nullptr;
-  int64_t lde = 0;
   // adapters: column j belongs to seg[j] (`none`: no adapter)
   const int* seg = nullptr;
   int none = 0, rank = 0;
@@ -68,33 +64,24 @@ template <int KEEP> __device__ __forceinline__ void slice_barrier() {
 }
 
 // One operand's slice of R rows x 64 positions, loaded by NT threads in chunks of 8 elements; NT * N chunks in all.  Slices are
-// taken one after the other: fetch() brings the next one into registers (nothing to do for DIRECT), commit() puts it into LDS.
+// taken one after the other.
 // Rows past the end are not cleared: whatever stands there meets only rows of C that are not stored.  Positions past the end of
 // the reduction are zero in both operands.
 // GATHER: row i is row order[i] of the matrix, and every chunk has an address of its own; otherwise they are 32-bit offsets from
-// a base that is the same in all lanes (256 rows or 64 lines of at most 2^22 elements).
-template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct SliceLoader {
+// a base that is the same in all lanes (256 rows or 64 lines of at most 2^21 elements).
+template <typename T, int LAY, int R, int NT, bool GATHER> struct SliceLoader {
   static_assert(LAY == KC || (R >= 128 && !GATHER), "the permutation of a line needs 16 chunks");
-  static_assert(SRC == DIRECT || (SRC == QUANT && LAY == MC), "what the operators need");
   static constexpr int N = R * 8 / NT;
   static constexpr int bytes = R * 128;
-  static constexpr int es = SRC == QUANT ? 1 : 2;
   static constexpr int NOFF = GATHER ? 1 : LAY == KC ? N : 1, NPTR = GATHER ? N : 1;
   static constexpr int lines = NT / (R / 8);     // MC: lines from one chunk of a thread to the next
-  using E = typename T::elem;
   using x8 = typename T::x8;
   const char* base;        // first position of the next slice
   int64_t step;            // bytes from one slice to the next
   int64_t across;          // MC: bytes from one chunk of a thread to the next
   unsigned off[NOFF];
   const char* ptr[NPTR];
-  int len;                 // MC: elements of this thread's chunks inside the matrix (0..8)
   int left;                // positions from the next slice's first to the end of the reduction
-  const uint8_t* ebase;
-  int64_t lde;
-  unsigned eoff;
-  uint64_t qreg[N];
-  unsigned ereg[N];
 
   static __device__ __forceinline__ int swizzle(int line) {
     // KC: rows 0..7 of an 8-lane phase; MC: lines {0..3, 8..11} (+4, +16) of a half wave, 32 bytes each
@@ -106,39 +93,37 @@ template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct Slice
     return LAY == KC ? ((t % 8) ^ swizzle(t / 8)) * 8 : t / (R / 8) + i * lines;
   }
 
-  __device__ __forceinline__ void init(const void* origin, int64_t ld, int row0, int rows, int k0, int count, const int* order,
-                                       const uint8_t* exponents, int64_t lde_) {
-    step = (LAY == KC ? 64 : 64 * ld) * es;
+  __device__ __forceinline__ void init(const void* origin, int64_t ld, int row0, int rows, int k0, int count, const int* order) {
+    step = (LAY == KC ? 64 : 64 * ld) * 2;
     left = count;
     base = static_cast<const char*>(origin);
     if constexpr (LAY == KC) {
-      base += ((GATHER ? 0 : row0 * ld) + k0) * es;
+      base += ((GATHER ? 0 : row0 * ld) + k0) * 2;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int line = threadIdx.x / 8 + i * (NT / 8);
         const int in = row0 + line < rows ? line : rows - 1 - row0;
-        if constexpr (GATHER) ptr[i] = base + ((int64_t)order[row0 + in] * ld + position(0)) * es;
-        else off[i] = (unsigned)((in * ld + position(0)) * es);
+        if constexpr (GATHER) ptr[i] = base + ((int64_t)order[row0 + in] * ld + position(0)) * 2;
+        else off[i] = (unsigned)((in * ld + position(0)) * 2);
       }
     } else {
       const int line = position(0), c = (threadIdx.x % (R / 8)) ^ swizzle(line);
-      const int row = row0 + c * 8;
-      len = rows - row < 0 ? 0 : (rows - row < 8 ? rows - row : 8);
-      base += (k0 * ld + row0) * es;
-      across = lines * ld * es;
-      off[0] = (unsigned)((line * ld + (len ? c * 8 : 0)) * es);
-      if constexpr (SRC == QUANT) {
-        lde = lde_;
-        ebase = exponents + (int64_t)k0 * lde + row0 / 32;
-        eoff = (unsigned)(line * lde + (len ? c / 4 : 0));
-      }
+      base += (k0 * ld + row0) * 2;
+      across = lines * ld * 2;
+      off[0] = (unsigned)((line * ld + (row0 + c * 8 < rows ? c * 8 : 0)) * 2);
     }
   }
   __device__ __forceinline__ const char* at(int i) const {
     if constexpr (GATHER) return ptr[i];
     else return LAY == KC ? base + off[i] : base + i * across + off[0];
   }
-  __device__ __forceinline__ const uint8_t* exponent_at(int i) const { return ebase + i * (lines * lde) + eoff; }
+  // Chunk i of a slice that is whole; next() behind the last one.
+  __device__ __forceinline__ void send(char* lds, int i) {
+    char* to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 1024 + i * NT * 16;
+    if constexpr (GATHER) load_to_lds(ptr[i], to);
+    else if constexpr (LAY == KC) load_to_lds(base, off[i], to);
+    else load_to_lds(base + i * across, off[0], to);
+  }
   __device__ __forceinline__ void next() {
     left -= 64;
     base += step;
@@ -146,64 +131,21 @@ template <typename T, int LAY, int SRC, int R, int NT, bool GATHER> struct Slice
 #pragma unroll
       for (int i = 0; i < N; ++i) ptr[i] += step;
     }
-    if constexpr (SRC == QUANT) ebase += 64 * lde;
   }
-
-  __device__ __forceinline__ void fetch() {
-    if constexpr (SRC == QUANT) {
-      if (left <= 0) return;
-      if (left >= 72) {
-        // Whole loads.  Past the end of a column they run into the next one (there are at least 8 more elements of columns
-        // behind this slice), and what they bring belongs to rows that are not stored.
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          __builtin_memcpy(&qreg[i], at(i), 8);
-          ereg[i] = *exponent_at(i);
-        }
-      } else {
-        // byte by byte, those outside from the zero page
-        const uint8_t* zero = reinterpret_cast<const uint8_t*>(zero_page);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int n = position(i) < left ? len : 0;
-          qreg[i] = 0;
-#pragma unroll
-          for (int t = 0; t < 8; ++t) qreg[i] |= (uint64_t)*(t < n ? reinterpret_cast<const uint8_t*>(at(i)) + t : zero) << (8 * t);
-          ereg[i] = *(n > 0 ? exponent_at(i) : zero);
-        }
-      }
-      next();
-    }
-  }
-
-  // DIRECT: chunk i of a slice that is whole; next() behind the last one.
-  __device__ __forceinline__ void send(char* lds, int i) {
-    char* to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 1024 + i * NT * 16;
-    if constexpr (GATHER) load_to_lds(ptr[i], to);
-    else if constexpr (LAY == KC) load_to_lds(base, off[i], to);
-    else load_to_lds(base + i * across, off[0], to);
-  }
+  // The next slice, if there is one.
   __device__ __forceinline__ void commit(char* lds) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    if constexpr (SRC == DIRECT) {
-      if (left <= 0) return;
-      char* to = lds + wave * 1024;
-      if (left >= 64) {
+    if (left <= 0) return;
+    if (left >= 64) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) send(lds, i);
-      } else {
-        // Whole chunks (the launcher sees to that; one that the reduction ends in has zeros behind its end); those outside: zeros.
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          load_to_lds((LAY == KC ? position(0) : position(i)) < left ? at(i) : reinterpret_cast<const char*>(zero_page), to + i * NT * 16);
-      }
-      next();
+      for (int i = 0; i < N; ++i) send(lds, i);
     } else {
+      // Whole chunks (the launcher sees to that; one that the reduction ends in has zeros behind its end); those outside: zeros.
+      char* to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 1024;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        *reinterpret_cast<x8*>(lds + (threadIdx.x + i * NT) * 16) = unpack_8<T>(qreg[i], exponent_scale(ereg[i]));
-      }
+      for (int i = 0; i < N; ++i)
+        load_to_lds((LAY == KC ? position(0) : position(i)) < left ? at(i) : reinterpret_cast<const char*>(zero_page), to + i * NT * 16);
     }
+    next();
   }
 
   // Fragment of rows row .. row + 15 and positions kk .. kk + 31 of a slice in LDS.
@@ -331,13 +273,12 @@ enum { OUT_HALF = 0, OUT_F32 = 1, OUT_F32_SWAPPED = 2 };
 
 // OUT_HALF: C in the operands' type, columns scattered by `order`, adapters added.
 // OUT_F32: C = beta C + A B in 32 bits.  OUT_F32_SWAPPED: the same with C stored transposed (N x M column-major).
-template <typename T, int LA, int SA, int LB, int SB, int OUT, int BM, int BN, int WM, int WN, int D>
+template <typename T, int LA, int LB, int OUT, int BM, int BN, int WM, int WN, int D>
 __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
   constexpr int NT = WM * WN * 64, TM = BM / WM, TN = BN / WN, NI = TM / 16, NJ = TN / 16;
-  using LoadA = SliceLoader<T, LA, SA, BM, NT, false>;
-  using LoadB = SliceLoader<T, LB, SB, BN, NT, OUT == OUT_HALF>;
+  using LoadA = SliceLoader<T, LA, BM, NT, false>;
+  using LoadB = SliceLoader<T, LB, BN, NT, OUT == OUT_HALF>;
   constexpr int slice = LoadA::bytes + LoadB::bytes;
-  static_assert(D == 2 || (SA == DIRECT && SB == DIRECT), "what passes through registers is one slice ahead of LDS");
   __shared__ __align__(1024) char lds[D * slice];
   const int tiles_m = (g.m + BM - 1) / BM, tiles_n = (g.n + BN - 1) / BN;
   int tm, tn;
@@ -350,8 +291,8 @@ __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
 
   LoadA la;
   LoadB lb;
-  la.init(g.a, g.lda, tm * BM, g.m, k_begin, k_count, nullptr, g.exponents, g.lde);
-  lb.init(g.b, g.ldb, tn * BN, g.n, k_begin, k_count, g.order, g.exponents, g.lde);
+  la.init(g.a, g.lda, tm * BM, g.m, k_begin, k_count, nullptr);
+  lb.init(g.b, g.ldb, tn * BN, g.n, k_begin, k_count, g.order);
   f32x4 acc[NI][NJ] = {};
   // D slices in LDS.  Each half of a slice (32 positions) is multiplied in P steps of 16 rows each x 4 (all rows of this wave, or the
   // upper and the lower half); while one step's products run, the fragments of the next are read.  A slice's buffer is free once
@@ -359,13 +300,9 @@ __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
   // slice s + 1 has to have arrived at that barrier, those behind it may still be under way.
 #pragma unroll 1
   for (int z = 0; z < D; ++z) {
-    la.fetch();
-    lb.fetch();
     la.commit(lds + z * slice);
     lb.commit(lds + z * slice + LoadA::bytes);
   }
-  la.fetch();
-  lb.fetch();
   if constexpr (OUT == OUT_HALF) {
     if (g.rank > 0 && blockIdx.y == 0) add_adapters<T, NI, NJ>(g, tm * BM + wr, tn * BN + wc, acc);
   }
@@ -411,44 +348,42 @@ __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
   constexpr int keep = (D - 2) * (LoadA::N + LoadB::N);
   char* here = lds;
   int s = 0;
-  if constexpr (SA == DIRECT && SB == DIRECT) {
-    // As long as slice s + D is whole its loads need no looking at: they go out between the products of the last step, one of
-    // each operand behind every group.
-    for (; la.left >= 64; ++s) {
-      char* other = here + slice == lds + D * slice ? lds : here + slice;
+  // As long as slice s + D is whole its loads need no looking at: they go out between the products of the last step, one of
+  // each operand behind every group.
+  for (; la.left >= 64; ++s) {
+    char* other = here + slice == lds + D * slice ? lds : here + slice;
 #pragma unroll
-      for (int q = 0; q + 1 < 2 * P; ++q) {
-        read(here, q + 1);
-        multiply(q);
-        if ((q + 1) % P == 0) interleave(ReadsAB{});
-        else interleave(ReadsA{});
-      }
-      slice_barrier<keep>();
-      constexpr int G = LoadA::N > LoadB::N ? LoadA::N : LoadB::N;
+    for (int q = 0; q + 1 < 2 * P; ++q) {
+      read(here, q + 1);
+      multiply(q);
+      if ((q + 1) % P == 0) interleave(ReadsAB{});
+      else interleave(ReadsA{});
+    }
+    slice_barrier<keep>();
+    constexpr int G = LoadA::N > LoadB::N ? LoadA::N : LoadB::N;
 #pragma unroll
-      for (int q = 0; q < G; ++q) {
-        if (q < LoadA::N) la.send(here, q);
-        if (q < LoadB::N) lb.send(here + LoadA::bytes, q);
+    for (int q = 0; q < G; ++q) {
+      if (q < LoadA::N) la.send(here, q);
+      if (q < LoadB::N) lb.send(here + LoadA::bytes, q);
 #pragma unroll
-        for (int i = 0; i < NH; ++i)
-          if (i * G / NH == q) fa[0][i] = LoadA::fragment(other, wr + i * 16, 0);
+      for (int i = 0; i < NH; ++i)
+        if (i * G / NH == q) fa[0][i] = LoadA::fragment(other, wr + i * 16, 0);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        if (j * G / NJ == q) fb[0][j] = LoadB::fragment(other + LoadA::bytes, wc + j * 16, 0);
+#pragma unroll
+      for (int i = 0; i < NH; ++i)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
-          if (j * G / NJ == q) fb[0][j] = LoadB::fragment(other + LoadA::bytes, wc + j * 16, 0);
-#pragma unroll
-        for (int i = 0; i < NH; ++i)
-#pragma unroll
-          for (int j = 0; j < NJ; ++j)
-            if ((i * NJ + j) * G / products == q) {
-              f32x4& c = acc[(P - 1) * NH + i][j];
-              c = T::mma(fa[1][i], fb[1][j], c);
-            }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      la.next();
-      lb.next();
-      here = other;
+          if ((i * NJ + j) * G / products == q) {
+            f32x4& c = acc[(P - 1) * NH + i][j];
+            c = OUT == OUT_F32_SWAPPED ? T::mma(fb[1][j], fa[1][i], c) : T::mma(fa[1][i], fb[1][j], c);
+          }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    la.next();
+    lb.next();
+    here = other;
   }
   for (; s < slices; ++s) {
     char* other = here + slice == lds + D * slice ? lds : here + slice;
@@ -463,8 +398,6 @@ __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
     else slice_barrier<keep>();
     la.commit(here);
     lb.commit(here + LoadA::bytes);
-    la.fetch();
-    lb.fetch();
     read(other, 0);     // (behind the last slice: what was there before, not used)
     multiply(2 * P - 1);
     interleave(ReadsAB{});

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void lora_add_f32_kernel(HalfGemm g) {
 
 template <typename T, int LA, int B, int WM, int WN, int D> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
   const dim3 grid((unsigned)(((g.m + B - 1) / B) * (((int64_t)g.n + B - 1) / B)), g.splits);
-  hipLaunchKernelGGL((half_gemm_kernel<T, LA, DIRECT, KC, DIRECT, OUT_HALF, B, B, WM, WN, D>), grid, dim3(WM * WN * 64), 0, s, g);
+  hipLaunchKernelGGL((half_gemm_kernel<T, LA, KC, OUT_HALF, B, B, WM, WN, D>), grid, dim3(WM * WN * 64), 0, s, g);
   return hipGetLastError();
 }
 template <typename T, int LA> hipError_t launch_form(const HalfGemm& g, int tile, hipStream_t s) {
@@ -171,6 +171,7 @@ template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArg
 
 // ------------------------------------------------------------------------------------------------ gradients of the factors
 constexpr int kGradRows = 256;
+enum { DIRECT, STAGED, QUANT };    // u: global -> LDS by hardware / through registers, any alignment / from 8 bits
 
 struct GradArgs {
   int rows, rank, n, none, chunk;
