@@ -3,6 +3,7 @@ device-resident matrices (``eigamd_lora_*``, ``eigamd_ckpt8_*`` of ``include/eig
 
 Column-major, one token per column: a torch tensor of shape (tokens, features) is ``DeviceMatrix(features, tokens)`` on the
 same storage.  Every call is asynchronous on ``stream`` (default: torch's current stream of the operands' device)."""
+import contextlib
 import ctypes
 
 import torch
@@ -12,6 +13,7 @@ from ._lib import lib
 from .device import DeviceMatrix, _TORCH_OF_KIND
 
 _KINDS = (_lib.F32, _lib.BF16, _lib.F16)
+_BYTES = {_lib.F32: 4, _lib.BF16: 2, _lib.F16: 2}
 
 
 class MatrixStack:
@@ -78,26 +80,34 @@ def _holds(storage, offset, ld, rows, cols, what):
 
 
 def _check_matrix(m, kind, rows, cols, what, count=1):
+    """Checks m (of a stack: its last matrix too) and returns its address.  Every operand of every call passes here, and a call's
+    host time is what a single token waits for, so it is written out."""
+    storage, offset = m.storage, m.offset
     if m.kind != kind:
         raise ValueError(f"{what} has the wrong scalar kind")
     if m.rows != rows or m.cols != cols:
         raise ValueError(f"{what} is {m.rows} x {m.cols}, expected {rows} x {cols}")
-    storage = m.storage
     if storage.dtype is not _TORCH_OF_KIND[kind] or not storage.is_contiguous():
         raise ValueError(f"{what}: the storage must be a contiguous tensor of the matrix's type")
-    _holds(storage, m.offset + (count - 1) * m.stride if count > 1 else m.offset, m.ld, rows, cols, what)
+    if rows and cols:
+        last = offset + m.ld * (cols - 1) + rows
+        if count > 1:
+            last += (count - 1) * m.stride
+        if offset < 0 or last > storage.numel():
+            raise ValueError(f"{what}: the storage is too small for the matrix")
+    return storage.data_ptr() + offset * _BYTES[kind] if offset else storage.data_ptr()
 
 
 def _check_stack(m, kind, rows, cols, count, what):
     if m.count != count:
         raise ValueError(f"{what} has {m.count} matrices, expected {count}")
-    if count:
-        _check_matrix(m, kind, rows, cols, what, count)
+    return _check_matrix(m, kind, rows, cols, what, count) if count else 0
 
 
 def _check_vector(v, n, dtype, what):
     if v.dtype is not dtype or v.numel() != n or not v.is_contiguous():
         raise ValueError(f"{what} must be {n} contiguous elements of {dtype}")
+    return v.data_ptr()
 
 
 _OPS = {"N": _lib.OP_N, "T": _lib.OP_T, "n": _lib.OP_N, "t": _lib.OP_T}
@@ -114,51 +124,59 @@ def _turned(op, rows, cols):
     return (cols, rows) if op == _lib.OP_T else (rows, cols)
 
 
-def _run(entry, stream, tensors, need, work, call):
-    """call(stream handle, address of the scratch memory, its bytes) with the operands' device as the current one; the scratch
-    memory is `work`, or allocated (and later used again) in the stream's own order."""
+def _here(stream, *tensors):
+    """The current stream's handle if this call can go straight there: no stream asked for, and the operands on the current
+    device.  Otherwise None; the call is then made again inside ``_there``."""
     device = tensors[0].get_device()
-    if device < 0:
-        raise ValueError("operands must be in device memory")
     for t in tensors:
         if t.get_device() != device:
             raise ValueError("operands lie on different devices")
+    if device < 0:
+        raise ValueError("operands must be in device memory")
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None and torch.cuda.current_device() == device else None
+
+
+@contextlib.contextmanager
+def _there(stream, tensor):
+    """tensor's device and the stream (there, by default its current one) as the current ones: scratch memory is then allocated,
+    and used again, in that stream's order."""
+    device = tensor.device
+    with torch.cuda.device(device):
+        s = torch.cuda.current_stream(device) if stream is None else stream
+        if s.device != device:
+            raise ValueError("the stream belongs to another device than the operands")
+        with torch.cuda.stream(s):
+            yield
+
+
+def _scratch(work, need, like):
+    """(address, bytes) of the scratch memory, and the tensor that holds it."""
     if need < 0:
         raise ValueError("extent out of range")
-    if work is not None and (work.get_device() != device or not work.is_contiguous() or work.numel() * work.element_size() < need):
+    if not need:
+        return 0, 0, None
+    if work is None:
+        work = torch.empty(need, dtype=torch.uint8, device=like.device)
+    elif work.get_device() != like.get_device() or not work.is_contiguous() or work.numel() * work.element_size() < need:
         raise ValueError(f"work needs {need} contiguous bytes on the operands' device")
-    if stream is None and torch.cuda.current_device() == device:
-        if work is None and need:
-            work = torch.empty(need, dtype=torch.uint8, device=tensors[0].device)
-        rc = call(torch._C._cuda_getCurrentRawStream(device), work.data_ptr() if need else 0, need)
-    else:
-        with torch.cuda.device(device):
-            s = torch.cuda.current_stream(device) if stream is None else stream
-            if s.device.index != device:
-                raise ValueError("the stream belongs to another device than the operands")
-            with torch.cuda.stream(s):
-                if work is None and need:
-                    work = torch.empty(need, dtype=torch.uint8, device=tensors[0].device)
-                rc = call(s.cuda_stream, work.data_ptr() if need else 0, need)
-    if rc != _lib.OK:
-        _lib.check(rc, entry)
+    return work.data_ptr(), need, work
 
 
 def lora_plan(adapter_of, n_adapters, stream=None):
     """Plan of a batch: ``adapter_of`` (int32, one per token; anything outside [0, n_adapters) means no adapter).  Made once per
     batch, used by every projection, forward and backward."""
     n, n_adapters = adapter_of.numel(), int(n_adapters)
-    _check_vector(adapter_of, n, torch.int32, "adapter_of")
+    ids = _check_vector(adapter_of, n, torch.int32, "adapter_of")
     ints = lib.eigamd_lora_plan_ints(n, n_adapters)
     if ints < 0:
         raise ValueError("number of tokens or adapters out of range")
-    plan = []
-
-    def call(s, work, have):
-        plan.append(torch.empty(ints, dtype=torch.int32, device=adapter_of.device))
-        return lib.eigamd_lora_plan_dev(n, n_adapters, adapter_of.data_ptr(), plan[0].data_ptr(), s)
-    _run("eigamd_lora_plan_dev", stream, (adapter_of,), 0, None, call)
-    return LoraPlan(n, n_adapters, plan[0])
+    s = _here(stream, adapter_of)
+    if s is None:
+        with _there(stream, adapter_of):
+            return lora_plan(adapter_of, n_adapters)
+    plan = torch.empty(ints, dtype=torch.int32, device=adapter_of.device)
+    _lib.check(lib.eigamd_lora_plan_dev(n, n_adapters, ids, plan.data_ptr(), s), "eigamd_lora_plan_dev")
+    return LoraPlan(n, n_adapters, plan)
 
 
 def lora_work_bytes(opw, w, x):
@@ -178,21 +196,24 @@ def lora_dev(opw, w, x, opa, a, opb, b, scale, plan, p, y, work=None, stream=Non
     kind = w.kind
     if kind not in _KINDS:
         raise ValueError("the kind must be F32, BF16 or F16")
-    m, k = _turned(ow, w.rows, w.cols)
-    n, rank = plan.n, p.rows
-    _check_matrix(w, kind, w.rows, w.cols, "w")
-    _check_matrix(x, kind, k, n, "x")
-    _check_matrix(y, kind, m, n, "y")
-    _check_matrix(p, _lib.F32, rank, n, "p")
-    _check_stack(a, kind, *_turned(oa, rank, k), plan.n_adapters, "a")
-    _check_stack(b, kind, *_turned(ob, m, rank), plan.n_adapters, "b")
-    _check_vector(scale, plan.n_adapters, torch.float32, "scale")
-    count = plan.n_adapters
-    _run("eigamd_lora_dev", stream, (x.storage, w.storage, a.storage, b.storage, scale, plan.storage, p.storage, y.storage),
-         lib.eigamd_lora_work_bytes(kind, ow, m, n, k, w.ptr, w.ld, x.ptr, x.ld), work,
-         lambda s, at, have: lib.eigamd_lora_dev(kind, ow, oa, ob, m, n, k, rank, count, w.ptr, w.ld, x.ptr, x.ld, a.ptr, a.ld, a.stride,
-                                                 b.ptr, b.ld, b.stride, scale.data_ptr(), plan.storage.data_ptr(), p.ptr, p.ld, y.ptr, y.ld,
-                                                 at, have, s))
+    m, k = (w.cols, w.rows) if ow else (w.rows, w.cols)
+    n, rank, count = plan.n, p.rows, plan.n_adapters
+    at_w = _check_matrix(w, kind, w.rows, w.cols, "w")
+    at_x = _check_matrix(x, kind, k, n, "x")
+    at_y = _check_matrix(y, kind, m, n, "y")
+    at_p = _check_matrix(p, _lib.F32, rank, n, "p")
+    at_a = _check_stack(a, kind, *_turned(oa, rank, k), count, "a")
+    at_b = _check_stack(b, kind, *_turned(ob, m, rank), count, "b")
+    at_s = _check_vector(scale, count, torch.float32, "scale")
+    s = _here(stream, x.storage, w.storage, a.storage, b.storage, scale, plan.storage, p.storage, y.storage)
+    if s is None:
+        with _there(stream, x.storage):
+            return lora_dev(opw, w, x, opa, a, opb, b, scale, plan, p, y, work)
+    at, have, work = _scratch(work, lib.eigamd_lora_work_bytes(kind, ow, m, n, k, at_w, w.ld, at_x, x.ld), x.storage)
+    rc = lib.eigamd_lora_dev(kind, ow, oa, ob, m, n, k, rank, count, at_w, w.ld, at_x, x.ld, at_a, a.ld, a.stride, at_b, b.ld, b.stride, at_s,
+                             plan.storage.data_ptr(), at_p, p.ld, at_y, y.ld, at, have, s)
+    if rc:
+        _lib.check(rc, "eigamd_lora_dev")
     return y
 
 
@@ -202,42 +223,56 @@ def lora_wgrad_dev(opg, u, p, scale, plan, beta, g, work=None, stream=None):
     u: DeviceMatrix (rows x tokens) or its Checkpoint8; p: F32 DeviceMatrix (rank x tokens); g: F32 MatrixStack, one matrix per
     adapter.  The gradient of b from u = dY and the forward pass's p; of a^T from u = x and the p of the call that made dX."""
     og = _op(opg)
-    if u.kind not in _KINDS:
+    kind = u.kind
+    if kind not in _KINDS:
         raise ValueError("the kind must be F32, BF16 or F16")
-    rows, n, rank = u.rows, plan.n, p.rows
-    packed = isinstance(u, Checkpoint8)
+    rows, n, rank, count = u.rows, plan.n, p.rows, plan.n_adapters
     if u.cols != n:
         raise ValueError("u and the plan have different numbers of tokens")
-    if not packed:
-        _check_matrix(u, u.kind, rows, n, "u")
-    _check_matrix(p, _lib.F32, rank, n, "p")
-    _check_stack(g, _lib.F32, *_turned(og, rows, rank), plan.n_adapters, "g")
-    _check_vector(scale, plan.n_adapters, torch.float32, "scale")
-    be, count = ctypes.c_float(beta), plan.n_adapters
-    tensors = (u.storage, p.storage, scale, plan.storage, g.storage)
-    exps, lde = 0, 0
-    if packed:
-        tensors, exps, lde = tensors + (u.exponents,), u.exponents.data_ptr(), u.lde
-    _run("eigamd_lora_wgrad_dev", stream, tensors, lib.eigamd_lora_wgrad_work_bytes(rows, n, rank, count), work,
-         lambda s, at, have: lib.eigamd_lora_wgrad_dev(u.kind, og, rows, n, rank, count, u.ptr, u.ld, exps, lde, p.ptr, p.ld,
-                                                       scale.data_ptr(), plan.storage.data_ptr(), ctypes.byref(be), g.ptr, g.ld, g.stride,
-                                                       at, have, s))
+    tensors, exps, lde = (u.storage, p.storage, scale, plan.storage, g.storage), 0, 0
+    if isinstance(u, Checkpoint8):
+        tensors, at_u, exps, lde = tensors + (u.exponents,), u.ptr, u.exponents.data_ptr(), u.lde
+    else:
+        at_u = _check_matrix(u, kind, rows, n, "u")
+    at_p = _check_matrix(p, _lib.F32, rank, n, "p")
+    at_g = _check_stack(g, _lib.F32, *_turned(og, rows, rank), count, "g")
+    at_s = _check_vector(scale, count, torch.float32, "scale")
+    s = _here(stream, *tensors)
+    if s is None:
+        with _there(stream, u.storage):
+            return lora_wgrad_dev(opg, u, p, scale, plan, beta, g, work)
+    at, have, work = _scratch(work, lib.eigamd_lora_wgrad_work_bytes(rows, n, rank, count), u.storage)
+    rc = lib.eigamd_lora_wgrad_dev(kind, og, rows, n, rank, count, at_u, u.ld, exps, lde, at_p, p.ld, at_s, plan.storage.data_ptr(),
+                                   ctypes.byref(ctypes.c_float(beta)), at_g, g.ld, g.stride, at, have, s)
+    if rc:
+        _lib.check(rc, "eigamd_lora_wgrad_dev")
     return g
+
+
+def _ckpt8(entry, x, c, stream, pack):
+    at_x = _check_matrix(x, c.kind, c.rows, c.cols, "x")
+    s = _here(stream, x.storage, c.storage, c.exponents)
+    if s is None:
+        with _there(stream, x.storage):
+            return _ckpt8(entry, x, c, None, pack)
+    at_q, at_e = c.storage.data_ptr(), c.exponents.data_ptr()
+    if pack:
+        rc = lib.eigamd_ckpt8_pack_dev(x.kind, x.rows, x.cols, at_x, x.ld, at_q, c.ld, at_e, c.lde, s)
+    else:
+        rc = lib.eigamd_ckpt8_unpack_dev(x.kind, x.rows, x.cols, at_q, c.ld, at_e, c.lde, at_x, x.ld, s)
+    if rc:
+        _lib.check(rc, entry)
 
 
 def ckpt8_pack_dev(x, c, stream=None):
     """The DeviceMatrix x (features x tokens) into the Checkpoint8 c of the same kind and shape."""
-    _check_matrix(x, c.kind, c.rows, c.cols, "x")
-    _run("eigamd_ckpt8_pack_dev", stream, (x.storage, c.storage, c.exponents), 0, None,
-         lambda s, at, have: lib.eigamd_ckpt8_pack_dev(x.kind, x.rows, x.cols, x.ptr, x.ld, c.ptr, c.ld, c.exponents.data_ptr(), c.lde, s))
+    _ckpt8("eigamd_ckpt8_pack_dev", x, c, stream, True)
     return c
 
 
 def ckpt8_unpack_dev(c, x, stream=None):
     """The values the Checkpoint8 c stands for into the DeviceMatrix x of the same kind and shape."""
-    _check_matrix(x, c.kind, c.rows, c.cols, "x")
-    _run("eigamd_ckpt8_unpack_dev", stream, (x.storage, c.storage, c.exponents), 0, None,
-         lambda s, at, have: lib.eigamd_ckpt8_unpack_dev(x.kind, x.rows, x.cols, c.ptr, c.ld, c.exponents.data_ptr(), c.lde, x.ptr, x.ld, s))
+    _ckpt8("eigamd_ckpt8_unpack_dev", x, c, stream, False)
     return x
 
 
@@ -245,13 +280,18 @@ def ckpt8_wgrad_dev(opw, dy, c, beta, dw, work=None, stream=None):
     """dw <- beta dw + dy x^T (opw 'N': features out x features in) or its transpose (opw 'T'), x the matrix that the
     Checkpoint8 c stands for; dy DeviceMatrix of c's kind, dw F32 DeviceMatrix."""
     ow = _op(opw)
-    m, n, k = dy.rows, c.cols, c.rows
-    if c.kind not in _KINDS:
+    kind, m, n, k = c.kind, dy.rows, c.cols, c.rows
+    if kind not in _KINDS:
         raise ValueError("the kind must be F32, BF16 or F16")
-    _check_matrix(dy, c.kind, m, n, "dy")
-    _check_matrix(dw, _lib.F32, *_turned(ow, m, k), "dw")
-    be = ctypes.c_float(beta)
-    _run("eigamd_ckpt8_wgrad_dev", stream, (dy.storage, c.storage, c.exponents, dw.storage), lib.eigamd_ckpt8_wgrad_work_bytes(c.kind, m, n, k, dy.ptr, dy.ld), work,
-         lambda s, at, have: lib.eigamd_ckpt8_wgrad_dev(c.kind, ow, m, n, k, dy.ptr, dy.ld, c.ptr, c.ld, c.exponents.data_ptr(), c.lde,
-                                                        ctypes.byref(be), dw.ptr, dw.ld, at, have, s))
+    at_dy = _check_matrix(dy, kind, m, n, "dy")
+    at_dw = _check_matrix(dw, _lib.F32, *_turned(ow, m, k), "dw")
+    s = _here(stream, dy.storage, c.storage, c.exponents, dw.storage)
+    if s is None:
+        with _there(stream, dy.storage):
+            return ckpt8_wgrad_dev(opw, dy, c, beta, dw, work)
+    at, have, work = _scratch(work, lib.eigamd_ckpt8_wgrad_work_bytes(kind, m, n, k, at_dy, dy.ld), dy.storage)
+    rc = lib.eigamd_ckpt8_wgrad_dev(kind, ow, m, n, k, at_dy, dy.ld, c.storage.data_ptr(), c.ld, c.exponents.data_ptr(), c.lde,
+                                    ctypes.byref(ctypes.c_float(beta)), at_dw, dw.ld, at, have, s)
+    if rc:
+        _lib.check(rc, "eigamd_ckpt8_wgrad_dev")
     return dw
