@@ -102,6 +102,17 @@ template <typename E, typename V> __device__ __forceinline__ V load_up_to_8(cons
   return v;
 }
 
+// The first n of 8 elements `stride` apart, the rest zero (p itself has to be readable even for n <= 0).  No load is conditional:
+// conditional ones would be waited for one by one.
+template <typename E, typename V> __device__ __forceinline__ V load_first(const E* p, int64_t stride, int n) {
+  V v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = p[(i < n ? i : 0) * stride];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? v[i] : (E)0.0f;
+  return v;
+}
+
 // n <= 8 whole numbers of 8 bits from p (any alignment), the rest zero.
 __device__ __forceinline__ uint64_t load_bytes(const int8_t* p, int n) {
   uint64_t v = 0;

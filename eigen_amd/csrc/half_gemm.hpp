@@ -170,88 +170,110 @@ template <typename T, int LAY, int R, int NT, bool GATHER> struct SliceLoader {
 // one adapter's factor must not reach another request's column, so the products are selected, not multiplied by zero).
 // P has 32 bits and goes through the matrix unit as two 16-bit pieces per value, normalised per token and 32 ranks: 16 bits
 // of it (bf16) or 22 (f16) take part, more than the result's type keeps.
+// Per 32 ranks, P's fragments do not depend on the adapter; of the adapters' factors the next one's are under way while one is
+// multiplied.
 template <typename T, int NI, int NJ>
 __device__ __forceinline__ void add_adapters(const HalfGemm& g, int row0, int col0, f32x4 (&acc)[NI][NJ]) {
   using E = typename T::elem;
   using x8 = typename T::x8;
+  using f32x8 = float __attribute__((ext_vector_type(8)));
   const int l = threadIdx.x & 63;
   const int col = col0 + l;
   const int mine = l < NJ * 16 && col < g.n ? g.seg[col] : g.none;
-  unsigned long long left = __ballot(mine != g.none);
+  const unsigned long long live = __ballot(mine != g.none);
+  if (!live) return;
   int64_t token[NJ];
+  float scale[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int c = col0 + j * 16 + (l & 15);
     token[j] = c < g.n ? g.order[c] : 0;
+    const int who = __shfl(mine, j * 16 + (l & 15));
+    scale[j] = who != g.none ? g.scale[who] : 0.0f;
   }
-  while (left) {
-    const int first = __builtin_ctzll(left);
-    const int who = __builtin_amdgcn_readlane(mine, first);
-    const unsigned long long mask = __ballot(mine == who);
-    left &= ~mask;
-    const E* up = static_cast<const E*>(g.up) + (int64_t)who * g.up_stride;
-    const float s = g.scale[who];
-    for (int r0 = 0; r0 < g.rank; r0 += 32) {
-      const int r = r0 + (l / 16) * 8, rn = g.rank - r;
-      x8 hi[NJ], lo[NJ];
-      float back[NJ];
+  for (int r0 = 0; r0 < g.rank; r0 += 32) {
+    // rows past the end repeat the last one (they are not stored); ranks past the end are zero in both operands
+    const int r = r0 + (l / 16) * 8 < g.rank ? r0 + (l / 16) * 8 : 0, rn = g.rank - r0 - (l / 16) * 8;
+    const bool chunks = g.rank % 8 == 0;
+    auto factor = [&](int who, int i) {
+      int row = row0 + i * 16 + (l & 15);
+      asm("" : "+v"(row));   // addresses are made here, not kept for every row block across the loops
+      row = row < g.m ? row : g.m - 1;
+      const E* at = static_cast<const E*>(g.up) + (int64_t)who * g.up_stride + (int64_t)row * g.up_row + (int64_t)r * g.up_rank;
+      if (!chunks || g.up_rank != 1) return load_first<E, x8>(at, g.up_rank, rn);
+      x8 u = load_8<E, x8>(at);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        if (!((mask >> (j * 16)) & 0xffff)) continue;
-        using f32x8 = float __attribute__((ext_vector_type(8)));
-        const f32x8 v = load_up_to_8<float, f32x8>(g.p + token[j] * g.ldp + r, rn);
+      for (int t = 0; t < 8; ++t) u[t] = rn > 0 ? u[t] : (E)0.0f;
+      return u;
+    };
+    x8 hi[NJ], lo[NJ];
+    float back[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const float* at = g.p + token[j] * g.ldp + r;
+      f32x8 v = chunks ? load_8<float, f32x8>(at) : load_first<float, f32x8>(at, 1, rn);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] = rn > 0 ? v[t] : 0.0f;
+      if constexpr (T::bytes == 4) {
+        back[j] = scale[j];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) hi[j][t] = v[t];
+      } else {
         float top = 0.0f;
 #pragma unroll
         for (int t = 0; t < 8; ++t) top = fmaxf(top, __builtin_fabsf(v[t]));
-        if constexpr (T::bytes == 4) {
-          back[j] = s;
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const Norm nm = norm_of(top);
+        back[j] = nm.up * scale[j];
 #pragma unroll
-          for (int t = 0; t < 8; ++t) hi[j][t] = v[t];
-        } else {
-          top = fmaxf(top, __shfl_xor(top, 16));
-          top = fmaxf(top, __shfl_xor(top, 32));
-          const Norm nm = norm_of(top);
-          back[j] = nm.up * s;
-#pragma unroll
-          for (int t = 0; t < 8; ++t) {
-            E piece[2];
-            split<T, 2>(v[t] * nm.down, piece);
-            hi[j][t] = piece[0];
-            lo[j][t] = piece[1];
-          }
+        for (int t = 0; t < 8; ++t) {
+          E piece[2];
+          split<T, 2>(v[t] * nm.down, piece);
+          hi[j][t] = piece[0];
+          lo[j][t] = piece[1];
         }
       }
-      // four row blocks' factors under way together
-      constexpr int GI = NI < 4 ? NI : 4;
+    }
+    // Four row blocks' factors under way together; those of the next adapter while this one's are multiplied, if they are all (the
+    // large tile has no registers for that).
+    constexpr int GI = NI < 4 ? NI : 4;
+    constexpr bool AHEAD = NI == GI;
+    unsigned long long left = live;
+    int who = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+    x8 u[GI];
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < GI; ++i) u[i] = factor(who, i);
+    }
+    while (true) {
+      const unsigned long long mask = __ballot(mine == who);
+      left &= ~mask;
+      const bool more = left != 0;
+      const int next = more ? __builtin_amdgcn_readlane(mine, __builtin_ctzll(left)) : who;
 #pragma unroll
       for (int i0 = 0; i0 < NI; i0 += GI) {
-        x8 u[GI];
+        if constexpr (!AHEAD) {
+#pragma unroll
+          for (int i = 0; i < GI; ++i) u[i] = factor(who, i0 + i);
+        }
 #pragma unroll
         for (int i = 0; i < GI; ++i) {
-          int row = row0 + (i0 + i) * 16 + (l & 15);
-          asm("" : "+v"(row));   // addresses are made here, not kept for every row block across the loops
-          const E* at = up + (int64_t)row * g.up_row + (int64_t)r * g.up_rank;
-          const int n = row < g.m ? rn : 0;
-          if (g.up_rank == 1) {
-            u[i] = load_up_to_8<E, x8>(at, n);
-          } else {
 #pragma unroll
-            for (int t = 0; t < 8; ++t) u[i][t] = t < n ? at[(int64_t)t * g.up_rank] : (E)0.0f;
+          for (int j = 0; j < NJ; ++j) {
+            if (!((mask >> (j * 16)) & 0xffff)) continue;
+            f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (T::bytes == 2) d = T::mma(u[i], lo[j], d);
+            d = T::mma(u[i], hi[j], d);
+            const bool on = (mask >> (j * 16 + (l & 15))) & 1;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc[i0 + i][j][t] += on ? d[t] * back[j] : 0.0f;
           }
-        }
-#pragma unroll
-        for (int i = 0; i < GI; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          if (!((mask >> (j * 16)) & 0xffff)) continue;
-          f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
-          if constexpr (T::bytes == 2) d = T::mma(u[i], lo[j], d);
-          d = T::mma(u[i], hi[j], d);
-          const bool on = (mask >> (j * 16 + (l & 15))) & 1;
-#pragma unroll
-          for (int t = 0; t < 4; ++t) acc[i0 + i][j][t] += on ? d[t] * back[j] : 0.0f;
+          if (AHEAD && more) u[i] = factor(next, i);
         }
       }
+      if (!more) break;
+      who = next;
     }
   }
 }
@@ -274,7 +296,7 @@ enum { OUT_HALF = 0, OUT_F32 = 1, OUT_F32_SWAPPED = 2 };
 // OUT_HALF: C in the operands' type, columns scattered by `order`, adapters added.
 // OUT_F32: C = beta C + A B in 32 bits.  OUT_F32_SWAPPED: the same with C stored transposed (N x M column-major).
 template <typename T, int LA, int LB, int OUT, int BM, int BN, int WM, int WN, int D>
-__global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
+__global__ __launch_bounds__(WM * WN * 64, 2) void half_gemm_kernel(HalfGemm g) {
   constexpr int NT = WM * WN * 64, TM = BM / WM, TN = BN / WN, NI = TM / 16, NJ = TN / 16;
   using LoadA = SliceLoader<T, LA, BM, NT, false>;
   using LoadB = SliceLoader<T, LB, BN, NT, OUT == OUT_HALF>;
@@ -405,81 +427,112 @@ __global__ __launch_bounds__(WM * WN * 64) void half_gemm_kernel(HalfGemm g) {
   }
   slice_barrier<0>();
 
-  const int row0 = tm * BM + wr, col0 = tn * BN + wc;
-  if (g.splits > 1) {
-    // sums of this piece, in C's own order; joined by a second kernel in the order of the pieces
-    float* out = g.partial + (int64_t)blockIdx.y * g.m * g.n;
-    const int64_t ld = OUT == OUT_F32_SWAPPED ? g.n : g.m;
-    const int rows = OUT == OUT_F32_SWAPPED ? g.n : g.m, cols = OUT == OUT_F32_SWAPPED ? g.m : g.n;
-    const bool wide = ld % 4 == 0;
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int r = (OUT == OUT_F32_SWAPPED ? col0 + j * 16 : row0 + i * 16) + (l / 16) * 4;
-        const int c = (OUT == OUT_F32_SWAPPED ? row0 + i * 16 : col0 + j * 16) + (l & 15);
-        if (c >= cols) continue;
-        float* at = out + (int64_t)c * ld + r;
-        if (wide && r < rows) *reinterpret_cast<f32x4*>(at) = acc[i][j];
-        else
-          for (int t = 0; t < 4; ++t)
-            if (r + t < rows) at[t] = acc[i][j][t];
-      }
-    return;
-  }
-  if constexpr (OUT == OUT_HALF) {
-    // through LDS (the slices are done with; every wave stays in its own part): whole lines of C per store
+  // Out through LDS (the slices are done with; every wave stays in its own part), 16 of this wave's columns of C at a time, so that
+  // neighbouring lanes store neighbouring rows, alignment or not.  Swapped: the tile's columns are C's rows.
+  constexpr bool SWAPPED = OUT == OUT_F32_SWAPPED;
+  constexpr int CR = SWAPPED ? TN : TM, CN = (SWAPPED ? TM : TN) / 16;
+  const int c_row0 = SWAPPED ? tn * BN + wc : tm * BM + wr, c_col0 = SWAPPED ? tm * BM + wr : tn * BN + wc;
+  const int c_rows = SWAPPED ? g.n : g.m, c_cols = SWAPPED ? g.m : g.n;
+  auto block = [&](int r, int c) -> const f32x4& { return SWAPPED ? acc[c][r] : acc[r][c]; };
+  if (OUT == OUT_HALF && g.splits == 1) {
     using E = typename T::elem;
-    constexpr int line = TM * 2 + 16;
+    using x4 = typename T::x4;
+    using x8 = typename T::x8;
+    constexpr int line = CR * 2 + 16;
     static_assert(16 * line * WM * WN <= D * slice, "the epilogue's part of LDS");
     char* mine = lds + w * 16 * line;
     E* C = static_cast<E*>(g.c);
     const bool wide = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && g.ldc % 8 == 0;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
+    for (int j = 0; j < CN; ++j) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        typename T::x4 v;
+      for (int i = 0; i < CR / 16; ++i) {
+        const f32x4& a = block(i, j);
+        x4 v;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) v[t] = (E)acc[i][j][t];
-        *reinterpret_cast<typename T::x4*>(mine + (l & 15) * line + (i * 16 + (l / 16) * 4) * 2) = v;
+        for (int t = 0; t < 4; ++t) v[t] = (E)a[t];
+        *reinterpret_cast<x4*>(mine + (l & 15) * line + (i * 16 + (l / 16) * 4) * 2) = v;
       }
       __builtin_amdgcn_wave_barrier();
-      constexpr int per = TM / 8;                    // 16-byte chunks of a column
+      if (wide) {
+        constexpr int per = CR / 8;                    // 16-byte chunks of a column
 #pragma unroll
-      for (int q = 0; q < 16 * per / 64; ++q) {
-        const int ch = q * 64 + l, cj = ch / per, r = row0 + (ch % per) * 8, c = col0 + j * 16 + cj;
-        const typename T::x8 v = *reinterpret_cast<const typename T::x8*>(mine + cj * line + (ch % per) * 16);
-        if (c >= g.n) continue;
-        E* at = C + (int64_t)(g.order ? g.order[c] : c) * g.ldc + r;
-        if (wide && r + 8 <= g.m) *reinterpret_cast<typename T::x8*>(at) = v;
-        else
-          for (int t = 0; t < 8; ++t)
-            if (r + t < g.m) at[t] = v[t];
+        for (int q = 0; q < 16 * per / 64; ++q) {
+          const int ch = q * 64 + l, c = c_col0 + j * 16 + ch / per, r = c_row0 + ch % per * 8;
+          const x8 v = *reinterpret_cast<const x8*>(mine + ch / per * line + ch % per * 16);
+          if (c >= c_cols) continue;
+          E* at = C + (int64_t)(g.order ? g.order[c] : c) * g.ldc + r;
+          if (r + 8 <= c_rows) *reinterpret_cast<x8*>(at) = v;
+          else
+            for (int t = 0; t < 8; ++t)
+              if (r + t < c_rows) at[t] = v[t];
+        }
+      } else {
+        for (int q = l; q < 16 * CR; q += 64) {
+          const int c = c_col0 + j * 16 + q / CR, r = c_row0 + q % CR;
+          const E v = *reinterpret_cast<const E*>(mine + q / CR * line + q % CR * 2);
+          if (c < c_cols && r < c_rows) C[(int64_t)(g.order ? g.order[c] : c) * g.ldc + r] = v;
+        }
       }
       __builtin_amdgcn_wave_barrier();
     }
-  } else {
-    float* C = static_cast<float*>(g.c);
-    const int rows = OUT == OUT_F32_SWAPPED ? g.n : g.m, cols = OUT == OUT_F32_SWAPPED ? g.m : g.n;
-    const bool wide = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && g.ldc % 4 == 0;
+    return;
+  }
+  // 32 bits: the result, or this piece's sums in C's own order (joined by a second kernel in the order of the pieces); a lane's four
+  // rows are 16 bytes of a column, four lanes 64, which go out as they are.
+  const bool sums = g.splits > 1;
+  float* C = sums ? g.partial + (int64_t)blockIdx.y * g.m * g.n : static_cast<float*>(g.c);
+  const int64_t ldc = sums ? c_rows : g.ldc;
+  const float beta = sums ? 0.0f : g.beta;
+  if ((reinterpret_cast<uintptr_t>(C) & 15) == 0 && ldc % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+    for (int j = 0; j < CN; ++j)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int r = (OUT == OUT_F32_SWAPPED ? col0 + j * 16 : row0 + i * 16) + (l / 16) * 4;
-        const int c = (OUT == OUT_F32_SWAPPED ? row0 + i * 16 : col0 + j * 16) + (l & 15);
-        if (c >= cols) continue;
-        float* at = C + (int64_t)c * g.ldc + r;
-        f32x4 v = acc[i][j];
-        if (wide && r + 4 <= rows) {
-          if (g.beta != 0.0f) v += g.beta * *reinterpret_cast<const f32x4*>(at);
+      for (int i = 0; i < CR / 16; ++i) {
+        const int r = c_row0 + i * 16 + (l / 16) * 4, c = c_col0 + j * 16 + (l & 15);
+        if (c >= c_cols) continue;
+        float* at = C + (int64_t)c * ldc + r;
+        f32x4 v = block(i, j);
+        if (r + 4 <= c_rows) {
+          if (beta != 0.0f) v += beta * *reinterpret_cast<const f32x4*>(at);
           *reinterpret_cast<f32x4*>(at) = v;
         } else {
           for (int t = 0; t < 4; ++t)
-            if (r + t < rows) at[t] = v[t] + (g.beta != 0.0f ? g.beta * at[t] : 0.0f);
+            if (r + t < c_rows) at[t] = v[t] + (beta != 0.0f ? beta * at[t] : 0.0f);
         }
       }
+    return;
+  }
+  constexpr int line = CR * 4 + 16;
+  static_assert(16 * line * WM * WN <= D * slice, "the epilogue's part of LDS");
+  char* mine = lds + w * 16 * line;
+#pragma unroll
+  for (int j = 0; j < CN; ++j) {
+#pragma unroll
+    for (int i = 0; i < CR / 16; ++i) *reinterpret_cast<f32x4*>(mine + (l & 15) * line + (i * 16 + (l / 16) * 4) * 4) = block(i, j);
+    __builtin_amdgcn_wave_barrier();
+    constexpr int B = 8;      // old values of this many rows under way together
+    static_assert(16 * CR / 64 % B == 0, "whole batches");
+#pragma unroll 1
+    for (int q0 = 0; q0 < 16 * CR / 64; q0 += B) {
+      float v[B], old[B];
+      float* at[B];
+#pragma unroll
+      for (int t = 0; t < B; ++t) {
+        const int q = (q0 + t) * 64 + l, c = c_col0 + j * 16 + q / CR, r = c_row0 + q % CR;
+        v[t] = *reinterpret_cast<const float*>(mine + q / CR * line + q % CR * 4);
+        at[t] = c < c_cols && r < c_rows ? C + (int64_t)c * ldc + r : nullptr;
+        old[t] = 0.0f;
+      }
+      if (beta != 0.0f) {
+#pragma unroll
+        for (int t = 0; t < B; ++t) old[t] = at[t] ? beta * *at[t] : 0.0f;
+      }
+#pragma unroll
+      for (int t = 0; t < B; ++t)
+        if (at[t]) *at[t] = v[t] + old[t];
+    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -560,10 +613,10 @@ inline hipError_t launch_half_join(const float* partial, int splits, int rows, i
   return hipGetLastError();
 }
 
-// Which tile, and how many pieces of the reduction.  Measured at k = 4096 (bf16), a round of the 256 compute units takes 90 us with
-// 256 x 256 tiles; 57 us with 128 x 128 tiles two to a unit, 48 us where each has its unit to itself; 39 us in the form for that
-// (eight waves, four slices in LDS).  A reduction is split where the tiles leave units idle: a piece costs about 0.55 us per 64
-// positions, the join a launch and the traffic of its sums.
+// Which tile, and how many pieces of the reduction.  Times of a 64-deep slice, measured with bf16 at 4096 rows and up to 4096
+// columns: 1.5 us with 256 x 256 tiles; 0.86 with 128 x 128 tiles two to a compute unit, 0.72 where each has its unit to itself;
+// 0.55 in the form for that (eight waves, four slices in LDS).  A round of tiles over the 256 units takes its slices and 11, 8 or
+// 5 us beside them; splitting the reduction costs another launch and the traffic of the sums.
 enum { TILE_256, TILE_128, TILE_128_ALONE };
 struct TilePlan {
   int tile, splits;
@@ -571,23 +624,24 @@ struct TilePlan {
 };
 inline TilePlan plan_tiles(int64_t m, int64_t n, int64_t k) {
   const int64_t t128 = ((m + 127) / 128) * ((n + 127) / 128), t256 = ((m + 255) / 256) * ((n + 255) / 256);
-  TilePlan plan = {TILE_128_ALONE, 1, k > 0 ? (k + 63) / 64 * 64 : 64};
-  if (t128 <= 256) {
-    double best = 1e30;
-    for (int64_t s = 1; s * t128 <= 256 && (s == 1 || k / s >= 128) && s <= 32; ++s) {
-      const int64_t piece = ((k + s - 1) / s + 63) / 64 * 64;
-      const double cost = 0.55 * (double)(piece / 64) + (s > 1 ? 2.5 + (double)s * (double)m * (double)n * 8.0 / 4.0e6 : 0.0);
-      if (cost < 0.9 * best) {
-        best = cost;
-        plan.k_piece = piece > 64 ? piece : 64;
-        plan.splits = (int)(k > 0 ? (k + plan.k_piece - 1) / plan.k_piece : 1);
+  TilePlan plan = {TILE_128_ALONE, 1, 64};
+  double best = 1e30;
+  for (int64_t s = 1; s <= 32 && (s == 1 || (k / s >= 128 && s * t256 <= 512)); ++s) {
+    const int64_t piece = k > 0 ? ((k + s - 1) / s + 63) / 64 * 64 : 64;
+    const double slices = (double)(piece / 64), join = s > 1 ? 2.5 + (double)s * (double)m * (double)n * 8.0 / 4.0e6 : 0.0;
+    const int64_t full = s * t128 / 512, rest = s * t128 % 512;
+    const double rounds256 = (double)((s * t256 + 255) / 256);
+    const double cost[3] = {
+        rounds256 * (1.5 * slices + 11.0),
+        (double)full * (0.86 * slices + 8.0) + (rest == 0 ? 0.0 : rest <= 256 ? 0.72 * slices + 8.0 : 0.86 * slices + 8.0),
+        s * t128 <= 256 ? 0.55 * slices + 5.0 : 1e30,
+    };
+    for (int t = 0; t < 3; ++t)
+      if (cost[t] + join < (s > 1 ? 0.92 : 0.999) * best) {      // a further piece has to win clearly
+        best = cost[t] + join;
+        plan = {t, (int)(k > 0 ? (k + piece - 1) / piece : 1), piece};
       }
-    }
-    return plan;
   }
-  const int64_t full = t128 / 512, rest = t128 % 512;
-  const double small = 57.0 * (double)full + (rest == 0 ? 0.0 : rest <= 256 ? 48.0 : 57.0), large = 90.0 * (double)((t256 + 255) / 256);
-  plan.tile = large <= small ? TILE_256 : TILE_128;
   return plan;
 }
 

@@ -57,10 +57,10 @@ __global__ __launch_bounds__(256) void lora_plan_kernel(const int* __restrict__ 
 
 template <typename T, int RT, int FORM> __global__ __launch_bounds__(512) void lora_project_kernel(ProjectArgs g) {
   __shared__ __align__(1024) char lds[project_lds(RT)];
-  project_piece<T, RT, FORM>(g, blockIdx.x, blockIdx.y * 64, lds);
+  project_piece<T, RT, FORM>(g, blockIdx.x, blockIdx.y * 16 * RT, lds);
 }
 template <typename T, int RT> hipError_t launch_project_rank(const ProjectArgs& g, hipStream_t s) {
-  const dim3 grid((unsigned)project_slots(g), (g.rank + 63) / 64);
+  const dim3 grid((unsigned)project_slots(g), (g.rank + 16 * RT - 1) / (16 * RT));
   switch (project_form<T>(g)) {
     case A_K: hipLaunchKernelGGL((lora_project_kernel<T, RT, A_K>), grid, dim3(512), 0, s, g); break;
     case A_R:
@@ -70,30 +70,26 @@ template <typename T, int RT> hipError_t launch_project_rank(const ProjectArgs& 
   }
   return hipGetLastError();
 }
+// Few pieces: 16 ranks a workgroup, so that there are more of them (142 tokens x 4032, rank 64: 25 -> 9 us); many: X is read once.
 template <typename T> hipError_t launch_project(const ProjectArgs& g, hipStream_t s) {
-  if (g.rank <= 16) return launch_project_rank<T, 1>(g, s);
+  if (g.rank <= 16 || project_slots(g) * ((g.rank + 15) / 16) <= 512) return launch_project_rank<T, 1>(g, s);
   if (g.rank <= 32) return launch_project_rank<T, 2>(g, s);
   return launch_project_rank<T, 4>(g, s);
 }
 
-// Y += s_j op(B_j) P in single precision, behind the plain product: a wave takes 16 rows of 64 columns, so that there are many of
-// them (64 rows a wave left most units idle: 777 tokens x 1024 took 24 us).
+// Y += s_j op(B_j) P in single precision, behind the plain product: a wave takes 16 rows of 16 columns, so that there are many of
+// them, each with few adapters (64 x 64 a wave left most units idle: 777 tokens x 1024 took 24 us, now 7).
 __global__ __launch_bounds__(256) void lora_add_f32_kernel(HalfGemm g) {
   const int w = threadIdx.x / 64, l = threadIdx.x & 63;
-  const int row0 = blockIdx.y * 64 + w * 16, col0 = blockIdx.x * 64;
+  const int row0 = blockIdx.y * 64 + w * 16, col0 = blockIdx.x * 16;
   if (row0 >= g.m) return;
-  f32x4 acc[1][4] = {};
-  add_adapters<Fp32, 1, 4>(g, row0, col0, acc);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int c = col0 + j * 16 + (l & 15);
-    if (c >= g.n || g.seg[c] == g.none) continue;
-    float* y = static_cast<float*>(g.c) + (int64_t)g.order[c] * g.ldc;
-    for (int t = 0; t < 4; ++t) {
-      const int r = row0 + (l / 16) * 4 + t;
-      if (r < g.m) y[r] += acc[0][j][t];
-    }
-  }
+  f32x4 acc[1][1] = {};
+  add_adapters<Fp32, 1, 1>(g, row0, col0, acc);
+  const int c = col0 + (l & 15), r = row0 + (l / 16) * 4;
+  if (c >= g.n || g.seg[c] == g.none) return;
+  float* y = static_cast<float*>(g.c) + (int64_t)g.order[c] * g.ldc;
+  for (int t = 0; t < 4; ++t)
+    if (r + t < g.m) y[r + t] += acc[0][0][t];
 }
 
 template <typename T, int LA, int B, int WM, int WN, int D> hipError_t launch_tiles(const HalfGemm& g, hipStream_t s) {
@@ -436,7 +432,7 @@ hipError_t lora_device(const LoraArgs& c, hipStream_t s) {
   g.up_rank = c.b_trans ? 1 : c.ldb;
   g.up_stride = c.stride_b;
   g.p = c.p; g.ldp = c.ldp; g.scale = c.scale;
-  hipLaunchKernelGGL(lora_add_f32_kernel, dim3((unsigned)((c.n + 63) / 64), (unsigned)((c.m + 63) / 64)), dim3(256), 0, s, g);
+  hipLaunchKernelGGL(lora_add_f32_kernel, dim3((unsigned)((c.n + 15) / 16), (unsigned)((c.m + 63) / 64)), dim3(256), 0, s, g);
   return hipGetLastError();
 }
 
