@@ -68,7 +68,7 @@ template <int KEEP> __device__ __forceinline__ void slice_barrier() {
 // Rows past the end are not cleared: whatever stands there meets only rows of C that are not stored.  Positions past the end of
 // the reduction are zero in both operands.
 // GATHER: row i is row order[i] of the matrix, and every chunk has an address of its own; otherwise they are 32-bit offsets from
-// a base that is the same in all lanes (256 rows or 64 lines of at most 2^21 elements).
+// a base that is the same in all lanes (256 rows or 64 lines of at most kMaxLine elements each: below 2^31 bytes).
 template <typename T, int LAY, int R, int NT, bool GATHER> struct SliceLoader {
   static_assert(LAY == KC || (R >= 128 && !GATHER), "the permutation of a line needs 16 chunks");
   static constexpr int N = R * 8 / NT;
@@ -536,10 +536,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void half_gemm_kernel(HalfGemm g) 
   }
 }
 
-// The direct loads take whole, aligned 16-byte chunks.  A matrix that has others (an odd leading dimension, an extent that is no
-// multiple of 8) is copied into scratch memory first, columns padded with zeros: reading it in place through registers took
+// The direct loads take whole, aligned 16-byte chunks at 32-bit offsets.  A matrix that has others (an odd leading dimension or one past
+// kMaxLine, an extent that is no multiple of 8) is copied into scratch memory first, columns padded with zeros: reading it in place through registers took
 // 378 us for 4096 tokens x 4095 x 4093, copies and product take 190 (4096 x 4096: 126).
-inline bool whole_chunks(const void* p, int64_t ld, int64_t rows) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && rows % 8 == 0; }
+constexpr int64_t kMaxLine = (int64_t)1 << 22;
+inline bool whole_chunks(const void* p, int64_t ld, int64_t rows) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && ld <= kMaxLine && rows % 8 == 0;
+}
 inline int64_t padded(int64_t rows) { return (rows + 7) / 8 * 8; }
 inline int64_t padded_bytes(int64_t rows, int64_t cols) { return (padded(rows) * cols * 2 + 255) / 256 * 256; }
 struct PadCopy {

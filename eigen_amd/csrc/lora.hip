@@ -23,54 +23,80 @@ hipError_t lora_few_device(int kind, bool w_trans, const HalfGemm& g, const Proj
 namespace {
 
 // ---------------------------------------------------------------------------------------------------------------- plan
-// One wave per adapter (and one for the tokens without): it counts the tokens in front of its run and lists its own in their
-// order, by ballots -- no atomics, no prefix sum over adapters, the same list every time.
-__global__ __launch_bounds__(256) void lora_plan_kernel(const int* __restrict__ ids, int n, int adapters, int* __restrict__ order,
+// One workgroup per adapter (and one for the tokens without): its waves count, each in its part of the batch, the tokens in front
+// of the adapter's run and the adapter's own, and then list those in their order, by ballots -- no atomics, no prefix sum over
+// adapters, the same list every time.  Eight loads of a wave are under way together.
+__global__ __launch_bounds__(512) void lora_plan_kernel(const int* __restrict__ ids, int n, int adapters, int* __restrict__ order,
                                                         int* __restrict__ seg, int* __restrict__ starts) {
-  const int j = blockIdx.x * 4 + threadIdx.x / 64, l = threadIdx.x & 63;
-  if (j > adapters) return;
-  int before = 0;
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    const int i = i0 + l;
-    int id = i < n ? ids[i] : -1;
-    if (id < 0 || id >= adapters) id = adapters;
-    before += __popcll(__ballot(i < n && id < j));
+  __shared__ int before[8], own[8];
+  const int j = blockIdx.x, w = threadIdx.x / 64, l = threadIdx.x & 63;
+  const int share = (n + 511) / 512 * 64, begin = w * share, end = begin + share < n ? begin + share : n;
+  auto load = [&](int i0, int (&id)[8]) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) id[t] = ids[i0 + t * 64 + l < end ? i0 + t * 64 + l : i0];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      if ((unsigned)id[t] >= (unsigned)adapters) id[t] = adapters;
+      if (i0 + t * 64 + l >= end) id[t] = adapters + 1;      // behind everything
+    }
+  };
+  int less = 0, same = 0;
+  for (int i0 = begin; i0 < end; i0 += 512) {
+    int id[8];
+    load(i0, id);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      less += __popcll(__ballot(id[t] < j));
+      same += __popcll(__ballot(id[t] == j));
+    }
   }
   if (l == 0) {
-    starts[j] = before;
+    before[w] = less;
+    own[w] = same;
+  }
+  __syncthreads();
+  int start = 0, at = 0;
+  for (int z = 0; z < 8; ++z) {
+    start += before[z];
+    at += z < w ? own[z] : 0;
+  }
+  if (threadIdx.x == 0) {
+    starts[j] = start;
     if (j == adapters) starts[adapters + 1] = n;
   }
-  int at = before;
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    const int i = i0 + l;
-    int id = i < n ? ids[i] : -1;
-    if (id < 0 || id >= adapters) id = adapters;
-    const unsigned long long mine = __ballot(i < n && id == j);
-    if (i < n && id == j) {
-      const int to = at + __popcll(mine & ((1ull << l) - 1));
-      order[to] = i;
-      seg[to] = j;
+  at += start;
+  for (int i0 = begin; i0 < end; i0 += 512) {
+    int id[8];
+    load(i0, id);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const unsigned long long mine = __ballot(id[t] == j);
+      if (id[t] == j) {
+        const int to = at + __popcll(mine & ((1ull << l) - 1));
+        order[to] = i0 + t * 64 + l;
+        seg[to] = j;
+      }
+      at += __popcll(mine);
     }
-    at += __popcll(mine);
   }
 }
 
-template <typename T, int RT, int FORM> __global__ __launch_bounds__(512) void lora_project_kernel(ProjectArgs g) {
+template <typename T, int RT, int FORM> __global__ __launch_bounds__(kProjWaves * 64) void lora_project_kernel(ProjectArgs g) {
   __shared__ __align__(1024) char lds[project_lds(RT)];
   project_piece<T, RT, FORM>(g, blockIdx.x, blockIdx.y * 16 * RT, lds);
 }
 template <typename T, int RT> hipError_t launch_project_rank(const ProjectArgs& g, hipStream_t s) {
   const dim3 grid((unsigned)project_slots(g), (g.rank + 16 * RT - 1) / (16 * RT));
   switch (project_form<T>(g)) {
-    case A_K: hipLaunchKernelGGL((lora_project_kernel<T, RT, A_K>), grid, dim3(512), 0, s, g); break;
+    case A_K: hipLaunchKernelGGL((lora_project_kernel<T, RT, A_K>), grid, dim3(kProjWaves * 64), 0, s, g); break;
     case A_R:
-      if constexpr (T::bytes == 2) hipLaunchKernelGGL((lora_project_kernel<T, RT, A_R>), grid, dim3(512), 0, s, g);
+      if constexpr (T::bytes == 2) hipLaunchKernelGGL((lora_project_kernel<T, RT, A_R>), grid, dim3(kProjWaves * 64), 0, s, g);
       break;
-    default: hipLaunchKernelGGL((lora_project_kernel<T, RT, A_ANY>), grid, dim3(512), 0, s, g);
+    default: hipLaunchKernelGGL((lora_project_kernel<T, RT, A_ANY>), grid, dim3(kProjWaves * 64), 0, s, g);
   }
   return hipGetLastError();
 }
-// Few pieces: 16 ranks a workgroup, so that there are more of them (142 tokens x 4032, rank 64: 25 -> 9 us); many: X is read once.
+// Few pieces: 16 ranks a workgroup, so that there are more of them (142 tokens x 4032, rank 64: 25 -> 15 us); many: X is read once.
 template <typename T> hipError_t launch_project(const ProjectArgs& g, hipStream_t s) {
   if (g.rank <= 16 || project_slots(g) * ((g.rank + 15) / 16) <= 512) return launch_project_rank<T, 1>(g, s);
   if (g.rank <= 32) return launch_project_rank<T, 2>(g, s);
@@ -123,7 +149,7 @@ HalfWork half_work(bool w_trans, int64_t m, int64_t n, int64_t k, const void* w,
   return need;
 }
 
-template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArgs& q, hipStream_t s) {
+HalfGemm gemm_args(const LoraArgs& c) {
   HalfGemm g;
   g.m = (int)c.m; g.n = (int)c.n; g.k = (int)c.k;
   g.a = c.w; g.lda = c.ldw;
@@ -139,6 +165,13 @@ template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArg
   g.up_stride = c.stride_b;
   g.p = c.p; g.ldp = c.ldp;
   g.scale = c.scale;
+  return g;
+}
+// Single precision has the few-token form for W with a contiguous reduction (there is no transposing read of 32-bit elements).
+bool few_f32(bool w_trans, int64_t n) { return w_trans && lora_few(n); }
+
+template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArgs& q, hipStream_t s) {
+  HalfGemm g = gemm_args(c);
   const HalfWork need = half_work(c.w_trans, c.m, c.n, c.k, c.w, c.ldw, c.x, c.ldx);
   char* work = static_cast<char*>(c.work);
   g.partial = reinterpret_cast<float*>(work);
@@ -385,14 +418,14 @@ hipError_t lora_project_device(int kind, const ProjectArgs& g, hipStream_t s) {
 }
 
 hipError_t lora_plan_device(const int* ids, int64_t n, int64_t adapters, int* d_plan, hipStream_t s) {
-  hipLaunchKernelGGL(lora_plan_kernel, dim3((unsigned)(adapters / 4 + 1)), dim3(256), 0, s, ids, (int)n, (int)adapters, d_plan,
+  hipLaunchKernelGGL(lora_plan_kernel, dim3((unsigned)(adapters + 1)), dim3(512), 0, s, ids, (int)n, (int)adapters, d_plan,
                      d_plan + n, d_plan + 2 * n);
   return hipGetLastError();
 }
 
 int64_t lora_work_bytes(int kind, bool w_trans, int64_t m, int64_t n, int64_t k, const void* w, int64_t ldw, const void* x, int64_t ldx) {
   if (m <= 0 || n <= 0) return 0;
-  if (kind == F32) return std::min<int64_t>(16 * m * n * 4, (int64_t)256 << 20);
+  if (kind == F32) return few_f32(w_trans, n) ? lora_few_work_bytes(m, n, k) : std::min<int64_t>(16 * m * n * 4, (int64_t)256 << 20);
   const HalfWork need = half_work(w_trans, m, n, k, w, ldw, x, ldx);
   return need.sums + need.w_copy + need.x_copy;
 }
@@ -407,6 +440,11 @@ hipError_t lora_device(const LoraArgs& c, hipStream_t s) {
   p.a_stride = c.stride_a;
   p.order = c.plan.order; p.starts = c.plan.starts;
   p.p = c.p; p.ldp = c.ldp;
+  if (c.m > 0 && c.kind == F32 && few_f32(c.w_trans, c.n)) {
+    HalfGemm g = gemm_args(c);
+    g.partial = static_cast<float*>(c.work);
+    return lora_few_device(F32, true, g, p, s);
+  }
   if (c.m > 0 && c.kind == BF16) return launch_half<Bf16>(c, p, s);
   if (c.m > 0 && c.kind == F16K) return launch_half<F16>(c, p, s);
   hipError_t e = hipSuccess;
@@ -423,15 +461,7 @@ hipError_t lora_device(const LoraArgs& c, hipStream_t s) {
   q.partials_bytes = c.work ? (size_t)c.work_bytes : 0;
   e = launch_gemm_f32(q, s);
   if (e != hipSuccess || c.plan.adapters == 0) return e;
-  HalfGemm g;
-  g.m = (int)c.m; g.n = (int)c.n; g.k = (int)c.k;
-  g.c = c.y; g.ldc = c.ldy;
-  g.order = c.plan.order; g.seg = c.plan.seg; g.none = c.plan.adapters; g.rank = (int)c.rank;
-  g.up = c.b;
-  g.up_row = c.b_trans ? c.ldb : 1;
-  g.up_rank = c.b_trans ? 1 : c.ldb;
-  g.up_stride = c.stride_b;
-  g.p = c.p; g.ldp = c.ldp; g.scale = c.scale;
+  const HalfGemm g = gemm_args(c);
   hipLaunchKernelGGL(lora_add_f32_kernel, dim3((unsigned)((c.n + 15) / 16), (unsigned)((c.m + 63) / 64)), dim3(256), 0, s, g);
   return hipGetLastError();
 }

@@ -52,61 +52,74 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
     b[c] = static_cast<const E*>(g.b) + (int64_t)g.order[at < g.n ? at : g.n - 1] * g.ldb;
   }
   f32x4 acc[4][NG] = {};
-  constexpr int S = NG == 4 ? 1 : NG == 2 || LA == MC ? 2 : 4, turn = 8 * 32 * S;
-  x8 fa[2][S][4], fb[2][S][NG];
-  auto load = [&](int k0, int set) {
-    const bool whole = k0 + 32 * S <= k_end;
+  // whole turns, then what is left, one product a wave (as in project_piece)
+  constexpr int S = NG == 4 || T::bytes == 4 ? 1 : NG == 2 || LA == MC ? 2 : 4;
+  using Whole = std::true_type;
+  using Rest = std::false_type;
+  auto load = [&](int k0, x8(&fa)[4], x8(&fb)[NG], auto whole) {
+    const int k = k0 + (l / 16) * 8, left = k_end - k;
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int k = k0 + s * 32 + (l / 16) * 8, left = k_end - k;
+    for (int t = 0; t < 4; ++t) {
+      if constexpr (LA == KC) {
+        fa[t] = whole ? load_8<E, x8>(a[t] + k) : load_first<E, x8>(a[t] + (left > 0 ? k : 0), 1, left);
+      } else {
+        const bool in = whole || k0 + t * 8 + l / 8 < k_end;
+        x8 v = load_8<E, x8>(in ? a[t] + (int64_t)k0 * g.lda : static_cast<const E*>(g.a));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = in ? v[e] : (E)0.0f;
+        fa[t] = v;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NG; ++c) fb[c] = whole ? load_8<E, x8>(b[c] + k) : load_first<E, x8>(b[c] + (left > 0 ? k : 0), 1, left);
+  };
+  auto multiply = [&](const x8(&fa)[4], const x8(&fb)[NG]) {
+    x8 f[4];
+    if constexpr (LA == MC) {
+      // lines of 64 rows, 128 bytes; chunks permuted so that the 8 lines a half wave reads meet all banks once
+      char* mine = lds + w * 4096;
+      auto slot = [](int line, int ch) { return line * 128 + (ch ^ (((line >> 1) & 1) | ((line >> 2) & 2)) << 1) * 16; };
+#pragma unroll
+      for (int t = 0; t < 4; ++t) *reinterpret_cast<x8*>(mine + slot(t * 8 + l / 8, l % 8)) = fa[t];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        if constexpr (LA == KC) fa[set][s][t] = whole ? load_8<E, x8>(a[t] + k) : load_up_to_8<E, x8>(a[t] + k, left);
-        else {
-          const int line = k0 + s * 32 + t * 8 + l / 8;
-          fa[set][s][t] = load_up_to_8<E, x8>(a[t] + (int64_t)(k0 + s * 32) * g.lda, whole || line < k_end ? 8 : 0);
-        }
+        union { x8 v; typename T::x4 h[2]; } u;
+        const int line = (l / 16) * 8 + (l & 15) / 4, ch = t * 2 + (l & 3) / 2;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) u.h[h] = T::read_transposed(mine + slot(line + 4 * h, ch) + (l & 1) * 8);
+        f[t] = u.v;
       }
+    } else {
 #pragma unroll
-      for (int c = 0; c < NG; ++c) fb[set][s][c] = whole ? load_8<E, x8>(b[c] + k) : load_up_to_8<E, x8>(b[c] + k, left);
+      for (int t = 0; t < 4; ++t) f[t] = fa[t];
     }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int c = 0; c < NG; ++c) acc[t][c] = T::mma(f[t], fb[c], acc[t][c]);
   };
-  auto multiply = [&](int set) {
+  x8 fa[2][S][4], fb[2][S][NG];
+  auto load_turn = [&](int turn, int set) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      x8 f[4];
-      if constexpr (LA == MC) {
-        // lines of 64 rows, 128 bytes; chunks permuted so that the 8 lines a half wave reads meet all banks once
-        char* mine = lds + w * 4096;
-        auto slot = [](int line, int ch) { return line * 128 + (ch ^ (((line >> 1) & 1) | ((line >> 2) & 2)) << 1) * 16; };
-#pragma unroll
-        for (int t = 0; t < 4; ++t) *reinterpret_cast<x8*>(mine + slot(t * 8 + l / 8, l % 8)) = fa[set][s][t];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          union { x8 v; typename T::x4 h[2]; } u;
-          const int line = (l / 16) * 8 + (l & 15) / 4, ch = t * 2 + (l & 3) / 2;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) u.h[h] = T::read_transposed(mine + slot(line + 4 * h, ch) + (l & 1) * 8);
-          f[t] = u.v;
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) f[t] = fa[set][s][t];
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int c = 0; c < NG; ++c) acc[t][c] = T::mma(f[t], fb[set][s][c], acc[t][c]);
-    }
+    for (int s = 0; s < S; ++s) load(k_begin + (turn * S + s) * 32, fa[set][s], fb[set][s], Whole{});
   };
-  int k0 = k_begin + w * 32 * S;
-  if (k0 < k_end) load(k0, 0);
-  for (; k0 < k_end; k0 += 2 * turn) {
-    if (k0 + turn < k_end) load(k0 + turn, 1);
-    multiply(0);
-    if (k0 + turn >= k_end) break;
-    if (k0 + 2 * turn < k_end) load(k0 + 2 * turn, 0);
-    multiply(1);
+  auto multiply_turn = [&](int set) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) multiply(fa[set][s], fb[set][s]);
+  };
+  const int turns = (k_end - k_begin) / (32 * S);
+  int at = w;
+  if (at < turns) load_turn(at, 0);
+  for (; at < turns; at += 16) {
+    if (at + 8 < turns) load_turn(at + 8, 1);
+    multiply_turn(0);
+    if (at + 8 >= turns) break;
+    if (at + 16 < turns) load_turn(at + 16, 0);
+    multiply_turn(1);
+  }
+  if (const int k0 = k_begin + (turns * S + w) * 32; k0 < k_end) {
+    load(k0, fa[0][0], fb[0][0], Rest{});
+    multiply(fa[0][0], fb[0][0]);
   }
   if constexpr (LA == MC) __syncthreads();
   f32x4(&red)[8][4][NG][64] = *reinterpret_cast<f32x4(*)[8][4][NG][64]>(lds);
@@ -159,14 +172,9 @@ template <typename T> __global__ __launch_bounds__(256) void lora_few_join_kerne
     const float* p = g.p + token * g.ldp;
     float d = 0.0f;
     for (int t = 0; t < g.rank; t += 8) {
-      const f32x8 pv = load_up_to_8<float, f32x8>(p + t, g.rank - t);
-      x8 u;
-      if (g.up_rank == 1) {
-        u = load_up_to_8<E, x8>(up + t, g.rank - t);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] = t + e < g.rank ? up[(int64_t)(t + e) * g.up_rank] : (E)0.0f;
-      }
+      const bool whole = t + 8 <= g.rank;
+      const f32x8 pv = whole ? load_8<float, f32x8>(p + t) : load_first<float, f32x8>(p + t, 1, g.rank - t);
+      const x8 u = whole && g.up_rank == 1 ? load_8<E, x8>(up + t) : load_first<E, x8>(up + (int64_t)t * g.up_rank, g.up_rank, g.rank - t);
 #pragma unroll
       for (int e = 0; e < 8; ++e) d += (float)u[e] * pv[e];
     }
@@ -195,8 +203,10 @@ int few_pieces(int64_t m, int64_t k, int64_t project, int64_t* k_piece) {
 template <typename T, int LA, int NG> hipError_t launch_few_tokens(const HalfGemm& g, const ProjectArgs& q, int form, hipStream_t s) {
   const int slots = q.none && form != A_ANY ? (int)project_slots(q) : 0, project = slots * ((q.rank + 15) / 16);
   const dim3 grid((unsigned)(project + (g.m + 63) / 64 * g.splits));
-  if (form == A_R) hipLaunchKernelGGL((lora_few_kernel<T, LA, NG, A_R>), grid, dim3(512), 0, s, g, q, project, slots);
-  else hipLaunchKernelGGL((lora_few_kernel<T, LA, NG, A_K>), grid, dim3(512), 0, s, g, q, project, slots);
+  if constexpr (T::bytes == 2) {
+    if (form == A_R) hipLaunchKernelGGL((lora_few_kernel<T, LA, NG, A_R>), grid, dim3(512), 0, s, g, q, project, slots);
+  }
+  if (form != A_R) hipLaunchKernelGGL((lora_few_kernel<T, LA, NG, A_K>), grid, dim3(512), 0, s, g, q, project, slots);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(lora_few_join_kernel<T>, dim3((unsigned)((g.m + 255) / 256), (unsigned)g.n), dim3(256), 0, s, g);
@@ -206,7 +216,7 @@ template <typename T, int LA> hipError_t launch_few(HalfGemm g, const ProjectArg
   // factors that are read element by element keep the projection in a launch of its own
   const int form = project_form<T>(q);
   if (q.none && form == A_ANY) {
-    hipError_t e = lora_project_device(__is_same(T, Bf16) ? (int)BF16 : (int)F16K, q, s);
+    hipError_t e = lora_project_device(T::bytes == 4 ? 0 : __is_same(T, Bf16) ? (int)BF16 : (int)F16K, q, s);
     if (e != hipSuccess) return e;
   }
   int64_t piece;
@@ -226,6 +236,7 @@ int64_t lora_few_work_bytes(int64_t m, int64_t n, int64_t k) {
 }
 
 hipError_t lora_few_device(int kind, bool w_trans, const HalfGemm& g, const ProjectArgs& q, hipStream_t s) {
+  if (kind != BF16 && kind != F16K) return w_trans ? launch_few<Fp32, KC>(g, q, s) : hipErrorInvalidValue;
   if (kind == BF16) return w_trans ? launch_few<Bf16, KC>(g, q, s) : launch_few<Bf16, MC>(g, q, s);
   return w_trans ? launch_few<F16, KC>(g, q, s) : launch_few<F16, MC>(g, q, s);
 }

@@ -1,10 +1,12 @@
 // The projection of the adapter product, P(:,i) = op(A_j) x_i: the body that its own launch and the few-token launch share.
 #pragma once
+#include <type_traits>
+
 #include "half.hpp"
 
 namespace eigamd {
 
-constexpr int kProjTokens = 32;
+constexpr int kProjTokens = 32, kProjWaves = 8;
 struct ProjectArgs {
   int n, k, rank, none;
   const void* x; int64_t ldx;
@@ -23,16 +25,16 @@ struct ProjectArgs {
 //         x 4096, now 18)
 //   A_ANY element by element: ranks that are no multiple of 8, odd strides
 enum { A_K, A_R, A_ANY };
-constexpr int project_lds(int rt) { return 8 * rt * 2 * 64 * 16; }
+constexpr int project_lds(int rt) { return kProjWaves * rt * 2 * 64 * 16; }
 template <typename T, int RT, int FORM> __device__ __forceinline__ void project_piece(const ProjectArgs& g, int slot_id, int r0, char* lds) {
   using E = typename T::elem;
   using x8 = typename T::x8;
   Piece piece;
   if (!find_piece(g.starts, g.none + 1, kProjTokens, slot_id, piece)) return;
-  const int w = threadIdx.x / 64, l = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63;
   constexpr int line = RT * 32;                      // A_R: 32 positions x 16 RT ranks per wave
-  static_assert(8 * 32 * line <= project_lds(RT), "transposition and sums share LDS");
-  f32x4(&red)[8][RT][2][64] = *reinterpret_cast<f32x4(*)[8][RT][2][64]>(lds);
+  static_assert(kProjWaves * 32 * line <= project_lds(RT), "transposition and sums share LDS");
+  f32x4(&red)[kProjWaves][RT][2][64] = *reinterpret_cast<f32x4(*)[kProjWaves][RT][2][64]>(lds);
   const bool live = piece.adapter != g.none;
   if (live) {
     // lanes past the piece or the rank repeat the last one; what they compute is not stored
@@ -57,64 +59,77 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
         a[t] = factor + (int64_t)(r < g.rank ? r : g.rank - 1) * g.a_row;
       }
     }
-    constexpr int S = T::bytes == 4 ? (RT == 1 ? 2 : 1) : RT == 4 ? 2 : 4, turn = 8 * 32 * S;      // products of a turn; positions all waves take in one
-    x8 fx[2][S][2], fa[2][S][RT];
-    auto load = [&](int k0, int set) {
-      const bool whole = k0 + 32 * S <= g.k;
+    // Turns of S products.  Whole turns and what is left behind the last one (up to S products, one a wave) are loaded by code of
+    // their own: a bound on every load of the loop made it several times as long, and fetching it was most of a short call.
+    constexpr int S = T::bytes == 4 ? (RT == 1 ? 2 : 1) : RT == 4 ? 2 : 4;
+    static_assert(S <= kProjWaves, "one product a wave");
+    using Whole = std::true_type;
+    using Rest = std::false_type;
+    auto load = [&](int k0, x8(&fx)[2], x8(&fa)[RT], auto whole) {
+      const int k = k0 + (l / 16) * 8, left = g.k - k;
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const int k = k0 + s * 32 + (l / 16) * 8, left = g.k - k;
+      for (int c = 0; c < 2; ++c) fx[c] = whole ? load_8<E, x8>(x[c] + k) : load_first<E, x8>(x[c] + (left > 0 ? k : 0), 1, left);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) fx[set][s][c] = whole ? load_8<E, x8>(x[c] + k) : load_up_to_8<E, x8>(x[c] + k, left);
+      for (int t = 0; t < RT; ++t) {
+        if constexpr (FORM == A_R) {
+          const bool in = whole || k0 + (t * 64 + l) / per < g.k;
+          x8 v = load_8<E, x8>(in ? a[t] + (int64_t)k0 * g.a_k : factor);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = in ? v[e] : (E)0.0f;
+          fa[t] = v;
+        } else if constexpr (FORM == A_K && whole) {
+          fa[t] = load_8<E, x8>(a[t] + k);
+        } else {
+          fa[t] = load_first<E, x8>(a[t] + (left > 0 ? (int64_t)k * g.a_k : 0), g.a_k, whole ? 8 : left);
+        }
+      }
+    };
+    auto multiply = [&](const x8(&fx)[2], const x8(&fa)[RT]) {
+      x8 f[RT];
+      if constexpr (FORM == A_R) {
+        char* mine = lds + w * 32 * line;
+        auto slot = [&](int ln, int ch) { return ln * line + ((ch ^ ((ln & 3) << 1)) & (per - 1)) * 16; };
+#pragma unroll
+        for (int t = 0; t < RT; ++t) *reinterpret_cast<x8*>(mine + slot((t * 64 + l) / per, (t * 64 + l) % per)) = fa[t];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          if constexpr (FORM == A_K) {
-            fa[set][s][t] = whole ? load_8<E, x8>(a[t] + k) : load_up_to_8<E, x8>(a[t] + k, left);
-          } else if constexpr (FORM == A_R) {
-            const int at = k0 + s * 32 + (t * 64 + l) / per;
-            fa[set][s][t] = load_up_to_8<E, x8>(a[t] + (int64_t)(k0 + s * 32) * g.a_k, at < g.k ? 8 : 0);
-          } else {
+          union { x8 v; typename T::x4 h[2]; } u;
+          const int ln = (l / 16) * 8 + (l & 15) / 4, ch = t * 2 + (l & 3) / 2;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) fa[set][s][t][e] = e < left ? a[t][(int64_t)(k + e) * g.a_k] : (E)0.0f;
-          }
+          for (int h = 0; h < 2; ++h) u.h[h] = T::read_transposed(mine + slot(ln + 4 * h, ch) + (l & 1) * 8);
+          f[t] = u.v;
         }
+      } else {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) f[t] = fa[t];
       }
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) acc[t][c] = T::mma(f[t], fx[c], acc[t][c]);
     };
-    auto multiply = [&](int set) {
+    x8 fx[2][S][2], fa[2][S][RT];
+    auto load_turn = [&](int turn, int set) {
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        x8 f[RT];
-        if constexpr (FORM == A_R) {
-          char* mine = lds + w * 32 * line;
-          auto slot = [&](int ln, int ch) { return ln * line + ((ch ^ ((ln & 3) << 1)) & (per - 1)) * 16; };
-#pragma unroll
-          for (int t = 0; t < RT; ++t) *reinterpret_cast<x8*>(mine + slot((t * 64 + l) / per, (t * 64 + l) % per)) = fa[set][s][t];
-#pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            union { x8 v; typename T::x4 h[2]; } u;
-            const int ln = (l / 16) * 8 + (l & 15) / 4, ch = t * 2 + (l & 3) / 2;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) u.h[h] = T::read_transposed(mine + slot(ln + 4 * h, ch) + (l & 1) * 8);
-            f[t] = u.v;
-          }
-        } else {
-#pragma unroll
-          for (int t = 0; t < RT; ++t) f[t] = fa[set][s][t];
-        }
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) acc[t][c] = T::mma(f[t], fx[set][s][c], acc[t][c]);
-      }
+      for (int s = 0; s < S; ++s) load((turn * S + s) * 32, fx[set][s], fa[set][s], Whole{});
     };
-    int k0 = w * 32 * S;
-    if (k0 < g.k) load(k0, 0);
-    for (; k0 < g.k; k0 += 2 * turn) {
-      if (k0 + turn < g.k) load(k0 + turn, 1);
-      multiply(0);
-      if (k0 + turn >= g.k) break;
-      if (k0 + 2 * turn < g.k) load(k0 + 2 * turn, 0);
-      multiply(1);
+    auto multiply_turn = [&](int set) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) multiply(fx[set][s], fa[set][s]);
+    };
+    const int turns = g.k / (32 * S);
+    int at = w;
+    if (at < turns) load_turn(at, 0);
+    for (; at < turns; at += 2 * kProjWaves) {
+      if (at + kProjWaves < turns) load_turn(at + kProjWaves, 1);
+      multiply_turn(0);
+      if (at + kProjWaves >= turns) break;
+      if (at + 2 * kProjWaves < turns) load_turn(at + 2 * kProjWaves, 0);
+      multiply_turn(1);
+    }
+    if ((turns * S + w) * 32 < g.k) {
+      load((turns * S + w) * 32, fx[0][0], fa[0][0], Rest{});
+      multiply(fx[0][0], fa[0][0]);
     }
     if constexpr (FORM == A_R) __syncthreads();              // (the same LDS; `live` is the workgroup's)
 #pragma unroll
@@ -123,12 +138,12 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
       for (int c = 0; c < 2; ++c) red[w][t][c][l] = acc[t][c];
   }
   __syncthreads();
-  for (int q = threadIdx.x; q < RT * 2 * 64; q += 512) {
+  for (int q = threadIdx.x; q < RT * 2 * 64; q += kProjWaves * 64) {
     const int t = q / 128, c = (q / 64) % 2, at = piece.begin + c * 16 + (l & 15);
     if (at >= piece.end) continue;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     if (live)
-      for (int z = 0; z < 8; ++z) sum += red[z][t][c][l];
+      for (int z = 0; z < kProjWaves; ++z) sum += red[z][t][c][l];
     const int r = r0 + t * 16 + (l / 16) * 4;
     float* out = g.p + (int64_t)g.order[at] * g.ldp + r;
     for (int e = 0; e < 4; ++e)
