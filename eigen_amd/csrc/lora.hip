@@ -81,26 +81,33 @@ __global__ __launch_bounds__(512) void lora_plan_kernel(const int* __restrict__ 
   }
 }
 
+// The workgroups of a piece, 16 RT ranks each, run side by side on one XCD (consecutive ones go round the XCDs), where X is then
+// read from memory once.
 template <typename T, int RT, int FORM> __global__ __launch_bounds__(kProjWaves * 64) void lora_project_kernel(ProjectArgs g) {
-  __shared__ __align__(1024) char lds[project_lds(RT)];
-  project_piece<T, RT, FORM>(g, blockIdx.x, blockIdx.y * 16 * RT, lds);
+  __shared__ __align__(1024) char lds[project_lds(RT, T::bytes)];
+  const int across = (g.rank + 16 * RT - 1) / (16 * RT), at = blockIdx.x / 8;
+  project_piece<T, RT, FORM>(g, at / across * 8 + blockIdx.x % 8, at % across * 16 * RT, lds);
 }
 template <typename T, int RT> hipError_t launch_project_rank(const ProjectArgs& g, hipStream_t s) {
-  const dim3 grid((unsigned)project_slots(g), (g.rank + 16 * RT - 1) / (16 * RT));
+  const dim3 grid((unsigned)((project_slots(g) + 7) / 8 * 8 * ((g.rank + 16 * RT - 1) / (16 * RT)))), block(kProjWaves * 64);
   switch (project_form<T>(g)) {
-    case A_K: hipLaunchKernelGGL((lora_project_kernel<T, RT, A_K>), grid, dim3(kProjWaves * 64), 0, s, g); break;
+    case A_K: hipLaunchKernelGGL((lora_project_kernel<T, RT, A_K>), grid, block, 0, s, g); break;
     case A_R:
-      if constexpr (T::bytes == 2) hipLaunchKernelGGL((lora_project_kernel<T, RT, A_R>), grid, dim3(kProjWaves * 64), 0, s, g);
+      if constexpr (T::bytes == 2) hipLaunchKernelGGL((lora_project_kernel<T, RT, A_R>), grid, block, 0, s, g);
       break;
-    default: hipLaunchKernelGGL((lora_project_kernel<T, RT, A_ANY>), grid, dim3(kProjWaves * 64), 0, s, g);
+    default: hipLaunchKernelGGL((lora_project_kernel<T, RT, A_ANY>), grid, block, 0, s, g);
   }
   return hipGetLastError();
 }
-// Few pieces: 16 ranks a workgroup, so that there are more of them (142 tokens x 4032, rank 64: 25 -> 15 us); many: X is read once.
+// 16, 32 or 64 ranks a workgroup: they take about 9.5, 13 and 15 us with 4032 positions, as long as there are at most 256 of them, and
+// in proportion to their number beyond (rank 64, 3589 tokens: 16.2, 13.4, 15.5 us; 8192 tokens: 22.8, 23.9, 16.3; 142: 9.4, 12.8,
+// 14.2).
 template <typename T> hipError_t launch_project(const ProjectArgs& g, hipStream_t s) {
-  if (g.rank <= 16 || project_slots(g) * ((g.rank + 15) / 16) <= 512) return launch_project_rank<T, 1>(g, s);
-  if (g.rank <= 32) return launch_project_rank<T, 2>(g, s);
-  return launch_project_rank<T, 4>(g, s);
+  const double pieces = g.n / kProjTokens + (g.none + 1) * 0.5;      // an adapter's last piece is there or not
+  auto cost = [&](int rt, double us) { return std::max(1.0, pieces * ((g.rank + 16 * rt - 1) / (16 * rt)) / 256.0) * us; };
+  const double one = cost(1, 9.5), two = cost(2, 13.0), four = cost(4, 15.0);
+  if (one <= two && one <= four) return launch_project_rank<T, 1>(g, s);
+  return two <= four ? launch_project_rank<T, 2>(g, s) : launch_project_rank<T, 4>(g, s);
 }
 
 // Y += s_j op(B_j) P in single precision, behind the plain product: a wave takes 16 rows of 16 columns, so that there are many of

@@ -24,7 +24,10 @@ namespace {
 template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512) void lora_few_kernel(HalfGemm g, ProjectArgs q, int project, int slots) {
   using E = typename T::elem;
   using x8 = typename T::x8;
-  constexpr int red_bytes = 8 * 4 * NG * 64 * 16, lds_bytes = red_bytes > project_lds(1) ? red_bytes : project_lds(1);
+  using Block = RowBlock<T>;
+  constexpr int red_bytes = 8 * 4 * NG * 64 * 16, blocks_bytes = 8 * (4 + NG) * Block::bytes;
+  constexpr int loop_bytes = blocks_bytes > project_lds(1, T::bytes) ? blocks_bytes : project_lds(1, T::bytes);
+  constexpr int lds_bytes = red_bytes > loop_bytes ? red_bytes : loop_bytes;
   __shared__ __align__(1024) char lds[lds_bytes];
   if ((int)blockIdx.x < project) {
     project_piece<T, 1, FORM>(q, blockIdx.x % slots, blockIdx.x / slots * 16, lds);
@@ -39,7 +42,7 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     if constexpr (LA == KC) {
-      const int row = row0 + t * 16 + (l & 15);
+      const int row = row0 + t * 16 + Block::row();
       a[t] = static_cast<const E*>(g.a) + (int64_t)(row < g.m ? row : g.m - 1) * g.lda;
     } else {
       const int row = row0 + (l % 8) * 8;
@@ -48,16 +51,16 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
   }
 #pragma unroll
   for (int c = 0; c < NG; ++c) {
-    const int at = c * 16 + (l & 15);
+    const int at = c * 16 + Block::row();
     b[c] = static_cast<const E*>(g.b) + (int64_t)g.order[at < g.n ? at : g.n - 1] * g.ldb;
   }
   f32x4 acc[4][NG] = {};
   // whole turns, then what is left, one product a wave (as in project_piece)
-  constexpr int S = NG == 4 || T::bytes == 4 ? 1 : NG == 2 || LA == MC ? 2 : 4;
+  constexpr int S = NG == 4 || T::bytes == 4 ? 1 : 2;
   using Whole = std::true_type;
   using Rest = std::false_type;
   auto load = [&](int k0, x8(&fa)[4], x8(&fb)[NG], auto whole) {
-    const int k = k0 + (l / 16) * 8, left = k_end - k;
+    const int k = k0 + Block::position(), left = k_end - k;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if constexpr (LA == KC) {
@@ -74,10 +77,12 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
     for (int c = 0; c < NG; ++c) fb[c] = whole ? load_8<E, x8>(b[c] + k) : load_first<E, x8>(b[c] + (left > 0 ? k : 0), 1, left);
   };
   auto multiply = [&](const x8(&fa)[4], const x8(&fb)[NG]) {
-    x8 f[4];
+    x8 f[4], y[NG];
+    char* mine = lds + w * (4 + NG) * Block::bytes;
+#pragma unroll
+    for (int c = 0; c < NG; ++c) Block::put(mine + (4 + c) * Block::bytes, fb[c]);
     if constexpr (LA == MC) {
       // lines of 64 rows, 128 bytes; chunks permuted so that the 8 lines a half wave reads meet all banks once
-      char* mine = lds + w * 4096;
       auto slot = [](int line, int ch) { return line * 128 + (ch ^ (((line >> 1) & 1) | ((line >> 2) & 2)) << 1) * 16; };
 #pragma unroll
       for (int t = 0; t < 4; ++t) *reinterpret_cast<x8*>(mine + slot(t * 8 + l / 8, l % 8)) = fa[t];
@@ -91,12 +96,16 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
       }
     } else {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) f[t] = fa[t];
+      for (int t = 0; t < 4; ++t) Block::put(mine + t * Block::bytes, fa[t]);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) f[t] = Block::get(mine + t * Block::bytes);
     }
+#pragma unroll
+    for (int c = 0; c < NG; ++c) y[c] = Block::get(mine + (4 + c) * Block::bytes);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int c = 0; c < NG; ++c) acc[t][c] = T::mma(f[t], fb[c], acc[t][c]);
+      for (int c = 0; c < NG; ++c) acc[t][c] = T::mma(f[t], y[c], acc[t][c]);
   };
   x8 fa[2][S][4], fb[2][S][NG];
   auto load_turn = [&](int turn, int set) {
@@ -121,7 +130,7 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
     load(k0, fa[0][0], fb[0][0], Rest{});
     multiply(fa[0][0], fb[0][0]);
   }
-  if constexpr (LA == MC) __syncthreads();
+  __syncthreads();
   f32x4(&red)[8][4][NG][64] = *reinterpret_cast<f32x4(*)[8][4][NG][64]>(lds);
 #pragma unroll
   for (int t = 0; t < 4; ++t)

@@ -16,16 +16,47 @@ struct ProjectArgs {
   float* p; int64_t ldp;
 };
 
-// P for up to 32 tokens of one adapter and 16 RT ranks.  Eight waves share the reduction, 128 (down to 32) positions a turn, each straight
-// from memory to the matrix unit: one load of a wave is 64 bytes of each of 16 tokens.  The next turn's loads are under way
-// while this one's are multiplied.
+// 16 rows x 32 positions on their way from memory to the matrix unit.  A fragment has neighbouring lanes on different rows; loaded
+// so, a load takes the memory pipeline 64 cycles, a row's address at a time.  Here four neighbouring lanes take 64 bytes (128) of
+// one row, and the wave's own LDS turns them into fragments; chunks of a row are permuted so that the 16 lanes that read together meet
+// all banks once.
+template <typename T> struct RowBlock {
+  using x8 = typename T::x8;
+  static constexpr int bytes = 512 * T::bytes;
+  static __device__ __forceinline__ int row() { return (threadIdx.x & 63) / 4; }
+  static __device__ __forceinline__ int position() { return (threadIdx.x & 3) * 8; }
+  static __device__ __forceinline__ int at(int row, int chunk) {       // of 16 bytes
+    return T::bytes == 2 ? row * 64 + (chunk ^ ((row / 4) & 3)) * 16 : row * 128 + (chunk ^ ((row / 2) & 7)) * 16;
+  }
+  static __device__ __forceinline__ void put(char* lds, x8 v) {
+    const int l = threadIdx.x & 63;
+    constexpr int H = T::bytes / 2;
+    const Half<x8> u = __builtin_bit_cast(Half<x8>, v);
+#pragma unroll
+    for (int h = 0; h < H; ++h) *reinterpret_cast<f32x4*>(lds + at(l / 4, (l % 4) * H + h)) = u.part[h];
+  }
+  static __device__ __forceinline__ x8 get(const char* lds) {
+    const int l = threadIdx.x & 63;
+    constexpr int H = T::bytes / 2;
+    Half<x8> u;
+#pragma unroll
+    for (int h = 0; h < H; ++h) u.part[h] = *reinterpret_cast<const f32x4*>(lds + at(l % 16, (l / 16) * H + h));
+    return __builtin_bit_cast(x8, u);
+  }
+
+ private:
+  template <typename V> struct Half { f32x4 part[sizeof(V) / 16]; };
+};
+
+// P for up to 32 tokens of one adapter and 16 RT ranks.  Eight waves share the reduction, 128 (down to 32) positions a turn.  The next
+// turn's loads are under way while this one's are multiplied.
 //   A_K   the factor's reduction is contiguous: loaded like the tokens
 //   A_R   its ranks are (the backward pass): whole 16-byte chunks of ranks go through this wave's own LDS and come back
 //         transposed; one element at a time instead, the loads of a 64-rank factor took four times the rest (57 us of 4096 tokens
 //         x 4096, now 18)
 //   A_ANY element by element: ranks that are no multiple of 8, odd strides
 enum { A_K, A_R, A_ANY };
-constexpr int project_lds(int rt) { return kProjWaves * rt * 2 * 64 * 16; }
+constexpr int project_lds(int rt, int bytes) { return kProjWaves * (rt * 2048 > (2 + rt) * 512 * bytes ? rt * 2048 : (2 + rt) * 512 * bytes); }
 template <typename T, int RT, int FORM> __device__ __forceinline__ void project_piece(const ProjectArgs& g, int slot_id, int r0, char* lds) {
   using E = typename T::elem;
   using x8 = typename T::x8;
@@ -33,7 +64,6 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
   if (!find_piece(g.starts, g.none + 1, kProjTokens, slot_id, piece)) return;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63;
   constexpr int line = RT * 32;                      // A_R: 32 positions x 16 RT ranks per wave
-  static_assert(kProjWaves * 32 * line <= project_lds(RT), "transposition and sums share LDS");
   f32x4(&red)[kProjWaves][RT][2][64] = *reinterpret_cast<f32x4(*)[kProjWaves][RT][2][64]>(lds);
   const bool live = piece.adapter != g.none;
   if (live) {
@@ -44,7 +74,7 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
     const E* factor = static_cast<const E*>(g.a) + (int64_t)piece.adapter * g.a_stride;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const int at = piece.begin + c * 16 + (l & 15);
+      const int at = piece.begin + c * 16 + RowBlock<T>::row();
       x[c] = static_cast<const E*>(g.x) + (int64_t)g.order[at < piece.end ? at : piece.end - 1] * g.ldx;
     }
     constexpr int per = RT * 2;                              // A_R: 16-byte chunks of a line
@@ -55,7 +85,7 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
         const int ch = t * 64 + l, r = r0 + (ch % per) * 8;
         a[t] = factor + (int64_t)(ch / per) * g.a_k + (r < g.rank ? r : 0);
       } else {
-        const int r = r0 + t * 16 + (l & 15);
+        const int r = r0 + t * 16 + (FORM == A_K ? RowBlock<T>::row() : l & 15);
         a[t] = factor + (int64_t)(r < g.rank ? r : g.rank - 1) * g.a_row;
       }
     }
@@ -66,7 +96,7 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
     using Whole = std::true_type;
     using Rest = std::false_type;
     auto load = [&](int k0, x8(&fx)[2], x8(&fa)[RT], auto whole) {
-      const int k = k0 + (l / 16) * 8, left = g.k - k;
+      int k = k0 + RowBlock<T>::position(), left = g.k - k;
 #pragma unroll
       for (int c = 0; c < 2; ++c) fx[c] = whole ? load_8<E, x8>(x[c] + k) : load_first<E, x8>(x[c] + (left > 0 ? k : 0), 1, left);
 #pragma unroll
@@ -80,33 +110,47 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
         } else if constexpr (FORM == A_K && whole) {
           fa[t] = load_8<E, x8>(a[t] + k);
         } else {
+          if constexpr (FORM == A_ANY) {
+            k = k0 + (l / 16) * 8;
+            left = g.k - k;
+          }
           fa[t] = load_first<E, x8>(a[t] + (left > 0 ? (int64_t)k * g.a_k : 0), g.a_k, whole ? 8 : left);
         }
       }
     };
     auto multiply = [&](const x8(&fx)[2], const x8(&fa)[RT]) {
-      x8 f[RT];
+      char* mine = lds + w * (2 + RT) * RowBlock<T>::bytes;      // X's two blocks, then the factor's
+      x8 f[RT], y[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) RowBlock<T>::put(mine + c * RowBlock<T>::bytes, fx[c]);
+      char* own = mine + 2 * RowBlock<T>::bytes;
       if constexpr (FORM == A_R) {
-        char* mine = lds + w * 32 * line;
         auto slot = [&](int ln, int ch) { return ln * line + ((ch ^ ((ln & 3) << 1)) & (per - 1)) * 16; };
 #pragma unroll
-        for (int t = 0; t < RT; ++t) *reinterpret_cast<x8*>(mine + slot((t * 64 + l) / per, (t * 64 + l) % per)) = fa[t];
+        for (int t = 0; t < RT; ++t) *reinterpret_cast<x8*>(own + slot((t * 64 + l) / per, (t * 64 + l) % per)) = fa[t];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
           union { x8 v; typename T::x4 h[2]; } u;
           const int ln = (l / 16) * 8 + (l & 15) / 4, ch = t * 2 + (l & 3) / 2;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) u.h[h] = T::read_transposed(mine + slot(ln + 4 * h, ch) + (l & 1) * 8);
+          for (int h = 0; h < 2; ++h) u.h[h] = T::read_transposed(own + slot(ln + 4 * h, ch) + (l & 1) * 8);
           f[t] = u.v;
         }
+      } else if constexpr (FORM == A_K) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) RowBlock<T>::put(own + t * RowBlock<T>::bytes, fa[t]);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) f[t] = RowBlock<T>::get(own + t * RowBlock<T>::bytes);
       } else {
 #pragma unroll
         for (int t = 0; t < RT; ++t) f[t] = fa[t];
       }
 #pragma unroll
+      for (int c = 0; c < 2; ++c) y[c] = RowBlock<T>::get(mine + c * RowBlock<T>::bytes);
+#pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) acc[t][c] = T::mma(f[t], fx[c], acc[t][c]);
+        for (int c = 0; c < 2; ++c) acc[t][c] = T::mma(f[t], y[c], acc[t][c]);
     };
     x8 fx[2][S][2], fa[2][S][RT];
     auto load_turn = [&](int turn, int set) {
@@ -131,7 +175,7 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
       load((turns * S + w) * 32, fx[0][0], fa[0][0], Rest{});
       multiply(fx[0][0], fa[0][0]);
     }
-    if constexpr (FORM == A_R) __syncthreads();              // (the same LDS; `live` is the workgroup's)
+    __syncthreads();              // (the sums take the same LDS; `live` is the workgroup's)
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
