@@ -624,10 +624,11 @@ enum { TILE_256, TILE_128, TILE_128_ALONE };
 struct TilePlan {
   int tile, splits;
   int64_t k_piece;
+  double us;
 };
 inline TilePlan plan_tiles(int64_t m, int64_t n, int64_t k) {
   const int64_t t128 = ((m + 127) / 128) * ((n + 127) / 128), t256 = ((m + 255) / 256) * ((n + 255) / 256);
-  TilePlan plan = {TILE_128_ALONE, 1, 64};
+  TilePlan plan = {TILE_128_ALONE, 1, 64, 0.0};
   double best = 1e30;
   for (int64_t s = 1; s <= 32 && (s == 1 || (k / s >= 128 && s * t256 <= 512)); ++s) {
     const int64_t piece = k > 0 ? ((k + s - 1) / s + 63) / 64 * 64 : 64;
@@ -642,7 +643,7 @@ inline TilePlan plan_tiles(int64_t m, int64_t n, int64_t k) {
     for (int t = 0; t < 3; ++t)
       if (cost[t] + join < (s > 1 ? 0.92 : 0.999) * best) {      // a further piece has to win clearly
         best = cost[t] + join;
-        plan = {t, (int)(k > 0 ? (k + piece - 1) / piece : 1), piece};
+        plan = {t, (int)(k > 0 ? (k + piece - 1) / piece : 1), piece, best};
       }
   }
   return plan;

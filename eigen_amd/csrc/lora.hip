@@ -16,7 +16,7 @@
 namespace eigamd {
 
 // lora_few.hip
-bool lora_few(int64_t n);
+bool lora_few(bool f32, int64_t m, int64_t n, int64_t k);
 int64_t lora_few_work_bytes(int64_t m, int64_t n, int64_t k);
 hipError_t lora_few_device(int kind, bool w_trans, const HalfGemm& g, const ProjectArgs& q, hipStream_t s);
 
@@ -143,7 +143,7 @@ struct HalfWork {
 HalfWork half_work(bool w_trans, int64_t m, int64_t n, int64_t k, const void* w, int64_t ldw, const void* x, int64_t ldx) {
   HalfWork need = {0, 0, 0};
   const bool w_whole = whole_chunks(w, ldw, w_trans ? k : m);
-  if (lora_few(n)) {
+  if (lora_few(false, m, n, k)) {
     need.sums = lora_few_work_bytes(m, n, k);      // (W's reduction contiguous: read where it is, whatever its alignment)
     if (!w_trans && !w_whole) need.w_copy = padded_bytes(m, k);
   } else {
@@ -175,7 +175,7 @@ HalfGemm gemm_args(const LoraArgs& c) {
   return g;
 }
 // Single precision has the few-token form for W with a contiguous reduction (there is no transposing read of 32-bit elements).
-bool few_f32(bool w_trans, int64_t n) { return w_trans && lora_few(n); }
+bool few_f32(bool w_trans, int64_t m, int64_t n, int64_t k) { return w_trans && lora_few(true, m, n, k); }
 
 template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArgs& q, hipStream_t s) {
   HalfGemm g = gemm_args(c);
@@ -195,7 +195,7 @@ template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArg
   }
   hipError_t e = launch_pad_copy(w_copy, x_copy, s);
   if (e != hipSuccess) return e;
-  if (lora_few(c.n)) return lora_few_device(c.kind, c.w_trans, g, q, s);
+  if (lora_few(false, c.m, c.n, c.k)) return lora_few_device(c.kind, c.w_trans, g, q, s);
   if (q.none > 0 && (e = launch_project<T>(q, s)) != hipSuccess) return e;
   const TilePlan plan = plan_tiles(c.m, c.n, c.k);
   g.splits = plan.splits;
@@ -432,7 +432,7 @@ hipError_t lora_plan_device(const int* ids, int64_t n, int64_t adapters, int* d_
 
 int64_t lora_work_bytes(int kind, bool w_trans, int64_t m, int64_t n, int64_t k, const void* w, int64_t ldw, const void* x, int64_t ldx) {
   if (m <= 0 || n <= 0) return 0;
-  if (kind == F32) return few_f32(w_trans, n) ? lora_few_work_bytes(m, n, k) : std::min<int64_t>(16 * m * n * 4, (int64_t)256 << 20);
+  if (kind == F32) return few_f32(w_trans, m, n, k) ? lora_few_work_bytes(m, n, k) : std::min<int64_t>(16 * m * n * 4, (int64_t)256 << 20);
   const HalfWork need = half_work(w_trans, m, n, k, w, ldw, x, ldx);
   return need.sums + need.w_copy + need.x_copy;
 }
@@ -447,7 +447,7 @@ hipError_t lora_device(const LoraArgs& c, hipStream_t s) {
   p.a_stride = c.stride_a;
   p.order = c.plan.order; p.starts = c.plan.starts;
   p.p = c.p; p.ldp = c.ldp;
-  if (c.m > 0 && c.kind == F32 && few_f32(c.w_trans, c.n)) {
+  if (c.m > 0 && c.kind == F32 && few_f32(c.w_trans, c.m, c.n, c.k)) {
     HalfGemm g = gemm_args(c);
     g.partial = static_cast<float*>(c.work);
     return lora_few_device(F32, true, g, p, s);

@@ -14,7 +14,7 @@ hipError_t lora_project_device(int kind, const ProjectArgs& g, hipStream_t s);  
 
 namespace {
 
-// Y for at most 64 tokens (16 NG of them): the time is that of reading W once, from as many compute units as there are.  A
+// Y for few tokens, 16 NG of them a workgroup: the time is that of reading W, from as many compute units as there are.  A
 // workgroup owns 64 rows and one piece of the reduction, so that X, which every workgroup reads its piece of, costs little beside
 // W (with 16 rows and the whole reduction X was four times the traffic: 64 tokens x 4096 x 4096 took 22 us, now 12).  Its eight
 // waves share the piece, 64 (32) positions a turn, from memory to the matrix unit directly (W's reduction contiguous) or through the
@@ -33,8 +33,10 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
     project_piece<T, 1, FORM>(q, blockIdx.x % slots, blockIdx.x / slots * 16, lds);
     return;
   }
-  const int id = blockIdx.x - project, row_blocks = (g.m + 63) / 64;
-  const int row0 = id % row_blocks * 64, z = id / row_blocks;
+  const int id = blockIdx.x - project, row_blocks = (g.m + 63) / 64, groups = (g.n + 63) / 64;
+  const int part = id / 8 / groups * 8 + id % 8, col0 = id / 8 % groups * 64;
+  if (part >= row_blocks * g.splits) return;
+  const int row0 = part % row_blocks * 64, z = part / row_blocks;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63;
   const int k_begin = z * g.k_piece, k_end = k_begin + g.k_piece < g.k ? k_begin + g.k_piece : g.k;
   const E* a[4];                      // KC: rows of the four row blocks; MC: chunks of 8 lines
@@ -51,7 +53,7 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
   }
 #pragma unroll
   for (int c = 0; c < NG; ++c) {
-    const int at = c * 16 + Block::row();
+    const int at = col0 + c * 16 + Block::row();
     b[c] = static_cast<const E*>(g.b) + (int64_t)g.order[at < g.n ? at : g.n - 1] * g.ldb;
   }
   f32x4 acc[4][NG] = {};
@@ -141,11 +143,11 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
 #pragma unroll
   for (int v = threadIdx.x; v < 4 * NG * 64; v += 512) {
     // 16 neighbouring threads hold the 64 rows of a column
-    const int part = v % 16, col = v / 16, t = part / 4;
+    const int quad = v % 16, in = v / 16, col = col0 + in, t = quad / 4;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int y = 0; y < 8; ++y) sum += red[y][t][col / 16][(part % 4) * 16 + col % 16];
-    const int row = row0 + part * 4;
+    for (int y = 0; y < 8; ++y) sum += red[y][t][in / 16][(quad % 4) * 16 + in % 16];
+    const int row = row0 + quad * 4;
     if (col >= g.n) continue;
     float* at = out + (int64_t)col * g.m + row;
     if (g.m % 4 == 0 && row < g.m) *reinterpret_cast<f32x4*>(at) = sum;
@@ -192,15 +194,15 @@ template <typename T> __global__ __launch_bounds__(256) void lora_few_join_kerne
   static_cast<E*>(g.c)[token * g.ldc + row] = (E)sum;
 }
 
-// At most 64 tokens: pieces of the reduction, none shorter than 512 (eight waves, 64 positions each), at most 512 workgroups.
+// Pieces of the reduction, none shorter than 512 (eight waves, 64 positions each), at most 512 workgroups.
 bool piece_allowed(int64_t blocks, int64_t k, int64_t pieces) {
   return pieces == 1 || (pieces <= 16 && k / pieces >= 512 && blocks * pieces <= 512);
 }
 // A compute unit runs one of these workgroups at a time, so the 64-row blocks times the pieces and the projection's workgroups
 // should fill whole rounds of 256; a round costs what its piece does plus the latencies at both ends, about as much as 600
 // positions (64 tokens x 4096 x 4096: 512 workgroups 16.8 us, 256 12.6).
-int few_pieces(int64_t m, int64_t k, int64_t project, int64_t* k_piece) {
-  const int64_t blocks = (m + 63) / 64;
+int few_pieces(int64_t m, int64_t n, int64_t k, int64_t project, int64_t* k_piece) {
+  const int64_t blocks = (m + 63) / 64 * ((n + 63) / 64);
   int64_t best = 1, best_cost = INT64_MAX;
   for (int64_t pieces = 1; piece_allowed(blocks, k, pieces); ++pieces) {
     const int64_t piece = (k + pieces - 1) / pieces, cost = (blocks * pieces + project + 255) / 256 * (piece + 600);
@@ -211,7 +213,7 @@ int few_pieces(int64_t m, int64_t k, int64_t project, int64_t* k_piece) {
 }
 template <typename T, int LA, int NG> hipError_t launch_few_tokens(const HalfGemm& g, const ProjectArgs& q, int form, hipStream_t s) {
   const int slots = q.none && form != A_ANY ? (int)project_slots(q) : 0, project = slots * ((q.rank + 15) / 16);
-  const dim3 grid((unsigned)(project + (g.m + 63) / 64 * g.splits));
+  const dim3 grid((unsigned)(project + ((g.m + 63) / 64 * g.splits + 7) / 8 * 8 * ((g.n + 63) / 64)));
   if constexpr (T::bytes == 2) {
     if (form == A_R) hipLaunchKernelGGL((lora_few_kernel<T, LA, NG, A_R>), grid, dim3(512), 0, s, g, q, project, slots);
   }
@@ -229,7 +231,7 @@ template <typename T, int LA> hipError_t launch_few(HalfGemm g, const ProjectArg
     if (e != hipSuccess) return e;
   }
   int64_t piece;
-  g.splits = few_pieces(g.m, g.k, q.none && form != A_ANY ? project_slots(q) * ((q.rank + 15) / 16) : 0, &piece);
+  g.splits = few_pieces(g.m, g.n, g.k, q.none && form != A_ANY ? project_slots(q) * ((q.rank + 15) / 16) : 0, &piece);
   g.k_piece = (int)piece;
   return g.n <= 16 ? launch_few_tokens<T, LA, 1>(g, q, form, s) : g.n <= 32 ? launch_few_tokens<T, LA, 2>(g, q, form, s)
                                                                          : launch_few_tokens<T, LA, 4>(g, q, form, s);
@@ -237,10 +239,23 @@ template <typename T, int LA> hipError_t launch_few(HalfGemm g, const ProjectArg
 
 }  // namespace
 
-bool lora_few(int64_t n) { return n <= 64; }
+// Up to 64 tokens, and beyond as long as this is one round and quicker than large tiles with the projection in front of them: 3 us,
+// and 5 + 4.4 per thousand positions a round, against the plan's time, 6 us and 1.25 per thousand positions for the projection
+// (256 tokens x 1024 x 1024 18.7 -> 10.4 us, 142 x 2456 x 4032 29.6 -> 17.9, 192 x 4096 x 4096 31.5 -> 27.0; not 96 x 4096 x 16384,
+// 62.5 -> 69.2).  Single precision: against the library's product, which has larger tiles still, up to two rounds (777 x 1024 x
+// 1536 72.6 -> 45.9 us, 1500 x 1000 x 2000 114 -> 108, 2048 x 2048 x 2048 180 -> 214).
+bool lora_few(bool f32, int64_t m, int64_t n, int64_t k) {
+  if (n <= 64) return true;
+  const int64_t blocks = (m + 63) / 64 * ((n + 63) / 64), project = n / kProjTokens;
+  if (f32) return blocks <= 512;
+  if (blocks + project > 256) return false;
+  int64_t piece;
+  const int64_t pieces = few_pieces(m, n, k, project, &piece), rounds = (blocks * pieces + project + 255) / 256;
+  return 3.0 + (double)rounds * (5.0 + 4.4e-3 * (double)piece) < plan_tiles(m, n, k).us + 6.0 + 1.25e-3 * (double)k;
+}
 int64_t lora_few_work_bytes(int64_t m, int64_t n, int64_t k) {
   int64_t pieces = 1;
-  while (piece_allowed((m + 63) / 64, k, pieces + 1)) ++pieces;
+  while (piece_allowed((m + 63) / 64 * ((n + 63) / 64), k, pieces + 1)) ++pieces;
   return pieces * m * n * 4;
 }
 

@@ -118,6 +118,22 @@ def test_lora_large_tiles(kind, opw):
     Case(kind, 256 * 15 + 8, 256 * 14 + 37, 200, 16, 6, opw + "TT").run().check()
 
 
+@pytest.mark.parametrize("kind", [BF16, F16], ids=NAME.get)
+@pytest.mark.parametrize("ops", ["TTT", "NTT", "TNN", "NNN"])
+@pytest.mark.parametrize("m, n, k, rank", [(1100, 1130, 200, 40), (1101, 1130, 203, 7), (1096, 1130, 1288, 16), (2200, 2300, 264, 24), (1, 9000, 64, 3)])
+def test_lora_small_tiles(kind, ops, m, n, k, rank):
+    # tiles of 128 x 128, one or two to a compute unit, whole and split reductions, extents that are copied first
+    Case(kind, m, n, k, rank, 5, ops).run().check()
+
+
+@pytest.mark.parametrize("opw, ld", [("T", 2 ** 23 + 8), ("N", 2 ** 25 + 8)])
+def test_a_leading_dimension_of_several_gigabytes_a_tile(opw, ld):
+    # one tile's rows (lines) span more than 2^32 bytes
+    c = Case(BF16, 260, 4100, 72, 16, 3, opw + "TT")
+    c.W = store(turned(c.w, opw), BF16, ld - c.W.rows)
+    c.run().check()
+
+
 @pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
 @pytest.mark.parametrize("n", [5, 130])
 def test_lora_who_has_an_adapter(kind, n):
@@ -352,7 +368,7 @@ def test_pack_of_a_packed_matrix_changes_nothing(kind):
     assert float((once.as_strided().double() - x).abs().max()) <= float(step) / 2
 
 
-def run_wgrad(kind, m, n, k, opw, beta, pad=0, shift=0, seed=21):
+def run_wgrad(kind, m, n, k, opw, beta, pad=0, shift=0, seed=21, dy_pad=None):
     dy, x = rand((m, n), kind, seed, 0.1), rand((k, n), kind, seed + 1)
     X, c = store(x, kind), lowrank.Checkpoint8(k, n, kind, ld=max(k + pad, 1), lde=(k + 31) // 32 + pad)
     lowrank.ckpt8_pack_dev(X, c)
@@ -361,7 +377,7 @@ def run_wgrad(kind, m, n, k, opw, beta, pad=0, shift=0, seed=21):
     kept = back.as_strided().double()
     old = rand((m, k), F32, seed + 2)
     dw = store(turned(old if beta else torch.full_like(old, float("nan")), opw), F32, pad)
-    lowrank.ckpt8_wgrad_dev(opw, store(dy, kind, pad, shift), c, beta, dw)
+    lowrank.ckpt8_wgrad_dev(opw, store(dy, kind, pad if dy_pad is None else dy_pad, shift), c, beta, dw)
     dyd = dy.cuda()
     want = dyd @ kept.t().contiguous()
     mag = dyd.abs() @ kept.abs().t().contiguous()
@@ -390,6 +406,17 @@ def test_ckpt8_wgrad_leading_dimensions_and_alignment(kind, pad, shift):
 @pytest.mark.parametrize("opw", "NT")
 def test_ckpt8_wgrad_large_tiles(kind, opw):
     run_wgrad(kind, 256 * 14 + 40, 130, 256 * 15 + 8, opw, 1.0)
+
+
+@pytest.mark.parametrize("kind", [BF16, F16], ids=NAME.get)
+@pytest.mark.parametrize("opw", "NT")
+def test_ckpt8_wgrad_small_tiles(kind, opw):
+    run_wgrad(kind, 2300, 264, 2200, opw, 1.0)
+    run_wgrad(kind, 1100, 1300, 1130, opw, 0.0)
+
+
+def test_ckpt8_wgrad_with_a_leading_dimension_of_several_gigabytes_a_tile():
+    run_wgrad(BF16, 136, 72, 264, "N", 1.0, dy_pad=2 ** 25 + 8 - 136)
 
 
 # -------------------------------------------------------------------------------------------------- all of them, as they are used
