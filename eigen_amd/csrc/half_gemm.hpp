@@ -503,34 +503,47 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void half_gemm_kernel(HalfGemm g) 
       }
     return;
   }
+  // Otherwise through LDS again.  What C held is loaded a step ahead of the stores; behind them every step waits for memory (589
+  // tokens x 2840 x 3774: 68 us, now 42).
   constexpr int line = CR * 4 + 16;
   static_assert(16 * line * WM * WN <= D * slice, "the epilogue's part of LDS");
   char* mine = lds + w * 16 * line;
+  constexpr int B = 8, NB = 16 * CR / 64 / B;      // values a lane takes in one step, steps of 16 columns
+  static_assert(16 * CR / 64 % B == 0, "whole steps");
+  float next[B] = {};
+  auto place = [&](int step, int t) -> float* {
+    const int q = (step % NB * B + t) * 64 + l, c = c_col0 + step / NB * 16 + q / CR, r = c_row0 + q % CR;
+    return c < c_cols && r < c_rows ? C + (int64_t)c * ldc + r : nullptr;
+  };
+  auto fetch = [&](int step) {
+#pragma unroll
+    for (int t = 0; t < B; ++t) {
+      const float* at = place(step, t);
+      next[t] = *(at ? at : reinterpret_cast<const float*>(zero_page));
+    }
+  };
+  if (beta != 0.0f) fetch(0);
 #pragma unroll
   for (int j = 0; j < CN; ++j) {
 #pragma unroll
     for (int i = 0; i < CR / 16; ++i) *reinterpret_cast<f32x4*>(mine + (l & 15) * line + (i * 16 + (l / 16) * 4) * 4) = block(i, j);
     __builtin_amdgcn_wave_barrier();
-    constexpr int B = 8;      // old values of this many rows under way together
-    static_assert(16 * CR / 64 % B == 0, "whole batches");
 #pragma unroll 1
-    for (int q0 = 0; q0 < 16 * CR / 64; q0 += B) {
-      float v[B], old[B];
-      float* at[B];
+    for (int b = 0; b < NB; ++b) {
+      const int step = j * NB + b;
+      float v[B];
 #pragma unroll
       for (int t = 0; t < B; ++t) {
-        const int q = (q0 + t) * 64 + l, c = c_col0 + j * 16 + q / CR, r = c_row0 + q % CR;
+        const int q = (b * B + t) * 64 + l;
         v[t] = *reinterpret_cast<const float*>(mine + q / CR * line + q % CR * 4);
-        at[t] = c < c_cols && r < c_rows ? C + (int64_t)c * ldc + r : nullptr;
-        old[t] = 0.0f;
+        v[t] += beta != 0.0f ? beta * next[t] : 0.0f;
       }
-      if (beta != 0.0f) {
+      if (beta != 0.0f && step + 1 < CN * NB) fetch(step + 1);
 #pragma unroll
-        for (int t = 0; t < B; ++t) old[t] = at[t] ? beta * *at[t] : 0.0f;
+      for (int t = 0; t < B; ++t) {
+        float* at = place(step, t);
+        if (at) *at = v[t];
       }
-#pragma unroll
-      for (int t = 0; t < B; ++t)
-        if (at[t]) *at[t] = v[t] + old[t];
     }
     __builtin_amdgcn_wave_barrier();
   }

@@ -126,6 +126,13 @@ def test_lora_small_tiles(kind, ops, m, n, k, rank):
     Case(kind, m, n, k, rank, 5, ops).run().check()
 
 
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("ops", ["TTT", "NNN"])
+@pytest.mark.parametrize("m, n, k, rank", [(1601, 130, 136, 100), (1600, 99, 520, 130)])
+def test_lora_few_tokens_and_large_ranks(kind, ops, m, n, k, rank):
+    Case(kind, m, n, k, rank, 9, ops).run().check()
+
+
 @pytest.mark.parametrize("opw, ld", [("T", 2 ** 23 + 8), ("N", 2 ** 25 + 8)])
 def test_a_leading_dimension_of_several_gigabytes_a_tile(opw, ld):
     # one tile's rows (lines) span more than 2^32 bytes
