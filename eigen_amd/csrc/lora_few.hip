@@ -10,8 +10,6 @@
 
 namespace eigamd {
 
-hipError_t lora_project_device(int kind, const ProjectArgs& g, hipStream_t s);   // lora.hip
-
 namespace {
 
 // Y for few tokens, 16 NG of them a workgroup: the time is that of reading W, from as many compute units as there are.  A
@@ -218,8 +216,13 @@ template <typename T> __global__ __launch_bounds__(256) void lora_few_tile_join_
   }
   sum += acc[0][0];
   E* at = static_cast<E*>(g.c) + (int64_t)g.order[col] * g.ldc + row;
-  for (int t = 0; t < 4; ++t)
-    if (row + t < g.m) at[t] = (E)sum[t];
+  using e4 = E __attribute__((ext_vector_type(4)));
+  if (wide && g.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(g.c) % sizeof(e4) == 0) {
+    *reinterpret_cast<e4*>(at) = __builtin_convertvector(sum, e4);
+  } else {
+    for (int t = 0; t < 4; ++t)
+      if (row + t < g.m) at[t] = (E)sum[t];
+  }
 }
 
 // Pieces of the reduction, none shorter than 512 (eight waves, 64 positions each), at most 512 workgroups.
@@ -239,13 +242,14 @@ int few_pieces(int64_t m, int64_t n, int64_t k, int64_t project, int64_t* k_piec
   *k_piece = std::max<int64_t>(((k + best - 1) / best + 63) / 64 * 64, 64);
   return (int)std::max<int64_t>((k + *k_piece - 1) / *k_piece, 1);
 }
-template <typename T, int LA, int NG> hipError_t launch_few_tokens(const HalfGemm& g, const ProjectArgs& q, int form, hipStream_t s) {
-  const int slots = q.none && form != A_ANY ? (int)project_slots(q) : 0, project = slots * ((q.rank + 15) / 16);
+template <typename T, int LA, int NG> hipError_t launch_few_tokens(const HalfGemm& g, const ProjectArgs& q, hipStream_t s) {
+  const int form = project_form<T>(q), slots = q.none ? (int)project_slots(q) : 0, project = slots * ((q.rank + 15) / 16);
   const dim3 grid((unsigned)(project + ((g.m + 63) / 64 * g.splits + 7) / 8 * 8 * ((g.n + 63) / 64)));
+  if (form == A_K) hipLaunchKernelGGL((lora_few_kernel<T, LA, NG, A_K>), grid, dim3(512), 0, s, g, q, project, slots);
   if constexpr (T::bytes == 2) {
     if (form == A_R) hipLaunchKernelGGL((lora_few_kernel<T, LA, NG, A_R>), grid, dim3(512), 0, s, g, q, project, slots);
   }
-  if (form != A_R) hipLaunchKernelGGL((lora_few_kernel<T, LA, NG, A_K>), grid, dim3(512), 0, s, g, q, project, slots);
+  if (form == A_ANY) hipLaunchKernelGGL((lora_few_kernel<T, LA, NG, A_ANY>), grid, dim3(512), 0, s, g, q, project, slots);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   // Every output's own product with its factor's row, until that is the most of the call (167 tokens x 3264, 8 adapters: rank 16
@@ -257,17 +261,10 @@ template <typename T, int LA, int NG> hipError_t launch_few_tokens(const HalfGem
   return hipGetLastError();
 }
 template <typename T, int LA> hipError_t launch_few(HalfGemm g, const ProjectArgs& q, hipStream_t s) {
-  // factors that are read element by element keep the projection in a launch of its own
-  const int form = project_form<T>(q);
-  if (q.none && form == A_ANY) {
-    hipError_t e = lora_project_device(T::bytes == 4 ? 0 : __is_same(T, Bf16) ? (int)BF16 : (int)F16K, q, s);
-    if (e != hipSuccess) return e;
-  }
   int64_t piece;
-  g.splits = few_pieces(g.m, g.n, g.k, q.none && form != A_ANY ? project_slots(q) * ((q.rank + 15) / 16) : 0, &piece);
+  g.splits = few_pieces(g.m, g.n, g.k, q.none ? project_slots(q) * ((q.rank + 15) / 16) : 0, &piece);
   g.k_piece = (int)piece;
-  return g.n <= 16 ? launch_few_tokens<T, LA, 1>(g, q, form, s) : g.n <= 32 ? launch_few_tokens<T, LA, 2>(g, q, form, s)
-                                                                         : launch_few_tokens<T, LA, 4>(g, q, form, s);
+  return g.n <= 16 ? launch_few_tokens<T, LA, 1>(g, q, s) : g.n <= 32 ? launch_few_tokens<T, LA, 2>(g, q, s) : launch_few_tokens<T, LA, 4>(g, q, s);
 }
 
 }  // namespace

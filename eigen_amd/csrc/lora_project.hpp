@@ -182,6 +182,7 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
       for (int c = 0; c < 2; ++c) red[w][t][c][l] = acc[t][c];
   }
   __syncthreads();
+  const bool wide = g.ldp % 4 == 0 && (reinterpret_cast<uintptr_t>(g.p) & 15) == 0;
   for (int q = threadIdx.x; q < RT * 2 * 64; q += kProjWaves * 64) {
     const int t = q / 128, c = (q / 64) % 2, at = piece.begin + c * 16 + (l & 15);
     if (at >= piece.end) continue;
@@ -190,8 +191,12 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
       for (int z = 0; z < kProjWaves; ++z) sum += red[z][t][c][l];
     const int r = r0 + t * 16 + (l / 16) * 4;
     float* out = g.p + (int64_t)g.order[at] * g.ldp + r;
-    for (int e = 0; e < 4; ++e)
-      if (r + e < g.rank) out[e] = sum[e];
+    if (wide && r + 4 <= g.rank) {
+      *reinterpret_cast<f32x4*>(out) = sum;
+    } else {
+      for (int e = 0; e < 4; ++e)
+        if (r + e < g.rank) out[e] = sum[e];
+    }
   }
 }
 
