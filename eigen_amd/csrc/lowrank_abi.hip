@@ -17,7 +17,7 @@ using namespace eigamd;
 namespace {
 
 // Extents the kernels' 32-bit indices and grids are good for.
-constexpr int64_t kMaxFeatures = (int64_t)1 << 21, kMaxTokens = (int64_t)1 << 24, kMaxRank = 256, kMaxAdapters = 4096;
+constexpr int64_t kMaxFeatures = (int64_t)1 << 21, kMaxTokens = (int64_t)1 << 24, kMaxRank = 256, kMaxAdapters = 4096, kMaxStride = (int64_t)1 << 48;
 
 int bad(const char* entry, const char* what) { return abi_fail(EIGAMD_ERR_ARG, std::string(entry) + ": " + what); }
 int done(const char* entry, hipError_t e) {
@@ -30,9 +30,10 @@ bool kind_ok(int dtype) { return dtype == EIGAMD_F32 || dtype == EIGAMD_BF16 || 
 int bytes_of(int dtype) { return dtype == EIGAMD_F32 ? 4 : 2; }
 bool op_ok(int op) { return op == EIGAMD_OP_N || op == EIGAMD_OP_T; }
 bool extent_ok(int64_t v, int64_t most) { return v >= 0 && v <= most; }
-// a matrix of rows x cols at p: leading dimension, element alignment, and a pointer if there are elements
+// a matrix of rows x cols at p: leading dimension (to 2^38, so that no offset leaves 64 bits), element alignment, and a pointer if there
+// are elements
 bool matrix_ok(const void* p, int64_t rows, int64_t cols, int64_t ld, int es) {
-  return ld >= std::max<int64_t>(rows, 1) && (reinterpret_cast<uintptr_t>(p) % es) == 0 && (p || rows == 0 || cols == 0);
+  return ld >= std::max<int64_t>(rows, 1) && ld <= (int64_t)1 << 38 && (reinterpret_cast<uintptr_t>(p) % es) == 0 && (p || rows == 0 || cols == 0);
 }
 bool work_ok(const void* work, int64_t have, int64_t need) {
   return need == 0 || (work && have >= need && reinterpret_cast<uintptr_t>(work) % 16 == 0);
@@ -80,14 +81,14 @@ int eigamd_lora_dev(int dtype, int opw, int opa, int opb, int64_t m, int64_t n, 
   if (!matrix_ok(d_x, k, n, ldx, es)) return bad(me, "X: pointer, alignment or leading dimension");
   if (!matrix_ok(d_y, m, n, ldy, es)) return bad(me, "Y: pointer, alignment or leading dimension");
   if (n_adapters > 0) {
-    if (!matrix_ok(d_a, at ? k : rank, at ? rank : k, lda, es) || stride_a < 0) return bad(me, "A: pointer, alignment, leading dimension or stride");
-    if (!matrix_ok(d_b, bt ? rank : m, bt ? m : rank, ldb, es) || stride_b < 0) return bad(me, "B: pointer, alignment, leading dimension or stride");
+    if (!matrix_ok(d_a, at ? k : rank, at ? rank : k, lda, es) || !extent_ok(stride_a, kMaxStride)) return bad(me, "A: pointer, alignment, leading dimension or stride");
+    if (!matrix_ok(d_b, bt ? rank : m, bt ? m : rank, ldb, es) || !extent_ok(stride_b, kMaxStride)) return bad(me, "B: pointer, alignment, leading dimension or stride");
     if (!matrix_ok(d_p, rank, n, ldp, 4)) return bad(me, "P: pointer, alignment or leading dimension");
     if (!d_scale) return bad(me, "scale is null");
   }
   if (n == 0 || (m == 0 && n_adapters == 0)) return EIGAMD_OK;
   if (!d_plan) return bad(me, "plan is null");
-  if (d_y == d_x || (m > 0 && k > 0 && d_y == d_w)) return bad(me, "Y overlaps an input");
+  if (m > 0 && k > 0 && (d_y == d_x || d_y == d_w)) return bad(me, "Y overlaps an input");
   if (!work_ok(d_work, work_bytes, lora_work_bytes(dtype, wt, m, n, k, d_w, ldw, d_x, ldx))) return bad(me, "work is smaller than eigamd_lora_work_bytes or not 16-byte aligned");
   int rc = abi_ensure_device();
   if (rc != EIGAMD_OK) return rc;
@@ -123,12 +124,12 @@ int eigamd_lora_wgrad_dev(int dtype, int opg, int64_t rows, int64_t n, int64_t r
   if (rank < 1 || rank > kMaxRank) return bad(me, "rank out of range");
   if (!extent_ok(n_adapters, kMaxAdapters)) return bad(me, "number of adapters out of range");
   if (!matrix_ok(d_u, rows, n, ldu, d_exponents ? 1 : bytes_of(dtype))) return bad(me, "U: pointer, alignment or leading dimension");
-  if (d_exponents && lde < std::max<int64_t>((rows + 31) / 32, 1)) return bad(me, "exponents: leading dimension");
+  if (d_exponents && !matrix_ok(d_exponents, (rows + 31) / 32, n, lde, 1)) return bad(me, "exponents: leading dimension");
   if (!matrix_ok(d_p, rank, n, ldp, 4)) return bad(me, "P: pointer, alignment or leading dimension");
   const bool gt = opg == EIGAMD_OP_T;
   const int64_t gr = gt ? rank : rows, gc = gt ? rows : rank;
   if (n_adapters > 0 && !matrix_ok(d_g, gr, gc, ldg, 4)) return bad(me, "G: pointer, alignment or leading dimension");
-  if (n_adapters > 1 && rows > 0 && stride_g < ldg * (gc - 1) + gr) return bad(me, "G: matrices of neighbouring adapters overlap");
+  if (n_adapters > 1 && rows > 0 && (stride_g < ldg * (gc - 1) + gr || stride_g > kMaxStride)) return bad(me, "G: matrices of neighbouring adapters overlap, or a stride out of range");
   if (!beta) return bad(me, "beta is null");
   if (n_adapters == 0 || rows == 0) return EIGAMD_OK;
   if (!d_plan || !d_scale) return bad(me, "null pointer");

@@ -58,8 +58,11 @@ class Checkpoint8:
             exponents = torch.empty(self.lde * max(self.cols, 1), dtype=torch.uint8, device=storage.device)
         if storage.dtype != torch.int8 or exponents.dtype != torch.uint8:
             raise ValueError("storage must be int8 and exponents uint8")
-        _holds(storage, 0, self.ld, self.rows, self.cols, "storage")
-        _holds(exponents, 0, self.lde, blocks, self.cols, "exponents")
+        if not storage.is_contiguous() or not exponents.is_contiguous():
+            raise ValueError("storage and exponents must be contiguous")
+        if self.rows and self.cols and (self.ld * (self.cols - 1) + self.rows > storage.numel()
+                                        or self.lde * (self.cols - 1) + blocks > exponents.numel()):
+            raise ValueError("storage or exponents are too small for the matrix")
         self.storage, self.exponents = storage, exponents
 
     @property
@@ -72,11 +75,6 @@ class LoraPlan:
 
     def __init__(self, n, n_adapters, storage):
         self.n, self.n_adapters, self.storage = n, n_adapters, storage
-
-
-def _holds(storage, offset, ld, rows, cols, what):
-    if rows and cols and (offset < 0 or offset + ld * (cols - 1) + rows > storage.numel()):
-        raise ValueError(f"{what}: the storage is too small for the matrix")
 
 
 def _check_matrix(m, kind, rows, cols, what, count=1):

@@ -436,7 +436,8 @@ int eigamd_trmm_dev(int dtype, int side, int uplo, int op, int diag, int64_t m, 
  * or, with d_exponents, an 8-bit checkpoint (below; d_u then points to int8).  An adapter without tokens gets beta G_j; with
  * beta = 0 G is not read.
  *
- * Limits: m, k, rows <= 2^21, n <= 2^24, rank 1..256, n_adapters <= 4096; n = 0 and n_adapters = 0 are allowed.  d_work is
+ * Limits: m, k, rows <= 2^21, n <= 2^24, rank 1..256, n_adapters <= 4096, leading dimensions <= 2^38, strides <= 2^48; n = 0 and
+ * n_adapters = 0 are allowed.  d_work is
  * device memory of at least the bytes the matching query names (16-byte aligned; 0: may be NULL; it depends on the operands'
  * alignment: one without whole aligned 16-byte chunks along its columns may be copied there), free again behind the call;
  * calls that may overlap need one each, so do captured graphs.  Everything is asynchronous on `stream`, allocates nothing, and

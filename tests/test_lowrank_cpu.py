@@ -126,3 +126,21 @@ def test_python_layer_refuses_what_does_not_fit():
         lowrank.Checkpoint8(40, 2, kind, storage=torch.zeros(79, dtype=torch.int8))
     with pytest.raises(IndexError):
         st(r, k).matrix(2)
+
+
+def test_leading_dimensions_and_strides_out_of_range():
+    big = 2 ** 38 + 8
+    for change in (dict(ldw=big), dict(ldx=big), dict(ldy=big), dict(lda=big), dict(ldb=big), dict(ldp=big), dict(sa=2 ** 49), dict(sb=2 ** 49)):
+        assert call(lib.eigamd_lora_dev, LORA, **change) == _lib.ERR_ARG, change
+    for change in (dict(ldu=big), dict(ldp=big), dict(ldg=big, sg=2 ** 41), dict(sg=2 ** 49), dict(e=P, lde=big)):
+        assert call(lib.eigamd_lora_wgrad_dev, GRAD, **change) == _lib.ERR_ARG, change
+    for change in (dict(lddy=big), dict(ldq=big), dict(lde=big), dict(lddw=big)):
+        assert call(lib.eigamd_ckpt8_wgrad_dev, WGRAD, **change) == _lib.ERR_ARG, change
+
+
+def test_a_checkpoint_of_strided_storage_is_refused():
+    kind = _lib.BF16
+    with pytest.raises(ValueError):
+        lowrank.Checkpoint8(40, 2, kind, storage=torch.zeros(160, dtype=torch.int8)[::2])
+    with pytest.raises(ValueError):
+        lowrank.Checkpoint8(40, 2, kind, storage=torch.zeros(80, dtype=torch.int8), exponents=torch.zeros(8, dtype=torch.uint8)[::2])
