@@ -25,7 +25,8 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------- plan
 // One workgroup per adapter (and one for the tokens without): its waves count, each in its part of the batch, the tokens in front
 // of the adapter's run and the adapter's own, and then list those in their order, by ballots -- no atomics, no prefix sum over
-// adapters, the same list every time.  Eight loads of a wave are under way together.
+// adapters, the same list every time.  Eight loads of a wave are under way together, else every 64 tokens would wait for memory (8192
+// tokens, 48 adapters 4.6 us).
 __global__ __launch_bounds__(512) void lora_plan_kernel(const int* __restrict__ ids, int n, int adapters, int* __restrict__ order,
                                                         int* __restrict__ seg, int* __restrict__ starts) {
   __shared__ int before[8], own[8];
@@ -224,7 +225,7 @@ struct GradArgs {
 };
 
 // Tokens per workgroup: about 512 workgroups in all, between 128 and 1024 tokens each (1000 tokens x 1024, one
-// adapter of rank 8: 11.4 us, with 256 or more 16.0).
+// adapter of rank 8: 9.6 us, with 256 or more 14.2).
 int grad_chunk(int64_t rows, int64_t n) {
   const int64_t across = (rows + kGradRows - 1) / kGradRows;
   const int64_t pieces = std::max<int64_t>(512 / across, 1);

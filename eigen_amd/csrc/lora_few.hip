@@ -15,8 +15,8 @@ namespace {
 // Y for few tokens, 16 NG of them a workgroup: the time is that of reading W, from as many compute units as there are.  A
 // workgroup owns 64 rows and one piece of the reduction, so that X, which every workgroup reads its piece of, costs little beside
 // W (with 16 rows and the whole reduction X was four times the traffic: 64 tokens x 4096 x 4096 took 22 us, now 12).  Its eight
-// waves share the piece, 64 (32) positions a turn, from memory to the matrix unit directly (W's reduction contiguous) or through the
-// wave's own LDS and back transposed (its rows contiguous).  The sums go to memory in 32 bits; the second kernel adds the
+// waves share the piece, 64 (32) positions a turn, turned in the wave's own LDS (W's reduction contiguous: as a RowBlock; its rows: read
+// back transposed).  The sums go to memory in 32 bits; the second kernel adds the
 // pieces up and the low-rank part to them.
 // The projection needs nothing of this, so its workgroups (16 ranks each) are the first ones of the same launch.
 template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512) void lora_few_kernel(HalfGemm g, ProjectArgs q, int project, int slots) {
@@ -231,7 +231,7 @@ bool piece_allowed(int64_t blocks, int64_t k, int64_t pieces) {
 }
 // A compute unit runs one of these workgroups at a time, so the 64-row blocks times the pieces and the projection's workgroups
 // should fill whole rounds of 256; a round costs what its piece does plus the latencies at both ends, about as much as 600
-// positions (64 tokens x 4096 x 4096: 512 workgroups 16.8 us, 256 12.6).
+// positions (64 tokens x 4096 x 4096: 16.8 us, with pieces for 512 at a time 21.1).
 int few_pieces(int64_t m, int64_t n, int64_t k, int64_t project, int64_t* k_piece) {
   const int64_t blocks = (m + 63) / 64 * ((n + 63) / 64);
   int64_t best = 1, best_cost = INT64_MAX;
@@ -290,7 +290,7 @@ int64_t lora_few_work_bytes(int64_t m, int64_t n, int64_t k) {
 }
 
 hipError_t lora_few_device(int kind, bool w_trans, const HalfGemm& g, const ProjectArgs& q, hipStream_t s) {
-  if (kind != BF16 && kind != F16K) return w_trans ? launch_few<Fp32, KC>(g, q, s) : hipErrorInvalidValue;
+  if (kind != BF16 && kind != F16K) return launch_few<Fp32, KC>(g, q, s);      // (W transposed only)
   if (kind == BF16) return w_trans ? launch_few<Bf16, KC>(g, q, s) : launch_few<Bf16, MC>(g, q, s);
   return w_trans ? launch_few<F16, KC>(g, q, s) : launch_few<F16, MC>(g, q, s);
 }

@@ -5,6 +5,7 @@ Column-major, one token per column: a torch tensor of shape (tokens, features) i
 same storage.  Every call is asynchronous on ``stream`` (default: torch's current stream of the operands' device)."""
 import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -160,6 +161,12 @@ def _scratch(work, need, like):
     return work.data_ptr(), need, work
 
 
+# The queries depend on sizes and alignment alone (the pointers' last four bits stand for them), so a program's few answers are kept.
+_lora_need = functools.lru_cache(maxsize=4096)(lib.eigamd_lora_work_bytes)
+_lora_wgrad_need = functools.lru_cache(maxsize=4096)(lib.eigamd_lora_wgrad_work_bytes)
+_ckpt8_wgrad_need = functools.lru_cache(maxsize=4096)(lib.eigamd_ckpt8_wgrad_work_bytes)
+
+
 def lora_plan(adapter_of, n_adapters, stream=None):
     """Plan of a batch: ``adapter_of`` (int32, one per token; anything outside [0, n_adapters) means no adapter).  Made once per
     batch, used by every projection, forward and backward."""
@@ -207,7 +214,7 @@ def lora_dev(opw, w, x, opa, a, opb, b, scale, plan, p, y, work=None, stream=Non
     if s is None:
         with _there(stream, x.storage):
             return lora_dev(opw, w, x, opa, a, opb, b, scale, plan, p, y, work)
-    at, have, work = _scratch(work, lib.eigamd_lora_work_bytes(kind, ow, m, n, k, at_w, w.ld, at_x, x.ld), x.storage)
+    at, have, work = _scratch(work, _lora_need(kind, ow, m, n, k, at_w & 15, w.ld, at_x & 15, x.ld), x.storage)
     rc = lib.eigamd_lora_dev(kind, ow, oa, ob, m, n, k, rank, count, at_w, w.ld, at_x, x.ld, at_a, a.ld, a.stride, at_b, b.ld, b.stride, at_s,
                              plan.storage.data_ptr(), at_p, p.ld, at_y, y.ld, at, have, s)
     if rc:
@@ -239,7 +246,7 @@ def lora_wgrad_dev(opg, u, p, scale, plan, beta, g, work=None, stream=None):
     if s is None:
         with _there(stream, u.storage):
             return lora_wgrad_dev(opg, u, p, scale, plan, beta, g, work)
-    at, have, work = _scratch(work, lib.eigamd_lora_wgrad_work_bytes(rows, n, rank, count), u.storage)
+    at, have, work = _scratch(work, _lora_wgrad_need(rows, n, rank, count), u.storage)
     rc = lib.eigamd_lora_wgrad_dev(kind, og, rows, n, rank, count, at_u, u.ld, exps, lde, at_p, p.ld, at_s, plan.storage.data_ptr(),
                                    ctypes.byref(ctypes.c_float(beta)), at_g, g.ld, g.stride, at, have, s)
     if rc:
@@ -287,7 +294,7 @@ def ckpt8_wgrad_dev(opw, dy, c, beta, dw, work=None, stream=None):
     if s is None:
         with _there(stream, dy.storage):
             return ckpt8_wgrad_dev(opw, dy, c, beta, dw, work)
-    at, have, work = _scratch(work, lib.eigamd_ckpt8_wgrad_work_bytes(kind, m, n, k, at_dy, dy.ld), dy.storage)
+    at, have, work = _scratch(work, _ckpt8_wgrad_need(kind, m, n, k, at_dy & 15, dy.ld), dy.storage)
     rc = lib.eigamd_ckpt8_wgrad_dev(kind, ow, m, n, k, at_dy, dy.ld, c.storage.data_ptr(), c.ld, c.exponents.data_ptr(), c.lde,
                                     ctypes.byref(ctypes.c_float(beta)), at_dw, dw.ld, at, have, s)
     if rc:
