@@ -225,6 +225,102 @@ template <typename T> __global__ __launch_bounds__(256) void lora_few_tile_join_
   }
 }
 
+// One token with at most 32 ranks, W and its factor with a contiguous reduction: one launch.  A workgroup owns 16 rows; four of its
+// waves take them, 4 rows each, in lines of 1 KB; the other four compute P, every workgroup for itself (from the caches), so that
+// nothing has to be waited for and no sums go through memory: 2048 x 2048, rank 16 8.1 -> 6.1 us, 8192 x 8192 38 -> 33, 1024 x 16384
+// 23 -> 17; with rank 32 as fast (4096 x 4096 12.9) but for the second launch, beyond slower.
+constexpr int kTokenRanks = 32;
+template <typename T> __global__ __launch_bounds__(512) void lora_token_kernel(HalfGemm g, ProjectArgs q) {
+  using E = typename T::elem;
+  using x8 = typename T::x8;
+  __shared__ float y[16], p[kTokenRanks];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63;
+  const int row0 = blockIdx.x * 16, chunks = g.k / 8, token = g.order[0], who = g.seg[0], ranks = who != g.none ? g.rank : 0;
+  const E* x = static_cast<const E*>(g.b) + (int64_t)token * g.ldb;
+  // Sums of four rows with x: chunks of 8, two turns of 64 lanes under way together (four: 2048 x 2048 9.8 us), then what is left, one
+  // a lane.
+  auto dots = [&](const E* const (&row)[4], float (&sum)[4]) {
+    constexpr int TURNS = 2;
+    for (int c0 = 0; c0 < chunks; c0 += 64 * TURNS) {
+      x8 a[TURNS][4], b[TURNS];
+#pragma unroll
+      for (int u = 0; u < TURNS; ++u) {
+        const int c = c0 + u * 64 + l, at = (c < chunks ? c : chunks - 1) * 8;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) a[u][v] = load_8<E, x8>(row[v] + at);
+        b[u] = load_8<E, x8>(x + at);
+      }
+#pragma unroll
+      for (int u = 0; u < TURNS; ++u) {
+        const bool in = c0 + u * 64 + l < chunks;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          float d = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d = __builtin_fmaf((float)a[u][v][e], (float)b[u][e], d);
+          sum[v] += in ? d : 0.0f;
+        }
+      }
+    }
+    const int k = chunks * 8 + l;
+    if (k < g.k) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) sum[v] += (float)row[v][k] * (float)x[k];
+    }
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) sum[v] += __shfl_xor(sum[v], d);
+  };
+  // this row's part of the other factor, on its way before anything is waited for
+  const int row = row0 + threadIdx.x;
+  const bool mine = threadIdx.x < 16 && row < g.m;
+  x8 up[kTokenRanks / 8];
+  if (mine) {
+    const E* from = static_cast<const E*>(g.up) + (int64_t)who * g.up_stride + (int64_t)row * g.up_row;
+#pragma unroll
+    for (int r = 0; r < kTokenRanks; r += 8)
+      if (r < ranks) up[r / 8] = load_first<E, x8>(from + (int64_t)r * g.up_rank, g.up_rank, ranks - r);
+  }
+  const E* rows[4];
+  float sum[4] = {};
+  if (w < 4) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int r = row0 + w * 4 + v;
+      rows[v] = static_cast<const E*>(g.a) + (int64_t)(r < g.m ? r : g.m - 1) * g.lda;
+    }
+    dots(rows, sum);
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      if (l == 0) y[w * 4 + v] = sum[v];
+  } else {
+    for (int r0 = (w - 4) * 4; r0 < ranks; r0 += 16) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        rows[v] = static_cast<const E*>(q.a) + (int64_t)who * q.a_stride + (int64_t)(r0 + v < ranks ? r0 + v : ranks - 1) * q.a_row;
+        sum[v] = 0.0f;
+      }
+      dots(rows, sum);
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (l == 0 && r0 + v < ranks) p[r0 + v] = sum[v];
+    }
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && (int)threadIdx.x < g.rank) q.p[(int64_t)token * q.ldp + threadIdx.x] = ranks ? p[threadIdx.x] : 0.0f;
+  if (!mine) return;
+  float out = y[threadIdx.x];
+  if (ranks) {
+    float d = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kTokenRanks; ++r)
+      if (r < ranks) d += (float)up[r / 8][r % 8] * p[r];
+    out += g.scale[who] * d;
+  }
+  static_cast<E*>(g.c)[(int64_t)token * g.ldc + row] = (E)out;
+}
+
 // Pieces of the reduction, none shorter than 512 (eight waves, 64 positions each), at most 512 workgroups.
 bool piece_allowed(int64_t blocks, int64_t k, int64_t pieces) {
   return pieces == 1 || (pieces <= 16 && k / pieces >= 512 && blocks * pieces <= 512);
@@ -261,6 +357,12 @@ template <typename T, int LA, int NG> hipError_t launch_few_tokens(const HalfGem
   return hipGetLastError();
 }
 template <typename T, int LA> hipError_t launch_few(HalfGemm g, const ProjectArgs& q, hipStream_t s) {
+  if constexpr (LA == KC) {
+    if (g.n == 1 && g.rank <= kTokenRanks && (g.rank == 0 || project_form<T>(q) == A_K)) {
+      hipLaunchKernelGGL(lora_token_kernel<T>, dim3((unsigned)((g.m + 15) / 16)), dim3(512), 0, s, g, q);
+      return hipGetLastError();
+    }
+  }
   int64_t piece;
   g.splits = few_pieces(g.m, g.n, g.k, q.none ? project_slots(q) * ((q.rank + 15) / 16) : 0, &piece);
   g.k_piece = (int)piece;

@@ -127,6 +127,16 @@ def test_lora_small_tiles(kind, ops, m, n, k, rank):
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("pad, shift", [(0, 0), (3, 1)])
+@pytest.mark.parametrize("m, n, k, rank", [(130, 1, 2056, 32), (97, 1, 1003, 7), (16, 1, 7, 33), (520, 1, 4096, 16), (33, 2, 264, 9)])
+def test_lora_single_tokens(kind, pad, shift, m, n, k, rank):
+    # on both sides of 32 ranks; with and without an adapter
+    for ids in ([0] * n, [-1] * n, [2, 9, 0, 2][:n]):
+        Case(kind, m, n, k, rank, 3, "TTT", pad, shift, ids=ids).run().check()
+    Case(kind, m, n, k, rank, 3, "TTN", pad, shift).run().check()
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
 @pytest.mark.parametrize("ops", ["TTT", "NNN"])
 @pytest.mark.parametrize("m, n, k, rank", [(1601, 130, 136, 100), (1600, 99, 520, 130)])
 def test_lora_few_tokens_and_large_ranks(kind, ops, m, n, k, rank):
@@ -184,6 +194,19 @@ def test_what_is_not_finite_stays_with_its_request(kind, opw, n):
     d.run()
     rest = torch.arange(n, device="cuda") != 1
     assert bool(torch.isnan(d.Y.as_strided()[:, 1]).all()) and bool(torch.isfinite(d.Y.as_strided()[:, rest]).all())
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+def test_a_single_token_meets_its_own_adapter_only(kind):
+    for ids in ([0], [-1]):
+        c = Case(kind, 40, 1, 72, 5, 2, ids=ids)
+        c.A.matrix(1).as_strided().fill_(float("nan"))
+        c.B.matrix(1).as_strided().fill_(float("inf"))
+        c.run().check()
+        c.A.matrix(0).as_strided()[0, 0] = float("nan")
+        c.run()
+        bad = ids == [0]
+        assert bool(torch.isnan(c.Y.as_strided()).all()) == bad and bool(torch.isnan(c.P.as_strided()).any()) == bad
 
 
 @pytest.mark.parametrize("kind", [BF16, F16], ids=NAME.get)
