@@ -22,7 +22,10 @@ namespace {
 template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512) void lora_few_kernel(HalfGemm g, ProjectArgs q, int project, int slots) {
   using E = typename T::elem;
   using x8 = typename T::x8;
-  using Block = RowBlock<T>;
+  // Products of a turn, one block of each operand: lines of 128 bytes (64 tokens x 8192 x 8192 52 -> 45 us, 192 x 4096 x 4096 27 -> 25; 98 x
+  // 7744 x 1088 17.0 -> 17.6).  W's rows contiguous, 64 tokens: no registers for that.
+  constexpr int S = T::bytes == 4 || (NG == 4 && LA == MC) ? 1 : 2;
+  using Block = RowBlock<T, S>;
   constexpr int red_bytes = 8 * 4 * NG * 64 * 16, blocks_bytes = 8 * (4 + NG) * Block::bytes;
   constexpr int loop_bytes = blocks_bytes > project_lds(1, T::bytes) ? blocks_bytes : project_lds(1, T::bytes);
   constexpr int lds_bytes = red_bytes > loop_bytes ? red_bytes : loop_bytes;
@@ -37,98 +40,106 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
   const int row0 = part % row_blocks * 64, z = part / row_blocks;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63;
   const int k_begin = z * g.k_piece, k_end = k_begin + g.k_piece < g.k ? k_begin + g.k_piece : g.k;
-  const E* a[4];                      // KC: rows of the four row blocks; MC: chunks of 8 lines
-  const E* b[NG];                     // rows and columns past the end repeat the last one and are not stored
+  const E* a[4][S];                   // KC: rows of the four row blocks; MC: chunks of 8 lines
+  const E* b[NG][S];                  // rows and columns past the end repeat the last one and are not stored
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    if constexpr (LA == KC) {
-      const int row = row0 + t * 16 + Block::row();
-      a[t] = static_cast<const E*>(g.a) + (int64_t)(row < g.m ? row : g.m - 1) * g.lda;
-    } else {
-      const int row = row0 + (l % 8) * 8;
-      a[t] = static_cast<const E*>(g.a) + (int64_t)(t * 8 + l / 8) * g.lda + (row < g.m ? row : 0);
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int h = 0; h < S; ++h) {
+      if constexpr (LA == KC) {
+        const int row = row0 + t * 16 + Block::row(h);
+        a[t][h] = static_cast<const E*>(g.a) + (int64_t)(row < g.m ? row : g.m - 1) * g.lda;
+      } else {
+        const int row = row0 + (l % 8) * 8;
+        a[t][h] = static_cast<const E*>(g.a) + (int64_t)(h * 32 + t * 8 + l / 8) * g.lda + (row < g.m ? row : 0);
+      }
     }
-  }
 #pragma unroll
-  for (int c = 0; c < NG; ++c) {
-    const int at = col0 + c * 16 + Block::row();
-    b[c] = static_cast<const E*>(g.b) + (int64_t)g.order[at < g.n ? at : g.n - 1] * g.ldb;
-  }
+  for (int c = 0; c < NG; ++c)
+#pragma unroll
+    for (int h = 0; h < S; ++h) {
+      const int at = col0 + c * 16 + Block::row(h);
+      b[c][h] = static_cast<const E*>(g.b) + (int64_t)g.order[at < g.n ? at : g.n - 1] * g.ldb;
+    }
   f32x4 acc[4][NG] = {};
-  // whole turns, then what is left, one product a wave (as in project_piece)
-  constexpr int S = NG == 4 || T::bytes == 4 ? 1 : 2;
+  // whole turns, then what is left, by one wave (as in project_piece)
   using Whole = std::true_type;
   using Rest = std::false_type;
-  auto load = [&](int k0, x8(&fa)[4], x8(&fb)[NG], auto whole) {
+  auto load = [&](int k0, x8(&fa)[4][S], x8(&fb)[NG][S], auto whole) {
     const int k = k0 + Block::position(), left = k_end - k;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if constexpr (LA == KC) {
-        fa[t] = whole ? load_8<E, x8>(a[t] + k) : load_first<E, x8>(a[t] + (left > 0 ? k : 0), 1, left);
-      } else {
-        const bool in = whole || k0 + t * 8 + l / 8 < k_end;
-        x8 v = load_8<E, x8>(in ? a[t] + (int64_t)k0 * g.lda : static_cast<const E*>(g.a));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = in ? v[e] : (E)0.0f;
-        fa[t] = v;
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < NG; ++c) fb[c] = whole ? load_8<E, x8>(b[c] + k) : load_first<E, x8>(b[c] + (left > 0 ? k : 0), 1, left);
-  };
-  auto multiply = [&](const x8(&fa)[4], const x8(&fb)[NG]) {
-    x8 f[4], y[NG];
-    char* mine = lds + w * (4 + NG) * Block::bytes;
-#pragma unroll
-    for (int c = 0; c < NG; ++c) Block::put(mine + (4 + c) * Block::bytes, fb[c]);
-    if constexpr (LA == MC) {
-      // lines of 64 rows, 128 bytes; chunks permuted so that the 8 lines a half wave reads meet all banks once
-      auto slot = [](int line, int ch) { return line * 128 + (ch ^ (((line >> 1) & 1) | ((line >> 2) & 2)) << 1) * 16; };
-#pragma unroll
-      for (int t = 0; t < 4; ++t) *reinterpret_cast<x8*>(mine + slot(t * 8 + l / 8, l % 8)) = fa[t];
+    for (int h = 0; h < S; ++h) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        union { x8 v; typename T::x4 h[2]; } u;
-        const int line = (l / 16) * 8 + (l & 15) / 4, ch = t * 2 + (l & 3) / 2;
+        if constexpr (LA == KC) {
+          fa[t][h] = whole ? load_8<E, x8>(a[t][h] + k) : load_first<E, x8>(a[t][h] + (left > 0 ? k : 0), 1, left);
+        } else {
+          const bool in = whole || k0 + h * 32 + t * 8 + l / 8 < k_end;
+          x8 v = load_8<E, x8>(in ? a[t][h] + (int64_t)k0 * g.lda : static_cast<const E*>(g.a));
 #pragma unroll
-        for (int h = 0; h < 2; ++h) u.h[h] = T::read_transposed(mine + slot(line + 4 * h, ch) + (l & 1) * 8);
-        f[t] = u.v;
+          for (int e = 0; e < 8; ++e) v[e] = in ? v[e] : (E)0.0f;
+          fa[t][h] = v;
+        }
       }
-    } else {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) Block::put(mine + t * Block::bytes, fa[t]);
+      for (int c = 0; c < NG; ++c) fb[c][h] = whole ? load_8<E, x8>(b[c][h] + k) : load_first<E, x8>(b[c][h] + (left > 0 ? k : 0), 1, left);
+    }
+  };
+  auto multiply = [&](const x8(&fa)[4][S], const x8(&fb)[NG][S]) {
+    char* mine = lds + w * (4 + NG) * Block::bytes;
+    auto own = [&](int t) { return mine + t * Block::bytes; };
 #pragma unroll
-      for (int t = 0; t < 4; ++t) f[t] = Block::get(mine + t * Block::bytes);
+    for (int h = 0; h < S; ++h) {
+#pragma unroll
+      for (int c = 0; c < NG; ++c) Block::put(own(4 + c), fb[c][h], h);
+      if constexpr (LA == KC) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) Block::put(own(t), fa[t][h], h);
+      }
     }
 #pragma unroll
-    for (int c = 0; c < NG; ++c) y[c] = Block::get(mine + (4 + c) * Block::bytes);
+    for (int h = 0; h < S; ++h) {
+      x8 f[4], y[NG];
+      if constexpr (LA == MC) {
+        // lines of 64 rows, 128 bytes; chunks permuted so that the 8 lines a half wave reads meet all banks once
+        auto slot = [](int line, int ch) { return line * 128 + (ch ^ (((line >> 1) & 1) | ((line >> 2) & 2)) << 1) * 16; };
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t) *reinterpret_cast<x8*>(mine + slot(t * 8 + l / 8, l % 8)) = fa[t][h];
 #pragma unroll
-      for (int c = 0; c < NG; ++c) acc[t][c] = T::mma(f[t], y[c], acc[t][c]);
+        for (int t = 0; t < 4; ++t) {
+          union { x8 v; typename T::x4 h[2]; } u;
+          const int line = (l / 16) * 8 + (l & 15) / 4, ch = t * 2 + (l & 3) / 2;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) u.h[e] = T::read_transposed(mine + slot(line + 4 * e, ch) + (l & 1) * 8);
+          f[t] = u.v;
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) f[t] = Block::get(own(t), h);
+      }
+#pragma unroll
+      for (int c = 0; c < NG; ++c) y[c] = Block::get(own(4 + c), h);
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int c = 0; c < NG; ++c) acc[t][c] = T::mma(f[t], y[c], acc[t][c]);
+    }
   };
-  x8 fa[2][S][4], fb[2][S][NG];
-  auto load_turn = [&](int turn, int set) {
-#pragma unroll
-    for (int s = 0; s < S; ++s) load(k_begin + (turn * S + s) * 32, fa[set][s], fb[set][s], Whole{});
-  };
-  auto multiply_turn = [&](int set) {
-#pragma unroll
-    for (int s = 0; s < S; ++s) multiply(fa[set][s], fb[set][s]);
-  };
+  x8 fa[2][4][S], fb[2][NG][S];
   const int turns = (k_end - k_begin) / (32 * S);
+  auto load_turn = [&](int turn, int set) { load(k_begin + turn * 32 * S, fa[set], fb[set], Whole{}); };
   int at = w;
   if (at < turns) load_turn(at, 0);
   for (; at < turns; at += 16) {
     if (at + 8 < turns) load_turn(at + 8, 1);
-    multiply_turn(0);
+    multiply(fa[0], fb[0]);
     if (at + 8 >= turns) break;
     if (at + 16 < turns) load_turn(at + 16, 0);
-    multiply_turn(1);
+    multiply(fa[1], fb[1]);
   }
-  if (const int k0 = k_begin + (turns * S + w) * 32; k0 < k_end) {
-    load(k0, fa[0][0], fb[0][0], Rest{});
-    multiply(fa[0][0], fb[0][0]);
+  if (const int k0 = k_begin + turns * 32 * S; w == turns % 8 && k0 < k_end) {
+    load(k0, fa[0], fb[0], Rest{});
+    multiply(fa[0], fb[0]);
   }
   __syncthreads();
   f32x4(&red)[8][4][NG][64] = *reinterpret_cast<f32x4(*)[8][4][NG][64]>(lds);
@@ -373,7 +384,7 @@ template <typename T, int LA> hipError_t launch_few(HalfGemm g, const ProjectArg
 
 // Up to 64 tokens, and beyond as long as this is one round and quicker than large tiles with the projection in front of them: 3 us,
 // and 5 + 4.4 per thousand positions a round, against the plan's time, 6 us and 1.25 per thousand positions for the projection
-// (256 tokens x 1024 x 1024 18.7 -> 10.4 us, 142 x 2456 x 4032 29.6 -> 17.9, 192 x 4096 x 4096 31.5 -> 27.0; not 96 x 4096 x 16384,
+// (256 tokens x 1024 x 1024 18.7 -> 10.4 us, 142 x 2456 x 4032 29.6 -> 17.9, 192 x 4096 x 4096 31.5 -> 25.1; not 96 x 4096 x 16384,
 // 62.5 -> 69.2).  Single precision: against the library's product, which has larger tiles still, up to two rounds (777 x 1024 x
 // 1536 72.6 -> 45.9 us, 1500 x 1000 x 2000 114 -> 108, 2048 x 2048 x 2048 180 -> 214).
 bool lora_few(bool f32, int64_t m, int64_t n, int64_t k) {

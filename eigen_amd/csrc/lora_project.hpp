@@ -16,31 +16,31 @@ struct ProjectArgs {
   float* p; int64_t ldp;
 };
 
-// 16 rows x 32 positions on their way from memory to the matrix unit.  A fragment has neighbouring lanes on different rows; loaded
-// so, a load takes the memory pipeline 64 cycles, a row's address at a time.  Here four neighbouring lanes take 64 bytes (128) of
-// one row, and the wave's own LDS turns them into fragments (the projection of 32 tokens x 4032 to 16 ranks: 15 us, now 9); chunks of
-// a row are permuted so that the 16 lanes that read together meet all banks once.
-template <typename T> struct RowBlock {
+// 16 rows x 32 S positions on their way from memory to the matrix unit.  A fragment has neighbouring lanes on different rows; loaded
+// so, a load takes the memory pipeline 64 cycles, a row's address at a time.  Here 4 S neighbouring lanes take 64 S bytes (128 of
+// single precision) of one row, S loads a block, and the wave's own LDS turns them into fragments (the projection of 32 tokens x 4032
+// to 16 ranks: 15 us, now 9); chunks of a row are permuted so that the 16 lanes that read together meet all banks once.
+template <typename T, int S = 1> struct RowBlock {
   using x8 = typename T::x8;
-  static constexpr int bytes = 512 * T::bytes;
-  static __device__ __forceinline__ int row() { return (threadIdx.x & 63) / 4; }
-  static __device__ __forceinline__ int position() { return (threadIdx.x & 3) * 8; }
+  static_assert(S == 1 || (S == 2 && T::bytes == 2), "rows of 64 or 128 bytes");
+  static constexpr int bytes = 512 * S * T::bytes;
+  static __device__ __forceinline__ int row(int load = 0) { return load * (16 / S) + (threadIdx.x & 63) / (4 * S); }
+  static __device__ __forceinline__ int position() { return threadIdx.x % (4 * S) * 8; }
   static __device__ __forceinline__ int at(int row, int chunk) {       // of 16 bytes
-    return T::bytes == 2 ? row * 64 + (chunk ^ ((row / 4) & 3)) * 16 : row * 128 + (chunk ^ ((row / 2) & 7)) * 16;
+    return S * T::bytes == 2 ? row * 64 + (chunk ^ ((row / 4) & 3)) * 16 : row * 128 + (chunk ^ ((row / 2) & 7)) * 16;
   }
-  static __device__ __forceinline__ void put(char* lds, x8 v) {
-    const int l = threadIdx.x & 63;
+  static __device__ __forceinline__ void put(char* lds, x8 v, int load = 0) {
     constexpr int H = T::bytes / 2;
     const Half<x8> u = __builtin_bit_cast(Half<x8>, v);
 #pragma unroll
-    for (int h = 0; h < H; ++h) *reinterpret_cast<f32x4*>(lds + at(l / 4, (l % 4) * H + h)) = u.part[h];
+    for (int h = 0; h < H; ++h) *reinterpret_cast<f32x4*>(lds + at(row(load), threadIdx.x % (4 * S) * H + h)) = u.part[h];
   }
-  static __device__ __forceinline__ x8 get(const char* lds) {
+  static __device__ __forceinline__ x8 get(const char* lds, int step = 0) {
     const int l = threadIdx.x & 63;
     constexpr int H = T::bytes / 2;
     Half<x8> u;
 #pragma unroll
-    for (int h = 0; h < H; ++h) u.part[h] = *reinterpret_cast<const f32x4*>(lds + at(l % 16, (l / 16) * H + h));
+    for (int h = 0; h < H; ++h) u.part[h] = *reinterpret_cast<const f32x4*>(lds + at(l % 16, step * 4 + (l / 16) * H + h));
     return __builtin_bit_cast(x8, u);
   }
 
