@@ -145,8 +145,8 @@ HalfWork half_work(bool w_trans, int64_t m, int64_t n, int64_t k, const void* w,
   HalfWork need = {0, 0, 0};
   const bool w_whole = whole_chunks(w, ldw, w_trans ? k : m);
   if (lora_few(false, m, n, k)) {
-    need.sums = lora_few_work_bytes(m, n, k);      // (W's reduction contiguous: read where it is, whatever its alignment)
-    if (!w_trans && !w_whole) need.w_copy = padded_bytes(m, k);
+    need.sums = lora_few_work_bytes(m, n, k);      // (read where they are, whatever their alignment; chunks of 8 rows have to exist)
+    if (!w_trans && m < 8) need.w_copy = padded_bytes(m, k);
   } else {
     const int splits = plan_tiles(m, n, k).splits;
     if (splits > 1) need.sums = (int64_t)splits * m * n * 4;

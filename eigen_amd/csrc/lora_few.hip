@@ -40,6 +40,7 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
   const int row0 = part % row_blocks * 64, z = part / row_blocks;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63;
   const int k_begin = z * g.k_piece, k_end = k_begin + g.k_piece < g.k ? k_begin + g.k_piece : g.k;
+  const int last = g.m < 8 ? 0 : g.m - 8;      // MC: a chunk of 8 rows that would pass the end holds the last 8, some of them twice
   const E* a[4][S];                   // KC: rows of the four row blocks; MC: chunks of 8 lines
   const E* b[NG][S];                  // rows and columns past the end repeat the last one and are not stored
 #pragma unroll
@@ -51,7 +52,7 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
         a[t][h] = static_cast<const E*>(g.a) + (int64_t)(row < g.m ? row : g.m - 1) * g.lda;
       } else {
         const int row = row0 + (l % 8) * 8;
-        a[t][h] = static_cast<const E*>(g.a) + (int64_t)(h * 32 + t * 8 + l / 8) * g.lda + (row < g.m ? row : 0);
+        a[t][h] = static_cast<const E*>(g.a) + (int64_t)(h * 32 + t * 8 + l / 8) * g.lda + (row < last ? row : last);
       }
     }
 #pragma unroll
@@ -156,8 +157,9 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int y = 0; y < 8; ++y) sum += red[y][t][in / 16][(quad % 4) * 16 + in % 16];
-    const int row = row0 + quad * 4;
-    if (col >= g.n) continue;
+    int row = row0 + quad * 4;
+    if (col >= g.n || row0 + quad / 2 * 8 >= g.m) continue;
+    if (LA == MC && row0 + quad / 2 * 8 > last) row = last + quad % 2 * 4;
     float* at = out + (int64_t)col * g.m + row;
     if (g.m % 4 == 0 && row < g.m) *reinterpret_cast<f32x4*>(at) = sum;
     else

@@ -137,6 +137,14 @@ def test_lora_single_tokens(kind, pad, shift, m, n, k, rank):
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("pad, shift", [(0, 0), (1, 1), (8, 0)])
+@pytest.mark.parametrize("m", [1, 7, 8, 9, 12, 63, 65, 68, 127])
+def test_lora_few_tokens_and_rows_that_end_inside_a_chunk(kind, pad, shift, m):
+    for n in (2, 70):
+        Case(kind, m, n, 75, 5, 2, "NTT", pad, shift).run().check()
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
 @pytest.mark.parametrize("ops", ["TTT", "NNN"])
 @pytest.mark.parametrize("m, n, k, rank", [(1601, 130, 136, 100), (1600, 99, 520, 130)])
 def test_lora_few_tokens_and_large_ranks(kind, ops, m, n, k, rank):
