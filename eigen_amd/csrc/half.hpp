@@ -113,6 +113,14 @@ template <typename E, typename V> __device__ __forceinline__ V load_first(const 
   return v;
 }
 
+// Between the LDS accesses of a wave's lanes that meet each other's data: the hardware keeps a wave's accesses in order, and this makes
+// the compiler do so too (it reasons about one lane, whose own addresses may well differ).  No instruction.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // n <= 8 whole numbers of 8 bits from p (any alignment), the rest zero.
 __device__ __forceinline__ uint64_t load_bytes(const int8_t* p, int n) {
   uint64_t v = 0;

@@ -453,7 +453,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void half_gemm_kernel(HalfGemm g) 
         for (int t = 0; t < 4; ++t) v[t] = (E)a[t];
         *reinterpret_cast<x4*>(mine + (l & 15) * line + (i * 16 + (l / 16) * 4) * 2) = v;
       }
-      __builtin_amdgcn_wave_barrier();
+      wave_order();
       if (wide) {
         constexpr int per = CR / 8;                    // 16-byte chunks of a column
 #pragma unroll
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void half_gemm_kernel(HalfGemm g) 
           if (c < c_cols && r < c_rows) C[(int64_t)(g.order ? g.order[c] : c) * g.ldc + r] = v;
         }
       }
-      __builtin_amdgcn_wave_barrier();
+      wave_order();
     }
     return;
   }
@@ -527,7 +527,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void half_gemm_kernel(HalfGemm g) 
   for (int j = 0; j < CN; ++j) {
 #pragma unroll
     for (int i = 0; i < CR / 16; ++i) *reinterpret_cast<f32x4*>(mine + (l & 15) * line + (i * 16 + (l / 16) * 4) * 4) = block(i, j);
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
 #pragma unroll 1
     for (int b = 0; b < NB; ++b) {
       const int step = j * NB + b;
@@ -545,7 +545,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void half_gemm_kernel(HalfGemm g) 
         if (at) *at = v[t];
       }
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
   }
 }
 

@@ -175,8 +175,8 @@ HalfGemm gemm_args(const LoraArgs& c) {
   g.scale = c.scale;
   return g;
 }
-// Single precision has the few-token form for W with a contiguous reduction (there is no transposing read of 32-bit elements).
-bool few_f32(bool w_trans, int64_t m, int64_t n, int64_t k) { return w_trans && lora_few(true, m, n, k); }
+// (chunks of 4 rows have to exist)
+bool few_f32(bool w_trans, int64_t m, int64_t n, int64_t k) { return (w_trans || m >= 4) && lora_few(true, m, n, k); }
 
 template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArgs& q, hipStream_t s) {
   HalfGemm g = gemm_args(c);
@@ -470,7 +470,7 @@ hipError_t lora_device(const LoraArgs& c, hipStream_t s) {
   if (c.m > 0 && c.kind == F32 && few_f32(c.w_trans, c.m, c.n, c.k)) {
     HalfGemm g = gemm_args(c);
     g.partial = static_cast<float*>(c.work);
-    return lora_few_device(F32, true, g, p, s);
+    return lora_few_device(F32, c.w_trans, g, p, s);
   }
   if (c.m > 0 && c.kind == BF16) return launch_half<Bf16>(c, p, s);
   if (c.m > 0 && c.kind == F16K) return launch_half<F16>(c, p, s);

@@ -12,11 +12,13 @@ namespace eigamd {
 
 namespace {
 
+template <typename E, int N> using Part = E __attribute__((ext_vector_type(N)));
+
 // Y for few tokens, 16 NG of them a workgroup: the time is that of reading W, from as many compute units as there are.  A
 // workgroup owns 64 rows and one piece of the reduction, so that X, which every workgroup reads its piece of, costs little beside
 // W (with 16 rows and the whole reduction X was four times the traffic: 64 tokens x 4096 x 4096 took 22 us, now 12).  Its eight
 // waves share the piece, 64 (32) positions a turn, turned in the wave's own LDS (W's reduction contiguous: as a RowBlock; its rows: read
-// back transposed).  The sums go to memory in 32 bits; the second kernel adds the
+// back transposed, single precision one element at a time).  The sums go to memory in 32 bits; the second kernel adds the
 // pieces up and the low-rank part to them.
 // The projection needs nothing of this, so its workgroups (16 ranks each) are the first ones of the same launch.
 template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512) void lora_few_kernel(HalfGemm g, ProjectArgs q, int project, int slots) {
@@ -40,7 +42,9 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
   const int row0 = part % row_blocks * 64, z = part / row_blocks;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63;
   const int k_begin = z * g.k_piece, k_end = k_begin + g.k_piece < g.k ? k_begin + g.k_piece : g.k;
-  const int last = g.m < 8 ? 0 : g.m - 8;      // MC: a chunk of 8 rows that would pass the end holds the last 8, some of them twice
+  // MC: chunks of CH rows, one that would pass the end holds the last CH, some of them twice
+  constexpr int CH = T::bytes == 4 ? 4 : 8;
+  const int last = g.m < CH ? 0 : g.m - CH;
   const E* a[4][S];                   // KC: rows of the four row blocks; MC: chunks of 8 lines
   const E* b[NG][S];                  // rows and columns past the end repeat the last one and are not stored
 #pragma unroll
@@ -51,8 +55,8 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
         const int row = row0 + t * 16 + Block::row(h);
         a[t][h] = static_cast<const E*>(g.a) + (int64_t)(row < g.m ? row : g.m - 1) * g.lda;
       } else {
-        const int row = row0 + (l % 8) * 8;
-        a[t][h] = static_cast<const E*>(g.a) + (int64_t)(h * 32 + t * 8 + l / 8) * g.lda + (row < last ? row : last);
+        const int row = row0 + l % (64 / CH) * CH;
+        a[t][h] = static_cast<const E*>(g.a) + (int64_t)(h * 32 + t * 8 + l / (64 / CH)) * g.lda + (row < last ? row : last);
       }
     }
 #pragma unroll
@@ -75,11 +79,17 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
         if constexpr (LA == KC) {
           fa[t][h] = whole ? load_8<E, x8>(a[t][h] + k) : load_first<E, x8>(a[t][h] + (left > 0 ? k : 0), 1, left);
         } else {
-          const bool in = whole || k0 + h * 32 + t * 8 + l / 8 < k_end;
-          x8 v = load_8<E, x8>(in ? a[t][h] + (int64_t)k0 * g.lda : static_cast<const E*>(g.a));
+          // 16 bytes of a line; of single precision also of the line 4 further
+          constexpr int P = 8 / CH;
+          struct { Part<E, CH> part[P]; } v;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = in ? v[e] : (E)0.0f;
-          fa[t][h] = v;
+          for (int p = 0; p < P; ++p) {
+            const bool in = whole || k0 + h * 32 + t * 8 + p * 4 + l / (64 / CH) < k_end;
+            __builtin_memcpy(&v.part[p], in ? a[t][h] + (int64_t)(k0 + p * 4) * g.lda : static_cast<const E*>(g.a), 16);
+#pragma unroll
+            for (int e = 0; e < CH; ++e) v.part[p][e] = in ? v.part[p][e] : (E)0.0f;
+          }
+          fa[t][h] = __builtin_bit_cast(x8, v);
         }
       }
 #pragma unroll
@@ -89,6 +99,7 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
   auto multiply = [&](const x8(&fa)[4][S], const x8(&fb)[NG][S]) {
     char* mine = lds + w * (4 + NG) * Block::bytes;
     auto own = [&](int t) { return mine + t * Block::bytes; };
+    wave_order();
 #pragma unroll
     for (int h = 0; h < S; ++h) {
 #pragma unroll
@@ -101,11 +112,29 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
 #pragma unroll
     for (int h = 0; h < S; ++h) {
       x8 f[4], y[NG];
-      if constexpr (LA == MC) {
+      if (LA == KC && h == 0) wave_order();
+      if (LA == MC && h > 0) wave_order();
+      if constexpr (LA == MC && T::bytes == 4) {
+        // lines of 64 rows, 256 bytes, read back one element at a time; the four lines a wave reads together are turned by 16 rows
+        // against each other so that they meet all banks once
+        float* lines = reinterpret_cast<float*>(mine);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          struct { f32x4 part[2]; } v = __builtin_bit_cast(decltype(v), fa[t][h]);
+#pragma unroll
+          for (int p = 0; p < 2; ++p) *reinterpret_cast<f32x4*>(lines + (t * 8 + p * 4 + l / 16) * 64 + ((l % 16 * 4) ^ (t * 16))) = v.part[p];
+        }
+        wave_order();
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[t][e] = lines[(l / 16 * 8 + e) * 64 + ((t * 16 + l % 16) ^ (l / 16 * 16))];
+      } else if constexpr (LA == MC) {
         // lines of 64 rows, 128 bytes; chunks permuted so that the 8 lines a half wave reads meet all banks once
         auto slot = [](int line, int ch) { return line * 128 + (ch ^ (((line >> 1) & 1) | ((line >> 2) & 2)) << 1) * 16; };
 #pragma unroll
         for (int t = 0; t < 4; ++t) *reinterpret_cast<x8*>(mine + slot(t * 8 + l / 8, l % 8)) = fa[t][h];
+        wave_order();
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           union { x8 v; typename T::x4 h[2]; } u;
@@ -158,8 +187,9 @@ template <typename T, int LA, int NG, int FORM> __global__ __launch_bounds__(512
 #pragma unroll
     for (int y = 0; y < 8; ++y) sum += red[y][t][in / 16][(quad % 4) * 16 + in % 16];
     int row = row0 + quad * 4;
-    if (col >= g.n || row0 + quad / 2 * 8 >= g.m) continue;
-    if (LA == MC && row0 + quad / 2 * 8 > last) row = last + quad % 2 * 4;
+    const int chunk = row / CH * CH;      // (row0 is a multiple of 64)
+    if (col >= g.n || chunk >= g.m) continue;
+    if (LA == MC && chunk > last) row = last + row % CH;
     float* at = out + (int64_t)col * g.m + row;
     if (g.m % 4 == 0 && row < g.m) *reinterpret_cast<f32x4*>(at) = sum;
     else
@@ -388,7 +418,8 @@ template <typename T, int LA> hipError_t launch_few(HalfGemm g, const ProjectArg
 // and 5 + 4.4 per thousand positions a round, against the plan's time, 6 us and 1.25 per thousand positions for the projection
 // (256 tokens x 1024 x 1024 18.7 -> 10.4 us, 142 x 2456 x 4032 29.6 -> 17.9, 192 x 4096 x 4096 31.5 -> 25.1; not 96 x 4096 x 16384,
 // 62.5 -> 69.2).  Single precision: against the library's product, which has larger tiles still, up to two rounds (777 x 1024 x
-// 1536 72.6 -> 45.9 us, 1500 x 1000 x 2000 114 -> 108, 2048 x 2048 x 2048 180 -> 214).
+// 1536 72.6 -> 45.9 us, 1500 x 1000 x 2000 114 -> 108, 2048 x 2048 x 2048 180 -> 214; W not transposed 439 x 384 x 2048 50 -> 24, 1024 x
+// 2048 x 2048 111 -> 118).
 bool lora_few(bool f32, int64_t m, int64_t n, int64_t k) {
   if (n <= 64) return true;
   const int64_t blocks = (m + 63) / 64 * ((n + 63) / 64), project = n / kProjTokens;
@@ -405,7 +436,7 @@ int64_t lora_few_work_bytes(int64_t m, int64_t n, int64_t k) {
 }
 
 hipError_t lora_few_device(int kind, bool w_trans, const HalfGemm& g, const ProjectArgs& q, hipStream_t s) {
-  if (kind != BF16 && kind != F16K) return launch_few<Fp32, KC>(g, q, s);      // (W transposed only)
+  if (kind != BF16 && kind != F16K) return w_trans ? launch_few<Fp32, KC>(g, q, s) : launch_few<Fp32, MC>(g, q, s);
   if (kind == BF16) return w_trans ? launch_few<Bf16, KC>(g, q, s) : launch_few<Bf16, MC>(g, q, s);
   return w_trans ? launch_few<F16, KC>(g, q, s) : launch_few<F16, MC>(g, q, s);
 }

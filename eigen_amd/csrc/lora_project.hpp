@@ -121,6 +121,7 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
     auto multiply = [&](const x8(&fx)[2], const x8(&fa)[RT]) {
       char* mine = lds + w * (2 + RT) * RowBlock<T>::bytes;      // X's two blocks, then the factor's
       x8 f[RT], y[2];
+      wave_order();
 #pragma unroll
       for (int c = 0; c < 2; ++c) RowBlock<T>::put(mine + c * RowBlock<T>::bytes, fx[c]);
       char* own = mine + 2 * RowBlock<T>::bytes;
@@ -128,6 +129,7 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
         auto slot = [&](int ln, int ch) { return ln * line + ((ch ^ ((ln & 3) << 1)) & (per - 1)) * 16; };
 #pragma unroll
         for (int t = 0; t < RT; ++t) *reinterpret_cast<x8*>(own + slot((t * 64 + l) / per, (t * 64 + l) % per)) = fa[t];
+        wave_order();
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
           union { x8 v; typename T::x4 h[2]; } u;
@@ -139,9 +141,11 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
       } else if constexpr (FORM == A_K) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) RowBlock<T>::put(own + t * RowBlock<T>::bytes, fa[t]);
+        wave_order();
 #pragma unroll
         for (int t = 0; t < RT; ++t) f[t] = RowBlock<T>::get(own + t * RowBlock<T>::bytes);
       } else {
+        wave_order();
 #pragma unroll
         for (int t = 0; t < RT; ++t) f[t] = fa[t];
       }
