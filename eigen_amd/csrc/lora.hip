@@ -175,7 +175,7 @@ HalfGemm gemm_args(const LoraArgs& c) {
   g.scale = c.scale;
   return g;
 }
-// (chunks of 4 rows have to exist)
+// The few-token form in single precision; where W is not transposed, chunks of 4 rows have to exist.
 bool few_f32(bool w_trans, int64_t m, int64_t n, int64_t k) { return (w_trans || m >= 4) && lora_few(true, m, n, k); }
 
 template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArgs& q, hipStream_t s) {
