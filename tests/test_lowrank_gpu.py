@@ -536,7 +536,7 @@ def test_gradients_against_differences():
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
-@pytest.mark.parametrize("n", [24, 300])
+@pytest.mark.parametrize("n", [1, 24, 300, 4200])
 def test_captured_and_replayed(kind, n):
     """Plan, forward, checkpoint and gradients in one graph; new tokens and adapters before every replay."""
     c = Case(kind, 136, n, 264, 16, 4)
@@ -588,6 +588,32 @@ def test_two_streams_at_once_and_a_stream_of_ones_own():
     torch.cuda.synchronize()
     for c in cases:
         c.check()
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("n", [1, 40, 200])
+def test_gradients_on_two_streams_at_once(kind, n):
+    cases, streams = [Case(kind, 520, n, 264, 16, 3, seed=s) for s in (1, 50)], [torch.cuda.Stream() for _ in range(2)]
+    for c in cases:
+        c.run()
+    ck = [lowrank.ckpt8_pack_dev(c.X, lowrank.Checkpoint8(264, n, kind)) for c in cases]
+    outs = [(lowrank.MatrixStack(264, 16, 3, F32), DeviceMatrix(520, 264, F32)) for _ in cases]
+    def step(i, **more):
+        lowrank.lora_wgrad_dev("N", ck[i], cases[i].P, cases[i].S, cases[i].plan, 0.0, outs[i][0], **more)
+        lowrank.ckpt8_wgrad_dev("N", cases[i].Y, ck[i], 0.0, outs[i][1], **more)
+    want = []
+    for i in range(2):
+        step(i)
+        want.append([o.storage.clone() for o in outs[i]])
+        for o in outs[i]:
+            o.storage.zero_()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for i in range(2):
+            step(i, stream=streams[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o.storage, w) for o, w in zip(outs[i], want[i]))
 
 
 def test_an_offset_beyond_32_bits():
