@@ -61,16 +61,26 @@ template <typename T, int NP> __device__ __forceinline__ void split(float v, typ
   }
 }
 
-// Power of two that brings the largest of |v| into [2^13, 2^14), and its inverse (1 where that is zero or not finite).  The
-// second piece of an f16 value then stays clear of f16's subnormals for everything down to 2^-27 of the largest.
+// Power of two that brings the largest of |v| into [2^14, 2^15) (below it for what is smaller than 2^-112), and its inverse; 1 where that
+// is not finite.
 struct Norm {
   float down, up;
 };
 __device__ __forceinline__ Norm norm_of(float largest) {
   int e = (__float_as_int(largest) >> 23) & 255;
-  if (e == 255 || e == 0) return {1.0f, 1.0f};
-  e = e < 14 ? 14 : (e > 250 ? 250 : e);
-  return {__int_as_float((267 - e) << 23), __int_as_float((e - 13) << 23)};
+  if (e == 255) return {1.0f, 1.0f};
+  e = e < 15 ? 15 : e;
+  return {__int_as_float((268 - e) << 23), __int_as_float((e - 14) << 23)};
+}
+
+// The same in f16, 11 bits each, of a v below 2^15: the three hold all of v from 1/2 on, where its last bit is a whole multiple of f16's
+// smallest number, 2^-24.
+__device__ __forceinline__ void split_f16(float v, _Float16 (&piece)[3]) {
+  const bool finite = __builtin_fabsf(v) < __builtin_inff();
+  piece[0] = finite ? (_Float16)__builtin_amdgcn_cvt_pkrtz(v, 0.0f)[0] : (_Float16)v;
+  v = finite ? v - (float)piece[0] : 0.0f;
+  piece[1] = (_Float16)__builtin_amdgcn_cvt_pkrtz(v, 0.0f)[0];
+  piece[2] = (_Float16)(v - (float)piece[1]);
 }
 
 // 2^(e - 127) for an exponent byte.  255 gives infinity: a block that held infinities or NaN is stored as zeros with

@@ -288,12 +288,15 @@ template <typename T, int SRC> struct GradTile {
   }
 };
 
-// G_j over one piece of j's tokens: 256 rows x 16 RT ranks per workgroup, 32 tokens a turn.  p keeps (nearly) all of its 32 bits
-// as several 16-bit pieces; the sums are the matrix unit's 32 bits.  A run that is one piece goes straight to G_j.
+// G_j over one piece of j's tokens: 256 rows x 16 RT ranks per workgroup, 32 tokens a turn.  p keeps all of its 32 bits, as three 16-bit
+// pieces; the sums are the matrix unit's 32 bits.  A run that is one piece goes straight to G_j.
+// f16 has neither p's range nor room for three pieces of what is far below the largest: a turn's p is normalised rank by rank, and a wave
+// that holds a p below 2^-16 of its rank's largest (one turn in fifty of normally distributed p) takes that turn's products in single
+// precision, six times the work.
 template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(256) void lora_grad_kernel(GradArgs g) {
   using E = typename T::elem;
   using x8 = typename T::x8;
-  constexpr int NP = T::bytes == 4 ? 1 : (__is_same(T, Bf16) ? 3 : 2);
+  constexpr int NP = T::bytes == 4 ? 1 : 3;
   if ((int)blockIdx.y >= g.slots) {
     // an adapter without tokens gets beta G_j
     const int j = blockIdx.y - g.slots;
@@ -312,27 +315,11 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
   using Tile = GradTile<T, SRC>;
   __shared__ __align__(1024) char lds[2 * Tile::bytes];
   __shared__ int tok[1024 + 32];
-  __shared__ float tops[4];
   const int count = piece.end - piece.begin, turns = (count + 31) / 32;
   const int w = threadIdx.x / 64, l = threadIdx.x & 63;
   const int row0 = blockIdx.x * kGradRows, r0 = blockIdx.z * 64;
   for (int i = threadIdx.x; i < turns * 32; i += 256) tok[i] = i < count ? g.order[piece.begin + i] : -1;
   __syncthreads();
-  Norm nm = {1.0f, 1.0f};
-  if constexpr (__is_same(T, F16)) {
-    // one power of two for the piece's p, so that f16 pieces neither overflow nor vanish
-    float top = 0.0f;
-    const int width = g.rank - r0 < RT * 16 ? g.rank - r0 : RT * 16;
-    for (int i = threadIdx.x; i < count * width; i += 256) {
-      const float v = __builtin_fabsf(g.p[(int64_t)tok[i / width] * g.ldp + r0 + i % width]);
-      top = v < __builtin_inff() ? fmaxf(top, v) : top;
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    if (l == 0) tops[w] = top;
-    __syncthreads();
-    nm = norm_of(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-  }
   Tile tile;
   // RT waves beside each other take 16 ranks each (every wave then makes the pieces of its own p only), 4 / RT one behind the
   // other 64 RT rows each
@@ -360,22 +347,58 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
       tile.load(next, g, tok + (s + 1) * 32, row0);
     }
     x8 fp[NP];
+    auto product = [&](x8 fu, f32x4 sum) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if constexpr (NP == 1) {
-        fp[0][e] = pv[e];
-      } else {
+      for (int z = NP - 1; z >= 0; --z) sum = TRANS ? T::mma(fp[z], fu, sum) : T::mma(fu, fp[z], sum);
+      return sum;
+    };
+    if constexpr (__is_same(T, F16)) {
+      float top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = __builtin_fabsf(pv[e]) < __builtin_inff() ? fmaxf(top, __builtin_fabsf(pv[e])) : top;
+      top = fmaxf(top, __shfl_xor(top, 16));      // (lanes l, l + 16, ... hold the same rank)
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const Norm nm = norm_of(top);
+      bool small = false;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = pv[e] * nm.down;
+        small |= pv[e] != 0.0f && __builtin_fabsf(v) < 0.5f;
         E q[NP];
-        split<T, NP>(pv[e] * nm.down, q);
+        split_f16(v, q);
 #pragma unroll
         for (int z = 0; z < NP; ++z) fp[z][e] = q[z];
       }
-    }
+      if (__builtin_expect(__any(small), 0)) {
+        Fp32::x8 p;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const x8 fu = Tile::fragment(here, wr + i * 16);
+        for (int e = 0; e < 8; ++e) p[e] = pv[e];
 #pragma unroll
-      for (int z = NP - 1; z >= 0; --z) acc[i] = TRANS ? T::mma(fp[z], fu, acc[i]) : T::mma(fu, fp[z], acc[i]);
+        for (int i = 0; i < NI; ++i) {
+          const Fp32::x8 u = __builtin_convertvector(Tile::fragment(here, wr + i * 16), Fp32::x8);
+          acc[i] = TRANS ? Fp32::mma(p, u, acc[i]) : Fp32::mma(u, p, acc[i]);
+        }
+      } else {
+        f32x4 up;      // of the ranks of a lane's four results
+#pragma unroll
+        for (int t = 0; t < 4; ++t) up[t] = TRANS ? __shfl(nm.up, (l / 16) * 4 + t) : nm.up;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) acc[i] += up * product(Tile::fragment(here, wr + i * 16), f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (NP == 1) {
+          fp[0][e] = pv[e];
+        } else {
+          E q[NP];
+          split<T, NP>(pv[e], q);
+#pragma unroll
+          for (int z = 0; z < NP; ++z) fp[z][e] = q[z];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) acc[i] = product(Tile::fragment(here, wr + i * 16), acc[i]);
     }
     if (s + 1 < turns) tile.store(next);
     __syncthreads();
@@ -395,7 +418,7 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
     const int fast = (TRANS ? rank0 : top) + (l / 16) * 4, slow = (TRANS ? top : rank0) + (l & 15);
     if (slow >= (TRANS ? g.rows : g.rank)) continue;
     float* at = out + (int64_t)slow * ld + fast;
-    f32x4 v = acc[i] * nm.up * sj;
+    f32x4 v = acc[i] * sj;
     if (wide && fast + 4 <= limit) {
       // (one by one, four times as many addresses for the memory pipeline: 40 tokens x 1024, rank 64 16 us, now 7.7)
       if (beta != 0.0f) v += beta * *reinterpret_cast<const f32x4*>(at);
