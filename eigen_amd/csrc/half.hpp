@@ -42,22 +42,32 @@ struct Fp32 {
   }
 };
 
-// A float as a sum of NP values of the 16-bit type: each piece takes the leading bits of what is left.  Two pieces of a
-// normalised v leave 2^-17 (bf16) or 2^-23 (f16) of it out.  Three bf16 pieces hold all 24 bits of any finite v: they are cut,
-// not rounded, 8 bits each (rounding up could leave the range).  What is not finite stays in the first piece (a difference of
-// infinities would be a NaN).
-template <typename T, int NP> __device__ __forceinline__ void split(float v, typename T::elem (&piece)[NP]) {
+// A float as a sum of three bf16 values, each the leading 8 bits of what is left: they hold all 24 bits of any finite v.  They are cut,
+// not rounded (rounding up could leave the range).  What is not finite stays in the first piece (a difference of infinities would be a
+// NaN).
+__device__ __forceinline__ void split_bf16(float v, __bf16 (&piece)[3]) {
   const bool finite = __builtin_fabsf(v) < __builtin_inff();
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    if constexpr (__is_same(T, Bf16) && NP == 3) {
-      const float cut = finite ? __int_as_float(__float_as_int(v) & 0xffff0000) : v;
-      piece[i] = (typename T::elem)cut;
-      v = finite ? v - cut : 0.0f;
-    } else {
-      piece[i] = (typename T::elem)v;
-      v = finite ? v - (float)piece[i] : 0.0f;
-    }
+  for (int i = 0; i < 3; ++i) {
+    const float cut = finite ? __int_as_float(__float_as_int(v) & 0xffff0000) : v;
+    piece[i] = (__bf16)cut;
+    v = finite ? v - cut : 0.0f;
+  }
+}
+
+// Eight f16 values as two bf16 ones each, 8 and 3 of their 11 bits (cut in f16, where the difference is exact; what the floats have in
+// their upper halves is all of them).
+__device__ __forceinline__ void split_f16_to_bf16(F16::x8 v, Bf16::x8 (&piece)[2]) {
+  using u16x8 = uint16_t __attribute__((ext_vector_type(8)));
+  using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
+  const F16::x8 high = __builtin_bit_cast(F16::x8, __builtin_bit_cast(u16x8, v) & (uint16_t)0xfff8);
+  const F16::x8 part[2] = {high, v - high};
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+    u32x4 out;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) out[t] = __builtin_amdgcn_perm(__float_as_uint((float)part[z][2 * t + 1]), __float_as_uint((float)part[z][2 * t]), 0x07060302u);
+    piece[z] = __builtin_bit_cast(Bf16::x8, out);
   }
 }
 
@@ -73,7 +83,7 @@ __device__ __forceinline__ Norm norm_of(float largest) {
   return {__int_as_float((268 - e) << 23), __int_as_float((e - 14) << 23)};
 }
 
-// The same in f16, 11 bits each, of a v below 2^15: the three hold all of v from 1/2 on, where its last bit is a whole multiple of f16's
+// Three f16 values in the same way, 11 bits each, of a v below 2^15: they hold all of v from 1/2 on, where its last bit is a whole multiple of f16's
 // smallest number, 2^-24.
 __device__ __forceinline__ void split_f16(float v, _Float16 (&piece)[3]) {
   const bool finite = __builtin_fabsf(v) < __builtin_inff();

@@ -168,8 +168,8 @@ template <typename T, int LAY, int R, int NT, bool GATHER> struct SliceLoader {
 
 // Adds s_j up_j P to a wave's sums: column by column of the batch, only where the column belongs to j (an infinity or NaN in
 // one adapter's factor must not reach another request's column, so the products are selected, not multiplied by zero).
-// P has 32 bits and goes through the matrix unit as two 16-bit pieces per value, normalised per token and 32 ranks: 16 bits
-// of it (bf16) or 22 (f16) take part, more than the result's type keeps.
+// P goes through the matrix unit as three bf16 pieces per value, which hold all of its 32 bits.  An f16 factor becomes two bf16 pieces,
+// which hold all of its 11 bits: f16 has neither P's range nor room for the last pieces of a small one.
 // Per 32 ranks, P's fragments do not depend on the adapter; of the adapters' factors the next one's are under way while one is
 // multiplied.
 template <typename T, int NI, int NJ>
@@ -177,12 +177,14 @@ __device__ __forceinline__ void add_adapters(const HalfGemm& g, int row0, int co
   using E = typename T::elem;
   using x8 = typename T::x8;
   using f32x8 = float __attribute__((ext_vector_type(8)));
+  using M = std::conditional_t<T::bytes == 4, Fp32, Bf16>;      // what the unit multiplies
+  constexpr int NP = T::bytes == 4 ? 1 : 3, NU = __is_same(T, F16) ? 2 : 1;
   const int l = threadIdx.x & 63;
   const int col = col0 + l;
   const int mine = l < NJ * 16 && col < g.n ? g.seg[col] : g.none;
   const unsigned long long live = __ballot(mine != g.none);
   if (!live) return;
-  int64_t token[NJ];
+  int token[NJ];
   float scale[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
@@ -206,38 +208,27 @@ __device__ __forceinline__ void add_adapters(const HalfGemm& g, int row0, int co
       for (int t = 0; t < 8; ++t) u[t] = rn > 0 ? u[t] : (E)0.0f;
       return u;
     };
-    x8 hi[NJ], lo[NJ];
-    float back[NJ];
+    typename M::x8 part[NP][NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      const float* at = g.p + token[j] * g.ldp + r;
-      f32x8 v = chunks ? load_8<float, f32x8>(at) : load_first<float, f32x8>(at, 1, rn);
+      const float* at = g.p + (int64_t)token[j] * g.ldp + r;
+      const f32x8 v = chunks ? load_8<float, f32x8>(at) : load_first<float, f32x8>(at, 1, rn);
 #pragma unroll
-      for (int t = 0; t < 8; ++t) v[t] = rn > 0 ? v[t] : 0.0f;
-      if constexpr (T::bytes == 4) {
-        back[j] = scale[j];
+      for (int t = 0; t < 8; ++t) {
+        const float p = rn > 0 ? v[t] : 0.0f;
+        if constexpr (NP == 1) {
+          part[0][j][t] = p;
+        } else {
+          __bf16 piece[NP];
+          split_bf16(p, piece);
 #pragma unroll
-        for (int t = 0; t < 8; ++t) hi[j][t] = v[t];
-      } else {
-        float top = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 8; ++t) top = fmaxf(top, __builtin_fabsf(v[t]));
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const Norm nm = norm_of(top);
-        back[j] = nm.up * scale[j];
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          E piece[2];
-          split<T, 2>(v[t] * nm.down, piece);
-          hi[j][t] = piece[0];
-          lo[j][t] = piece[1];
+          for (int z = 0; z < NP; ++z) part[z][j][t] = piece[z];
         }
       }
     }
-    // Four row blocks' factors under way together; those of the next adapter while this one's are multiplied, if they are all (the
-    // large tile has no registers for that).
-    constexpr int GI = NI < 4 ? NI : 4;
+    // Four row blocks' factors under way together, two in the large tile, which has no registers for more; those of the next adapter while
+    // this one's are multiplied, if they are all.
+    constexpr int GI = NI < 4 ? NI : NI == 4 ? 4 : 2;
     constexpr bool AHEAD = NI == GI;
     unsigned long long left = live;
     int who = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
@@ -259,15 +250,20 @@ __device__ __forceinline__ void add_adapters(const HalfGemm& g, int row0, int co
         }
 #pragma unroll
         for (int i = 0; i < GI; ++i) {
+          typename M::x8 f[NU];
+          if constexpr (NU == 1) f[0] = u[i];
+          else split_f16_to_bf16(u[i], f);
 #pragma unroll
           for (int j = 0; j < NJ; ++j) {
             if (!((mask >> (j * 16)) & 0xffff)) continue;
             f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (T::bytes == 2) d = T::mma(u[i], lo[j], d);
-            d = T::mma(u[i], hi[j], d);
+#pragma unroll
+            for (int z = NP - 1; z >= 0; --z)
+#pragma unroll
+              for (int y = NU - 1; y >= 0; --y) d = M::mma(f[y], part[z][j], d);
             const bool on = (mask >> (j * 16 + (l & 15))) & 1;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) acc[i0 + i][j][t] += on ? d[t] * back[j] : 0.0f;
+            for (int t = 0; t < 4; ++t) acc[i0 + i][j][t] += on ? d[t] * scale[j] : 0.0f;
           }
           if (AHEAD && more) u[i] = factor(next, i);
         }

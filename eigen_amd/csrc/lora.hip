@@ -392,7 +392,7 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
           fp[0][e] = pv[e];
         } else {
           E q[NP];
-          split<T, NP>(pv[e], q);
+          split_bf16(pv[e], q);
 #pragma unroll
           for (int z = 0; z < NP; ++z) fp[z][e] = q[z];
         }

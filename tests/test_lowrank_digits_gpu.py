@@ -5,8 +5,8 @@ import torch
 import eigen_amd
 from eigen_amd import lowrank
 import lowrank_ref as ref
-from lowrank_ref import KINDS, NAME
-from test_lowrank_gpu import Grad, store
+from lowrank_ref import KINDS, NAME, TORCH
+from test_lowrank_gpu import Case, Grad, rand, store, store_stack, turned
 
 pytestmark = pytest.mark.gpu
 F32, BF16, F16 = eigen_amd.F32, eigen_amd.BF16, eigen_amd.F16
@@ -57,3 +57,66 @@ def test_gradients_of_projections_at_both_ends_of_floats_range(kind, opg):
         g, ga = ref.wgrad(c.u.cuda(), c.p.cuda(), c.scale.double().cuda(), c.ids.cuda(), 2)
         c.run()
         assert bool(((c.got().double() - g).abs() <= ref.wgrad_tolerance(c.n, g, ga)).all())
+
+
+# ------------------------------------------------------------------------------------------ the low-rank part of the product
+def whole_numbers(shape, low, high, seed):
+    return torch.randint(low, high + 1, shape, generator=torch.Generator().manual_seed(seed)).double()
+
+
+# tiles of 256 x 256 and 128 x 128, a split reduction, extents that are copied first, the matrix-unit join of few tokens, and the
+# joins that do without
+SIZES = [(256 * 15 + 8, 256 * 14 + 37, 200, 16), (1100, 1130, 200, 40), (1101, 1130, 203, 7), (1096, 1130, 1288, 16), (1601, 130, 136, 100),
+         (130, 70, 200, 33), (40, 17, 136, 16), (24, 1, 200, 4)]
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("opw", "TN")
+@pytest.mark.parametrize("m, n, k, rank", SIZES)
+def test_the_low_rank_part_uses_all_of_p(kind, opw, m, n, k, rank):
+    """Whole numbers, so that every sum is exact in 32 bits: P has 19 to 22 bits, neighbouring ranks of it differ by one entry of x and
+    enter with opposite signs, and what is left has to be right to the last bit.  (P is about 255 / 2 * 31 / 2 * k, and half of the pairs of ranks
+    take part: below 2^24 in every case.)"""
+    c = Case(kind, m, n, k, rank, 3, opw + "TT")
+    c.x = whole_numbers((k, n), 0, 255, 1)
+    c.a = whole_numbers((3, rank, k), 0, 31, 2)
+    c.b = torch.zeros(3, m, rank).double()
+    pairs = rank // 2
+    c.a[:, 1:2 * pairs:2] = c.a[:, 0:2 * pairs:2]
+    for r in range(pairs):
+        c.a[:, 2 * r + 1, (7 * r) % k] += 1
+    some = whole_numbers((3, m, pairs), 0, 1, 3)
+    c.b[:, :, 0:2 * pairs:2], c.b[:, :, 1:2 * pairs:2] = some, -some
+    c.w = torch.zeros(m, k).double()
+    c.w[:, ::16] = whole_numbers((m, (k + 15) // 16), -1, 1, 4)
+    c.scale = torch.tensor([0.5, 1.0, -0.25])
+    c.S = c.scale.cuda()
+    c.W, c.X = store(turned(c.w, opw), kind), store(c.x, kind)
+    c.A, c.B = store_stack(turned(c.a, "T"), kind), store_stack(turned(c.b, "T"), kind)
+    c.run()
+    d = [t.cuda() for t in (c.w, c.x, c.a, c.b)]
+    y, p, _, _ = ref.lora(*d, c.scale.double().cuda(), c.ids.cuda())
+    assert torch.equal(c.P.as_strided().double(), p)
+    assert torch.equal(c.Y.as_strided(), y.to(TORCH[kind]))
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("m, n, k, rank", [(256 * 15 + 8, 256 * 14 + 37, 72, 12), (1100, 1130, 72, 40), (1601, 130, 136, 100), (130, 70, 72, 9)])
+def test_quiet_ranks_beside_loud_ones_reach_y(kind, m, n, k, rank):
+    """P of ranks 2^29 apart: the loud ones meet zeros, and a scale brings the quiet ones back."""
+    c = Case(kind, m, n, k, rank, 2, "TTT")
+    quiet = (torch.arange(rank) % 3 > 0).double()
+    c.a = (rand(c.a.shape, kind, 31) * 2.0 ** (13.0 - 29.0 * quiet).unsqueeze(1)).to(TORCH[kind]).double()
+    c.x = (c.x * 2.0 ** (torch.arange(n) % 3 - 1.0)).to(TORCH[kind]).double()
+    c.b = c.b * quiet
+    c.w = torch.zeros_like(c.w)
+    c.scale = torch.tensor([2.0 ** 9, 2.0 ** 10])
+    c.S = c.scale.cuda()
+    c.W, c.X = store(turned(c.w, "T"), kind), store(c.x, kind)
+    c.A, c.B = store_stack(turned(c.a, "T"), kind), store_stack(turned(c.b, "T"), kind)
+    c.run()
+    y, p, ya, pa = ref.lora(*[t.cuda() for t in (c.w, c.x, c.a, c.b)], c.scale.double().cuda(), c.ids.cuda())
+    # as lora_tolerance, but nothing of P left out: k + rank products in 32 bits, and the one rounding
+    tol = ref.HALF[kind] * y.abs() + (2 * k + rank + 32) * 2.0 ** -23 * ya * (1 + ref.HALF[kind]) + ref.SMALL[kind]
+    err = (c.Y.as_strided().double() - y).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
