@@ -43,16 +43,14 @@ struct Fp32 {
 };
 
 // A float as a sum of three bf16 values, each the leading 8 bits of what is left: they hold all 24 bits of any finite v.  They are cut,
-// not rounded (rounding up could leave the range).  What is not finite stays in the first piece (a difference of infinities would be a
-// NaN).
+// not rounded (rounding up could leave the range).  An infinity or NaN stays in the first piece (a difference of infinities would be a
+// NaN).  Pieces may be zero, and an infinity times them is a NaN: who multiplies them looks for NaN and takes v itself then.
+__device__ __forceinline__ float upper_half(float v) { return __int_as_float(__float_as_int(v) & 0xffff0000); }
 __device__ __forceinline__ void split_bf16(float v, __bf16 (&piece)[3]) {
-  const bool finite = __builtin_fabsf(v) < __builtin_inff();
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    const float cut = finite ? __int_as_float(__float_as_int(v) & 0xffff0000) : v;
-    piece[i] = (__bf16)cut;
-    v = finite ? v - cut : 0.0f;
-  }
+  const float first = upper_half(v), left = __builtin_fabsf(v) < __builtin_inff() ? v - first : 0.0f, second = upper_half(left);
+  piece[0] = (__bf16)first;
+  piece[1] = (__bf16)second;
+  piece[2] = (__bf16)(left - second);
 }
 
 // Eight f16 values as two bf16 ones each, 8 and 3 of their 11 bits (cut in f16, where the difference is exact; what the floats have in
@@ -83,14 +81,13 @@ __device__ __forceinline__ Norm norm_of(float largest) {
   return {__int_as_float((268 - e) << 23), __int_as_float((e - 14) << 23)};
 }
 
-// Three f16 values in the same way, 11 bits each, of a v below 2^15: they hold all of v from 1/2 on, where its last bit is a whole multiple of f16's
+// Three f16 values, 11 bits each, of a v below 2^15: they hold all of v from 1/2 on, where its last bit is a whole multiple of f16's
 // smallest number, 2^-24.
 __device__ __forceinline__ void split_f16(float v, _Float16 (&piece)[3]) {
-  const bool finite = __builtin_fabsf(v) < __builtin_inff();
-  piece[0] = finite ? (_Float16)__builtin_amdgcn_cvt_pkrtz(v, 0.0f)[0] : (_Float16)v;
-  v = finite ? v - (float)piece[0] : 0.0f;
-  piece[1] = (_Float16)__builtin_amdgcn_cvt_pkrtz(v, 0.0f)[0];
-  piece[2] = (_Float16)(v - (float)piece[1]);
+  piece[0] = (_Float16)__builtin_amdgcn_cvt_pkrtz(v, 0.0f)[0];
+  const float left = __builtin_fabsf(v) < __builtin_inff() ? v - (float)piece[0] : 0.0f;
+  piece[1] = (_Float16)__builtin_amdgcn_cvt_pkrtz(left, 0.0f)[0];
+  piece[2] = (_Float16)(left - (float)piece[1]);
 }
 
 // 2^(e - 127) for an exponent byte.  255 gives infinity: a block that held infinities or NaN is stored as zeros with

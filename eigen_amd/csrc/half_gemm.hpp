@@ -173,7 +173,7 @@ template <typename T, int LAY, int R, int NT, bool GATHER> struct SliceLoader {
 // Per 32 ranks, P's fragments do not depend on the adapter; of the adapters' factors the next one's are under way while one is
 // multiplied.
 template <typename T, int NI, int NJ>
-__device__ __forceinline__ void add_adapters(const HalfGemm& g, int row0, int col0, f32x4 (&acc)[NI][NJ]) {
+__device__ __forceinline__ void adapters_in_pieces(const HalfGemm& g, int row0, int col0, f32x4 (&acc)[NI][NJ]) {
   using E = typename T::elem;
   using x8 = typename T::x8;
   using f32x8 = float __attribute__((ext_vector_type(8)));
@@ -270,6 +270,63 @@ __device__ __forceinline__ void add_adapters(const HalfGemm& g, int row0, int co
       }
       if (!more) break;
       who = next;
+    }
+  }
+}
+
+// The same in single precision, one block after the other: few registers beside the sums (and no addresses kept for the blocks).
+template <typename T, int NI, int NJ>
+__device__ __forceinline__ void adapters_in_single(const HalfGemm& g, int row0, int col0, f32x4 (&acc)[NI][NJ]) {
+  using E = typename T::elem;
+  const int l = threadIdx.x & 63;
+  const int mine = l < NJ * 16 && col0 + l < g.n ? g.seg[col0 + l] : g.none;
+  unsigned long long left = __ballot(mine != g.none);
+  while (left) {
+    const int who = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+    const unsigned long long mask = __ballot(mine == who);
+    left &= ~mask;
+    const float scale = g.scale[who];
+    const E* factor = static_cast<const E*>(g.up) + (int64_t)who * g.up_stride;
+    for (int r0 = 0; r0 < g.rank; r0 += 32) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          int lane = l;
+          asm volatile("" : "+v"(lane));
+          const int r = r0 + (lane / 16) * 8 < g.rank ? r0 + (lane / 16) * 8 : 0, rn = g.rank - r0 - (lane / 16) * 8;
+          const int c = col0 + j * 16 + (lane & 15), row = row0 + i * 16 + (lane & 15);
+          const Fp32::x8 p = load_first<float, Fp32::x8>(g.p + (int64_t)g.order[c < g.n ? c : g.n - 1] * g.ldp + r, 1, rn);
+          const typename T::x8 u = load_first<E, typename T::x8>(factor + (int64_t)(row < g.m ? row : g.m - 1) * g.up_row + (int64_t)r * g.up_rank, g.up_rank, rn);
+          const f32x4 d = Fp32::mma(__builtin_convertvector(u, Fp32::x8), p, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+          const bool on = (mask >> (j * 16 + (lane & 15))) & 1;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) acc[i][j][t] += on ? d[t] * scale : 0.0f;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+  }
+}
+
+// Into sums that are still zero.  A product of an infinity and a piece that is zero is a NaN, where the value's own product is an
+// infinity: where a NaN has come up it is all done again in single precision.
+template <typename T, int NI, int NJ>
+__device__ __forceinline__ void add_adapters(const HalfGemm& g, int row0, int col0, f32x4 (&acc)[NI][NJ]) {
+  adapters_in_pieces<T>(g, row0, col0, acc);
+  if constexpr (T::bytes == 2) {
+    f32x4 all = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) all += acc[i][j];
+    const float sum = (all[0] + all[1]) + (all[2] + all[3]);
+    if (__builtin_expect(__any(sum != sum), 0)) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      adapters_in_single<T>(g, row0, col0, acc);
     }
   }
 }

@@ -293,7 +293,10 @@ template <typename T, int SRC> struct GradTile {
 // f16 has neither p's range nor room for three pieces of what is far below the largest: a turn's p is normalised rank by rank, and a wave
 // that holds a p below 2^-16 of its rank's largest (one turn in fifty of normally distributed p) takes that turn's products in single
 // precision, six times the work.
-template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(256) void lora_grad_kernel(GradArgs g) {
+// The product of an infinity and a piece of p that is zero is a NaN, where that with p is an infinity: where a NaN has come up, a wave's
+// sums are made again in single precision, from memory as it is.
+// (Three waves a SIMD: left to itself the compiler takes two registers too many for rank 64 from a checkpoint, 45 -> 48 us.)
+template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(256, __is_same(T, Bf16) ? 3 : 1) void lora_grad_kernel(GradArgs g) {
   using E = typename T::elem;
   using x8 = typename T::x8;
   constexpr int NP = T::bytes == 4 ? 1 : 3;
@@ -404,6 +407,35 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < 8; ++e) pv[e] = pn[e];
+  }
+  if constexpr (T::bytes == 2) {
+    f32x4 all = acc[0];
+#pragma unroll
+    for (int i = 1; i < NI; ++i) all += acc[i];
+    const float sum = (all[0] + all[1]) + (all[2] + all[3]);
+    if (__builtin_expect(__any(sum != sum), 0)) {
+      auto value = [&](int token, int row) {
+        if (token < 0 || row >= g.rows) return 0.0f;
+        if constexpr (SRC == QUANT) return static_cast<const int8_t*>(g.u)[token * g.ldu + row] * exponent_scale(g.exponents[token * g.lde + row / 32]);
+        else return (float)static_cast<const E*>(g.u)[token * g.ldu + row];
+      };
+#pragma unroll
+      for (int i = 0; i < NI; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+      for (int s = 0; s < turns; ++s) {
+        load_p(pv, s);
+        Fp32::x8 p, u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = pv[e];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) u[e] = value(tok[s * 32 + (l / 16) * 8 + e], row0 + wr + i * 16 + (l & 15));
+          acc[i] = TRANS ? Fp32::mma(p, u, acc[i]) : Fp32::mma(u, p, acc[i]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
   }
   const bool whole = piece.run_end - piece.run_begin <= g.chunk;
   const float sj = whole ? g.scale[piece.adapter] : 1.0f;

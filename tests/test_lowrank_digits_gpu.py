@@ -1,4 +1,4 @@
-"""What the 16-bit forms of the adapter operators keep of P's 32 bits."""
+"""What the 16-bit forms of the adapter operators keep of P's 32 bits, and what they make of infinities."""
 import pytest
 import torch
 
@@ -120,3 +120,70 @@ def test_quiet_ranks_beside_loud_ones_reach_y(kind, m, n, k, rank):
     tol = ref.HALF[kind] * y.abs() + (2 * k + rank + 32) * 2.0 ** -23 * ya * (1 + ref.HALF[kind]) + ref.SMALL[kind]
     err = (c.Y.as_strided().double() - y).abs()
     assert bool((err <= tol).all()), float((err - tol).max())
+
+
+# --------------------------------------------------------------------------------------------------------------- infinities
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("opw", "TN")
+@pytest.mark.parametrize("m, n, k, rank", [(1100, 1130, 72, 20), (1601, 130, 136, 100), (72, 40, 72, 9), (24, 1, 72, 9)])
+def test_an_infinite_factor_gives_an_infinity_of_the_right_sign(kind, opw, m, n, k, rank):
+    c = Case(kind, m, n, k, rank, 2, opw + "TT", ids=[i % 2 for i in range(n)])
+    c.a[0, 3] = 0.0
+    c.a[0, 3, 5] = 1.0                       # p of rank 3 is one entry of x: a few bits, the other pieces of it are empty
+    c.x[5] = torch.where(torch.arange(n) % 4 < 2, 1.0, -1.5).double()
+    c.A, c.X = store_stack(turned(c.a, "T"), kind), store(c.x, kind)
+    c.b[0, 2, 3] = float("inf")
+    c.b[0, 7, 4] = float("-inf")
+    c.B = store_stack(turned(c.b, "T"), kind)
+    c.run()
+    on = c.ids.cuda() == 0
+    y, p = c.Y.as_strided().double(), c.P.as_strided().double()
+    assert torch.equal(y[2][on], torch.sign(p[3][on]) * float("inf") * float(c.scale[0]))
+    assert torch.equal(y[7][on], -torch.sign(p[4][on]) * float("inf") * float(c.scale[0]))
+    rest = torch.ones_like(y, dtype=torch.bool)
+    rest[2, on] = rest[7, on] = False
+    assert bool(torch.isfinite(y[rest]).all())
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("opw", "TN")
+@pytest.mark.parametrize("m, n, k, rank", [(1100, 1130, 72, 20), (1601, 130, 136, 100), (72, 40, 72, 9), (24, 1, 72, 9)])
+def test_an_infinite_projection_gives_infinities_of_the_right_sign(kind, opw, m, n, k, rank):
+    c = Case(kind, m, n, k, rank, 2, opw + "TT", ids=[i % 2 for i in range(n)])
+    c.a[0, 3, 5] = float("-inf")
+    c.b[0, ::3, 3] = 0.5                     # (few bits, as above)
+    c.b[0, 1, 3], c.b[0, 4, 3] = 0.0, float("inf")
+    c.A, c.B = store_stack(turned(c.a, "T"), kind), store_stack(turned(c.b, "T"), kind)
+    c.run()
+    on = c.ids.cuda() == 0
+    y, p = c.Y.as_strided().double(), c.P.as_strided().double()
+    assert torch.equal(p[3][on], (-torch.sign(c.x[5]) * float("inf")).cuda()[on]) and bool(torch.isfinite(p[:, ~on]).all())
+    want = torch.sign(c.b[0, :, 3]).cuda().unsqueeze(1) * p[3][on]            # 0 * inf: NaN
+    got = y[:, on]
+    assert torch.equal(torch.nan_to_num(got, nan=7.0, posinf=1.0, neginf=-1.0), torch.nan_to_num(want, nan=7.0, posinf=1.0, neginf=-1.0))
+    assert bool(torch.isfinite(y[:, ~on]).all())
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("opg", "NT")
+@pytest.mark.parametrize("spread", [0.0, 40.0])
+def test_an_infinite_gradient_gives_an_infinity_of_the_right_sign(kind, opg, spread):
+    """u of +-infinity: G's row is +-infinity by the sign of p (NaN where p is 0); and the other way round."""
+    c = Grad(kind, 72, 90, 20, 1, opg, ids=[0] * 90)
+    c.scale = torch.ones(1)
+    c.p[:, 4] = torch.where(torch.arange(20) % 2 == 0, 1.0, -3.0).double()      # a few bits of 24
+    c.p[7, 4] = 0.0
+    c.p[:, 5:] *= 2.0 ** spread
+    c.p[3, 8] = float("-inf")
+    c.u[11, 4] = float("inf")
+    c.u[5, 8] = 0.0
+    c.P, c.U = store(c.p, F32), store(c.u, kind)
+    c.run()
+    got = c.got()[0].double().cpu()
+    want = torch.sign(c.p[:, 4]) * float("inf")          # (0 * inf: NaN)
+    other = torch.arange(20) != 3
+    assert torch.equal(torch.nan_to_num(got[11][other], nan=7.0, posinf=1.0, neginf=-1.0), torch.nan_to_num(want[other], nan=7.0, posinf=1.0, neginf=-1.0))
+    rows = torch.arange(72) != 11
+    column = -torch.sign(c.u[:, 8]) * float("inf")       # rank 3: p of token 8 is -infinity, u of row 5 is 0 there
+    assert torch.equal(torch.nan_to_num(got[rows, 3], nan=7.0, posinf=1.0, neginf=-1.0), torch.nan_to_num(column[rows], nan=7.0, posinf=1.0, neginf=-1.0))
+    assert bool(torch.isfinite(got[rows][:, other]).all())
