@@ -274,16 +274,17 @@ __device__ __forceinline__ void adapters_in_pieces(const HalfGemm& g, int row0, 
   }
 }
 
-// The same in single precision, one block after the other: few registers beside the sums (and no addresses kept for the blocks).
+// The same in single precision for some of the columns, one block after the other: few registers beside the sums (and no addresses kept
+// for the blocks).
 template <typename T, int NI, int NJ>
-__device__ __forceinline__ void adapters_in_single(const HalfGemm& g, int row0, int col0, f32x4 (&acc)[NI][NJ]) {
+__device__ __forceinline__ void adapters_in_single(const HalfGemm& g, int row0, int col0, unsigned long long columns, f32x4 (&acc)[NI][NJ]) {
   using E = typename T::elem;
   const int l = threadIdx.x & 63;
   const int mine = l < NJ * 16 && col0 + l < g.n ? g.seg[col0 + l] : g.none;
-  unsigned long long left = __ballot(mine != g.none);
+  unsigned long long left = __ballot(mine != g.none) & columns;
   while (left) {
     const int who = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
-    const unsigned long long mask = __ballot(mine == who);
+    const unsigned long long mask = __ballot(mine == who) & columns;
     left &= ~mask;
     const float scale = g.scale[who];
     const E* factor = static_cast<const E*>(g.up) + (int64_t)who * g.up_stride;
@@ -310,23 +311,32 @@ __device__ __forceinline__ void adapters_in_single(const HalfGemm& g, int row0, 
 }
 
 // Into sums that are still zero.  A product of an infinity and a piece that is zero is a NaN, where the value's own product is an
-// infinity: where a NaN has come up it is all done again in single precision.
+// infinity: columns where a NaN has come up are done again in single precision (and only they: what a request gets does not depend on
+// what stands beside it).
 template <typename T, int NI, int NJ>
 __device__ __forceinline__ void add_adapters(const HalfGemm& g, int row0, int col0, f32x4 (&acc)[NI][NJ]) {
   adapters_in_pieces<T>(g, row0, col0, acc);
   if constexpr (T::bytes == 2) {
-    f32x4 all = {0.0f, 0.0f, 0.0f, 0.0f};
+    unsigned long long again = 0;
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+    for (int j = 0; j < NJ; ++j) {
+      f32x4 all = acc[0][j];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) all += acc[i][j];
-    const float sum = (all[0] + all[1]) + (all[2] + all[3]);
-    if (__builtin_expect(__any(sum != sum), 0)) {
+      for (int i = 1; i < NI; ++i) all += acc[i][j];
+      const float sum = (all[0] + all[1]) + (all[2] + all[3]);
+      unsigned long long nan = __ballot(sum != sum);
+      nan |= nan >> 32;
+      nan |= nan >> 16;
+      again |= (nan & 0xffff) << (j * 16);
+    }
+    if (__builtin_expect(again != 0, 0)) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      adapters_in_single<T>(g, row0, col0, acc);
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) acc[i][j][t] = (again >> (j * 16 + (threadIdx.x & 15))) & 1 ? 0.0f : acc[i][j][t];
+      adapters_in_single<T>(g, row0, col0, again, acc);
     }
   }
 }

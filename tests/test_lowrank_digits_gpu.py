@@ -187,3 +187,16 @@ def test_an_infinite_gradient_gives_an_infinity_of_the_right_sign(kind, opg, spr
     column = -torch.sign(c.u[:, 8]) * float("inf")       # rank 3: p of token 8 is -infinity, u of row 5 is 0 there
     assert torch.equal(torch.nan_to_num(got[rows, 3], nan=7.0, posinf=1.0, neginf=-1.0), torch.nan_to_num(column[rows], nan=7.0, posinf=1.0, neginf=-1.0))
     assert bool(torch.isfinite(got[rows][:, other]).all())
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("m, n, k, rank", [(256 * 15 + 8, 256 * 14 + 37, 72, 12), (1100, 1130, 72, 40), (1601, 130, 136, 100), (72, 40, 72, 9)])
+def test_what_a_request_gets_does_not_depend_on_infinities_beside_it(kind, m, n, k, rank):
+    c = Case(kind, m, n, k, rank, 5).run()
+    y, p = c.Y.as_strided().clone(), c.P.as_strided().clone()
+    c.B.matrix(1).as_strided()[2, 3] = float("inf")
+    c.A.matrix(3).as_strided()[5, 1] = float("nan")
+    c.run()
+    rest = ((c.ids != 1) & (c.ids != 3)).cuda()
+    assert torch.equal(c.Y.as_strided()[:, rest], y[:, rest]) and torch.equal(c.P.as_strided()[:, rest], p[:, rest])
+    assert not torch.equal(c.Y.as_strided(), y)
