@@ -197,7 +197,7 @@ template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArg
   hipError_t e = launch_pad_copy(w_copy, x_copy, s);
   if (e != hipSuccess) return e;
   if (lora_few(false, c.m, c.n, c.k)) return lora_few_device(c.kind, c.w_trans, g, q, s);
-  if (q.none > 0 && (e = launch_project<T>(q, s)) != hipSuccess) return e;
+  if (q.p && (e = launch_project<T>(q, s)) != hipSuccess) return e;
   const TilePlan plan = plan_tiles(c.m, c.n, c.k);
   g.splits = plan.splits;
   g.k_piece = (int)plan.k_piece;
@@ -530,7 +530,7 @@ hipError_t lora_device(const LoraArgs& c, hipStream_t s) {
   if (c.m > 0 && c.kind == BF16) return launch_half<Bf16>(c, p, s);
   if (c.m > 0 && c.kind == F16K) return launch_half<F16>(c, p, s);
   hipError_t e = hipSuccess;
-  if (p.none > 0) {
+  if (p.p) {
     e = c.kind == BF16 ? launch_project<Bf16>(p, s) : c.kind == F16K ? launch_project<F16>(p, s) : launch_project<Fp32>(p, s);
   }
   if (e != hipSuccess || c.m == 0) return e;

@@ -351,7 +351,7 @@ template <typename T> __global__ __launch_bounds__(512) void lora_token_kernel(H
     }
   }
   __syncthreads();
-  if (blockIdx.x == 0 && (int)threadIdx.x < g.rank) q.p[(int64_t)token * q.ldp + threadIdx.x] = ranks ? p[threadIdx.x] : 0.0f;
+  if (blockIdx.x == 0 && q.p && (int)threadIdx.x < q.rank) q.p[(int64_t)token * q.ldp + threadIdx.x] = ranks ? p[threadIdx.x] : 0.0f;
   if (!mine) return;
   float out = y[threadIdx.x];
   if (ranks) {
@@ -382,7 +382,7 @@ int few_pieces(int64_t m, int64_t n, int64_t k, int64_t project, int64_t* k_piec
   return (int)std::max<int64_t>((k + *k_piece - 1) / *k_piece, 1);
 }
 template <typename T, int LA, int NG> hipError_t launch_few_tokens(const HalfGemm& g, const ProjectArgs& q, hipStream_t s) {
-  const int form = project_form<T>(q), slots = q.none ? (int)project_slots(q) : 0, project = slots * ((q.rank + 15) / 16);
+  const int form = project_form<T>(q), slots = q.p ? (int)project_slots(q) : 0, project = slots * ((q.rank + 15) / 16);
   const dim3 grid((unsigned)(project + ((g.m + 63) / 64 * g.splits + 7) / 8 * 8 * ((g.n + 63) / 64)));
   if (form == A_K) hipLaunchKernelGGL((lora_few_kernel<T, LA, NG, A_K>), grid, dim3(512), 0, s, g, q, project, slots);
   if constexpr (T::bytes == 2) {
@@ -407,7 +407,7 @@ template <typename T, int LA> hipError_t launch_few(HalfGemm g, const ProjectArg
     }
   }
   int64_t piece;
-  g.splits = few_pieces(g.m, g.n, g.k, q.none ? project_slots(q) * ((q.rank + 15) / 16) : 0, &piece);
+  g.splits = few_pieces(g.m, g.n, g.k, q.p ? project_slots(q) * ((q.rank + 15) / 16) : 0, &piece);
   g.k_piece = (int)piece;
   return g.n <= 16 ? launch_few_tokens<T, LA, 1>(g, q, s) : g.n <= 32 ? launch_few_tokens<T, LA, 2>(g, q, s) : launch_few_tokens<T, LA, 4>(g, q, s);
 }

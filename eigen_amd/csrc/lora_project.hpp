@@ -13,7 +13,7 @@ struct ProjectArgs {
   const void* a; int64_t a_row, a_k, a_stride;    // strides of op(A_j)(r, k) and of j
   const int* order;
   const int* starts;
-  float* p; int64_t ldp;
+  float* p; int64_t ldp;                          // nullptr: no adapters, and nobody who wants the zeros
 };
 
 // 16 rows x 32 S positions on their way from memory to the matrix unit.  A fragment has neighbouring lanes on different rows; loaded

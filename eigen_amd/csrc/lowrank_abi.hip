@@ -83,9 +83,9 @@ int eigamd_lora_dev(int dtype, int opw, int opa, int opb, int64_t m, int64_t n, 
   if (n_adapters > 0) {
     if (!matrix_ok(d_a, at ? k : rank, at ? rank : k, lda, es) || !extent_ok(stride_a, kMaxStride)) return bad(me, "A: pointer, alignment, leading dimension or stride");
     if (!matrix_ok(d_b, bt ? rank : m, bt ? m : rank, ldb, es) || !extent_ok(stride_b, kMaxStride)) return bad(me, "B: pointer, alignment, leading dimension or stride");
-    if (!matrix_ok(d_p, rank, n, ldp, 4)) return bad(me, "P: pointer, alignment or leading dimension");
     if (!d_scale) return bad(me, "scale is null");
   }
+  if ((n_adapters > 0 || d_p) && !matrix_ok(d_p, rank, n, ldp, 4)) return bad(me, "P: pointer, alignment or leading dimension");
   if (n == 0 || (m == 0 && n_adapters == 0)) return EIGAMD_OK;
   if (!d_plan) return bad(me, "plan is null");
   if (m > 0 && k > 0 && (d_y == d_x || d_y == d_w)) return bad(me, "Y overlaps an input");

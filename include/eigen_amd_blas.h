@@ -420,8 +420,8 @@ int eigamd_trmm_dev(int dtype, int side, int uplo, int op, int diag, int64_t m, 
  *
  * X (k x n), Y (m x n) and P (rank x n) hold one token per column.  dtype (F32, BF16, F16) is that of W, X, A, B and Y; P and
  * the scales s are float; sums are kept in float and rounded once, into Y.  A token without an adapter gets op(W) x_i and a
- * zero column of P.  The factors lie `stride_a` / `stride_b` elements apart, adapter j at d_a + j * stride_a; op is N or T.
- * P is an output: the backward pass reads it.
+ * zero column of P (with n_adapters = 0 all of them; d_p may then be NULL, and with m = 0 besides nothing is done).  The factors
+ * lie `stride_a` / `stride_b` elements apart, adapter j at d_a + j * stride_a; op is N or T.  P is an output: the backward pass reads it.
  *
  * eigamd_lora_plan_dev prepares a batch: d_adapter_of[i] (device memory) is token i's adapter, anything outside
  * [0, n_adapters) means none; d_plan receives eigamd_lora_plan_ints(n, n_adapters) ints (tokens sorted by adapter).  The
