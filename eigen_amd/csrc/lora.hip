@@ -104,7 +104,8 @@ template <typename T, int RT> hipError_t launch_project_rank(const ProjectArgs& 
 // in proportion to their number beyond (rank 64, 3589 tokens: 16.2, 13.4, 15.5 us; 8192 tokens: 22.8, 23.9, 16.3; 142: 9.4, 12.8,
 // 14.2).
 template <typename T> hipError_t launch_project(const ProjectArgs& g, hipStream_t s) {
-  const double pieces = g.n / kProjTokens + (g.none + 1) * 0.5;      // an adapter's last piece is there or not
+  // (an adapter's last piece is there or not)
+  const double pieces = g.n / kProjTokens + (g.n <= g.none ? (double)g.n : (g.none + 1) * 0.5);
   auto cost = [&](int rt, double us) { return std::max(1.0, pieces * ((g.rank + 16 * rt - 1) / (16 * rt)) / 256.0) * us; };
   const double one = cost(1, 9.5), two = cost(2, 13.0), four = cost(4, 15.0);
   if (one <= two && one <= four) return launch_project_rank<T, 1>(g, s);
@@ -520,7 +521,7 @@ hipError_t lora_device(const LoraArgs& c, hipStream_t s) {
   p.a_row = c.a_trans ? c.lda : 1;
   p.a_k = c.a_trans ? 1 : c.lda;
   p.a_stride = c.stride_a;
-  p.order = c.plan.order; p.starts = c.plan.starts;
+  p.order = c.plan.order; p.seg = c.plan.seg; p.starts = c.plan.starts;
   p.p = c.p; p.ldp = c.ldp;
   if (c.m > 0 && c.kind == F32 && few_f32(c.w_trans, c.m, c.n, c.k)) {
     HalfGemm g = gemm_args(c);

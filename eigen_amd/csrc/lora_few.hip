@@ -420,6 +420,8 @@ template <typename T, int LA> hipError_t launch_few(HalfGemm g, const ProjectArg
 // 62.5 -> 69.2).  Single precision: against the library's product, which has larger tiles still, up to two rounds (777 x 1024 x
 // 1536 72.6 -> 45.9 us, 1500 x 1000 x 2000 114 -> 108, 2048 x 2048 x 2048 180 -> 214; W not transposed 439 x 384 x 2048 50 -> 24, 1024 x
 // 2048 x 2048 111 -> 118).
+// The projection counts with the workgroups that n tokens of one adapter take, however many there are: with many adapters the large
+// tiles lose more than it takes (100 x 4096 x 4096, 48 adapters of rank 128 67 -> 186 us, 200 x 2048 x 2048, rank 64 25 -> 53).
 bool lora_few(bool f32, int64_t m, int64_t n, int64_t k) {
   if (n <= 64) return true;
   const int64_t blocks = (m + 63) / 64 * ((n + 63) / 64), project = n / kProjTokens;

@@ -12,6 +12,7 @@ struct ProjectArgs {
   const void* x; int64_t ldx;
   const void* a; int64_t a_row, a_k, a_stride;    // strides of op(A_j)(r, k) and of j
   const int* order;
+  const int* seg;
   const int* starts;
   float* p; int64_t ldp;                          // nullptr: no adapters, and nobody who wants the zeros
 };
@@ -61,7 +62,7 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
   using E = typename T::elem;
   using x8 = typename T::x8;
   Piece piece;
-  if (!find_piece(g.starts, g.none + 1, kProjTokens, slot_id, piece)) return;
+  if (!(g.n <= g.none ? find_piece_by_tokens<kProjTokens>(g.seg, g.n, slot_id, piece) : find_piece(g.starts, g.none + 1, kProjTokens, slot_id, piece))) return;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x & 63;
   constexpr int line = RT * 32;                      // A_R: 32 positions x 16 RT ranks per wave
   f32x4(&red)[kProjWaves][RT][2][64] = *reinterpret_cast<f32x4(*)[kProjWaves][RT][2][64]>(lds);
@@ -204,7 +205,7 @@ template <typename T, int RT, int FORM> __device__ __forceinline__ void project_
   }
 }
 
-inline int64_t project_slots(const ProjectArgs& g) { return g.n / kProjTokens + g.none + 1; }
+inline int64_t project_slots(const ProjectArgs& g) { return g.n / kProjTokens + (g.n <= g.none ? g.n : g.none + 1); }
 template <typename T> int project_form(const ProjectArgs& g) {
   if (g.a_k == 1) return A_K;
   const bool chunks = g.a_row == 1 && g.a_k % 8 == 0 && g.rank % 8 == 0 && g.a_stride % 8 == 0 && (uintptr_t)g.a % 16 == 0;

@@ -1,10 +1,10 @@
-"""The adapter operators without adapters."""
+"""The adapter operators without adapters and with very many."""
 import pytest
 import torch
 
 from eigen_amd import _lib, lowrank
 from lowrank_ref import KINDS, NAME
-from test_lowrank_gpu import Case
+from test_lowrank_gpu import Case, Grad, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +33,33 @@ def test_without_adapters_there_may_be_no_p(kind, n):
                                   c.plan.storage.data_ptr(), 0, 1, c.Y.ptr, c.Y.ld, work.data_ptr(), work.numel(),
                                   torch.cuda.current_stream().cuda_stream)
     assert rc == _lib.OK and torch.equal(c.Y.storage, y)
+
+
+# ------------------------------------------------------------------------------------------------------------ many adapters
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("opw", "TN")
+@pytest.mark.parametrize("n, rank, count", [(2, 3, 65), (17, 64, 4096), (64, 20, 200), (130, 5, 65), (130, 40, 4096), (700, 20, 200), (700, 9, 4096)])
+def test_lora_with_many_adapters(kind, opw, n, rank, count):
+    c = Case(kind, 40, n, 72, rank, count, opw + "TT").run()
+    c.check()
+    # all tokens with the last ones, and none with any
+    for ids in ([count - 1 - i % 2 for i in range(n)], [-1] * n):
+        c.ids = torch.tensor(ids, dtype=torch.int32)
+        c.plan = lowrank.lora_plan(c.ids.cuda(), count)
+        c.run().check()
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("n, rank, count", [(17, 33, 4096), (64, 5, 200), (700, 16, 65), (1500, 5, 4096), (5000, 7, 129)])
+def test_lora_wgrad_with_many_adapters(kind, n, rank, count):
+    for opg, beta in (("N", 0.0), ("T", 1.0)):
+        c = Grad(kind, 40, n, rank, count, opg, beta).run()
+        c.check()
+        # a few long runs far apart among empty ones, in the order of their adapters and against it
+        for ids in ([(0, 63, 64, count - 1)[i * 4 // n] for i in range(n)], [count - 1 - i * 3 // (2 * n) for i in range(n)]):
+            c.ids = torch.tensor(ids, dtype=torch.int32)
+            c.plan = lowrank.lora_plan(c.ids.cuda(), count)
+            if beta:
+                for j in range(count):
+                    c.G.matrix(j).as_strided().copy_(turned(c.g0[j], opg))
+            c.run().check()
