@@ -43,30 +43,14 @@ struct Fp32 {
 };
 
 // A float as a sum of three bf16 values, each the leading 8 bits of what is left: they hold all 24 bits of any finite v.  They are cut,
-// not rounded (rounding up could leave the range).  An infinity or NaN stays in the first piece (a difference of infinities would be a
-// NaN).  Pieces may be zero, and an infinity times them is a NaN: who multiplies them looks for NaN and takes v itself then.
+// not rounded (rounding up could leave the range).  An infinity leaves NaN, and pieces may be zero, which an infinity on the other side
+// makes NaN: who multiplies them looks for NaN and takes v itself then.
 __device__ __forceinline__ float upper_half(float v) { return __int_as_float(__float_as_int(v) & 0xffff0000); }
 __device__ __forceinline__ void split_bf16(float v, __bf16 (&piece)[3]) {
-  const float first = upper_half(v), left = __builtin_fabsf(v) < __builtin_inff() ? v - first : 0.0f, second = upper_half(left);
+  const float first = upper_half(v), left = v - first, second = upper_half(left);
   piece[0] = (__bf16)first;
   piece[1] = (__bf16)second;
   piece[2] = (__bf16)(left - second);
-}
-
-// Eight f16 values as two bf16 ones each, 8 and 3 of their 11 bits (cut in f16, where the difference is exact; what the floats have in
-// their upper halves is all of them).
-__device__ __forceinline__ void split_f16_to_bf16(F16::x8 v, Bf16::x8 (&piece)[2]) {
-  using u16x8 = uint16_t __attribute__((ext_vector_type(8)));
-  using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
-  const F16::x8 high = __builtin_bit_cast(F16::x8, __builtin_bit_cast(u16x8, v) & (uint16_t)0xfff8);
-  const F16::x8 part[2] = {high, v - high};
-#pragma unroll
-  for (int z = 0; z < 2; ++z) {
-    u32x4 out;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) out[t] = __builtin_amdgcn_perm(__float_as_uint((float)part[z][2 * t + 1]), __float_as_uint((float)part[z][2 * t]), 0x07060302u);
-    piece[z] = __builtin_bit_cast(Bf16::x8, out);
-  }
 }
 
 // Power of two that brings the largest of |v| into [2^14, 2^15) (below it for what is smaller than 2^-112), and its inverse; 1 where that
@@ -81,13 +65,33 @@ __device__ __forceinline__ Norm norm_of(float largest) {
   return {__int_as_float((268 - e) << 23), __int_as_float((e - 14) << 23)};
 }
 
-// Three f16 values, 11 bits each, of a v below 2^15: they hold all of v from 1/2 on, where its last bit is a whole multiple of f16's
-// smallest number, 2^-24.
-__device__ __forceinline__ void split_f16(float v, _Float16 (&piece)[3]) {
+// A v below 2^15 as three f16 values in the same way, 11 bits each, the second and third of 2^UP times what the first leaves (UP at most
+// 10, as that is below 2^5).  They hold all of v from smallest_f16<UP>() on, where its last bit is a whole multiple of f16's smallest
+// number, 2^-24, over 2^UP.
+template <int UP> __device__ __forceinline__ void split_f16(float v, _Float16 (&piece)[3]) {
   piece[0] = (_Float16)__builtin_amdgcn_cvt_pkrtz(v, 0.0f)[0];
-  const float left = __builtin_fabsf(v) < __builtin_inff() ? v - (float)piece[0] : 0.0f;
+  const float left = (v - (float)piece[0]) * (float)(1 << UP);
   piece[1] = (_Float16)__builtin_amdgcn_cvt_pkrtz(left, 0.0f)[0];
   piece[2] = (_Float16)(left - (float)piece[1]);
+}
+template <int UP> constexpr float smallest_f16() { return 0.5f / (float)(1 << UP); }
+
+// Of 8 values: is one of them, other than zero, below `least` in magnitude?  (As whole numbers magnitudes keep their order, and zero, less
+// one, is above all of them.)
+template <typename V> __device__ __forceinline__ bool some_below(const V& v, float least) {
+  unsigned low = ~0u;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const unsigned b = (__float_as_uint(v[t]) & 0x7fffffff) - 1;
+    low = low < b ? low : b;
+  }
+  return low < __float_as_uint(least) - 1;
+}
+template <typename V> __device__ __forceinline__ float largest_of(const V& v) {
+  float top = 0.0f;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) top = fmaxf(top, __builtin_fabsf(v[t]));
+  return top;
 }
 
 // 2^(e - 127) for an exponent byte.  255 gives infinity: a block that held infinities or NaN is stored as zeros with
@@ -181,7 +185,7 @@ __device__ __forceinline__ bool find_piece(const int* starts, int segments, int 
 
 // The same where there are more adapters than tokens: slot t is the t-th place of the sorted batch where an adapter's tokens or a
 // multiple of SIZE begins; no more than n / SIZE + n slots, and n tokens to look at instead of all adapters (17 tokens x 2048 x 2048,
-// 4096 adapters of rank 64 577 -> 21 us).  (run_begin and run_end are not looked for.)
+// 4096 adapters of rank 64 577 -> 12 us).  (run_begin and run_end are not looked for.)
 template <int SIZE> __device__ __forceinline__ bool find_piece_by_tokens(const int* seg, int n, int t, Piece& out) {
   static_assert(64 % SIZE == 0, "a piece ends inside the 64 tokens it begins in");
   const int lane = threadIdx.x & 63;

@@ -166,19 +166,28 @@ template <typename T, int LAY, int R, int NT, bool GATHER> struct SliceLoader {
   }
 };
 
+// A bit for each of the 16 columns that a wave's lanes hold: one of the column's four lanes says so.
+__device__ __forceinline__ unsigned long long by_column(bool say) {
+  unsigned long long b = __ballot(say);
+  b |= b >> 32;
+  b |= b >> 16;
+  return b & 0xffff;
+}
+
 // Adds s_j up_j P to a wave's sums: column by column of the batch, only where the column belongs to j (an infinity or NaN in
 // one adapter's factor must not reach another request's column, so the products are selected, not multiplied by zero).
-// P goes through the matrix unit as three bf16 pieces per value, which hold all of its 32 bits.  An f16 factor becomes two bf16 pieces,
-// which hold all of its 11 bits: f16 has neither P's range nor room for the last pieces of a small one.
+// P goes through the matrix unit as three 16-bit pieces per value, which hold all of its 32 bits.  f16 has not P's range: there it is
+// normalised per token and 32 ranks, and the second and third piece are 2^10 times as large and summed up apart.  Columns with a P below
+// 2^-26 of that largest are left to adapters_in_single (`again`, a bit a column).
 // Per 32 ranks, P's fragments do not depend on the adapter; of the adapters' factors the next one's are under way while one is
 // multiplied.
 template <typename T, int NI, int NJ>
-__device__ __forceinline__ void adapters_in_pieces(const HalfGemm& g, int row0, int col0, f32x4 (&acc)[NI][NJ]) {
+__device__ __forceinline__ void adapters_in_pieces(const HalfGemm& g, int row0, int col0, f32x4 (&acc)[NI][NJ], unsigned long long& again) {
   using E = typename T::elem;
   using x8 = typename T::x8;
   using f32x8 = float __attribute__((ext_vector_type(8)));
-  using M = std::conditional_t<T::bytes == 4, Fp32, Bf16>;      // what the unit multiplies
-  constexpr int NP = T::bytes == 4 ? 1 : 3, NU = __is_same(T, F16) ? 2 : 1;
+  constexpr int NP = T::bytes == 4 ? 1 : 3, UP = 10;
+  constexpr bool APART = __is_same(T, F16);
   const int l = threadIdx.x & 63;
   const int col = col0 + l;
   const int mine = l < NJ * 16 && col < g.n ? g.seg[col] : g.none;
@@ -208,19 +217,34 @@ __device__ __forceinline__ void adapters_in_pieces(const HalfGemm& g, int row0, 
       for (int t = 0; t < 8; ++t) u[t] = rn > 0 ? u[t] : (E)0.0f;
       return u;
     };
-    typename M::x8 part[NP][NJ];
+    x8 part[NP][NJ];
+    float back[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const float* at = g.p + (int64_t)token[j] * g.ldp + r;
-      const f32x8 v = chunks ? load_8<float, f32x8>(at) : load_first<float, f32x8>(at, 1, rn);
+      f32x8 v = chunks ? load_8<float, f32x8>(at) : load_first<float, f32x8>(at, 1, rn);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] = rn > 0 ? v[t] : 0.0f;
+      back[j] = scale[j];
+      if constexpr (APART) {
+        // (one that is infinite leaves nothing finite in its column)
+        float top = largest_of(v);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const Norm nm = norm_of(top);
+        back[j] *= nm.up;
+        again |= by_column(some_below(v, smallest_f16<UP>() * nm.up)) << (j * 16);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) v[t] *= nm.down;
+      }
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
-        const float p = rn > 0 ? v[t] : 0.0f;
         if constexpr (NP == 1) {
-          part[0][j][t] = p;
+          part[0][j][t] = v[t];
         } else {
-          __bf16 piece[NP];
-          split_bf16(p, piece);
+          E piece[NP];
+          if constexpr (APART) split_f16<UP>(v[t], piece);
+          else split_bf16(v[t], piece);
 #pragma unroll
           for (int z = 0; z < NP; ++z) part[z][j][t] = piece[z];
         }
@@ -250,20 +274,18 @@ __device__ __forceinline__ void adapters_in_pieces(const HalfGemm& g, int row0, 
         }
 #pragma unroll
         for (int i = 0; i < GI; ++i) {
-          typename M::x8 f[NU];
-          if constexpr (NU == 1) f[0] = u[i];
-          else split_f16_to_bf16(u[i], f);
 #pragma unroll
           for (int j = 0; j < NJ; ++j) {
             if (!((mask >> (j * 16)) & 0xffff)) continue;
             f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int z = NP - 1; z >= 0; --z)
-#pragma unroll
-              for (int y = NU - 1; y >= 0; --y) d = M::mma(f[y], part[z][j], d);
+            for (int z = NP - 1; z >= 0; --z) {
+              if (APART && z == 0) d *= 1.0f / (float)(1 << UP);
+              d = T::mma(u[i], part[z][j], d);
+            }
             const bool on = (mask >> (j * 16 + (l & 15))) & 1;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) acc[i0 + i][j][t] += on ? d[t] * scale[j] : 0.0f;
+            for (int t = 0; t < 4; ++t) acc[i0 + i][j][t] += on ? d[t] * back[j] : 0.0f;
           }
           if (AHEAD && more) u[i] = factor(next, i);
         }
@@ -311,23 +333,20 @@ __device__ __forceinline__ void adapters_in_single(const HalfGemm& g, int row0, 
 }
 
 // Into sums that are still zero.  A product of an infinity and a piece that is zero is a NaN, where the value's own product is an
-// infinity: columns where a NaN has come up are done again in single precision (and only they: what a request gets does not depend on
-// what stands beside it).
+// infinity: columns where a NaN has come up are done again in single precision, like those that the pieces do not hold (and only they:
+// what a request gets does not depend on what stands beside it).
 template <typename T, int NI, int NJ>
 __device__ __forceinline__ void add_adapters(const HalfGemm& g, int row0, int col0, f32x4 (&acc)[NI][NJ]) {
-  adapters_in_pieces<T>(g, row0, col0, acc);
+  unsigned long long again = 0;
+  adapters_in_pieces<T>(g, row0, col0, acc, again);
   if constexpr (T::bytes == 2) {
-    unsigned long long again = 0;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       f32x4 all = acc[0][j];
 #pragma unroll
       for (int i = 1; i < NI; ++i) all += acc[i][j];
       const float sum = (all[0] + all[1]) + (all[2] + all[3]);
-      unsigned long long nan = __ballot(sum != sum);
-      nan |= nan >> 32;
-      nan |= nan >> 16;
-      again |= (nan & 0xffff) << (j * 16);
+      again |= by_column(sum != sum) << (j * 16);
     }
     if (__builtin_expect(again != 0, 0)) {
 #pragma unroll

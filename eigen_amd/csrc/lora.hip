@@ -357,22 +357,20 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
       return sum;
     };
     if constexpr (__is_same(T, F16)) {
-      float top = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = __builtin_fabsf(pv[e]) < __builtin_inff() ? fmaxf(top, __builtin_fabsf(pv[e])) : top;
+      float top = largest_of(pv);      // (one that is infinite leaves nothing finite in its rank)
       top = fmaxf(top, __shfl_xor(top, 16));      // (lanes l, l + 16, ... hold the same rank)
       top = fmaxf(top, __shfl_xor(top, 32));
       const Norm nm = norm_of(top);
-      bool small = false;
+      float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float v = pv[e] * nm.down;
-        small |= pv[e] != 0.0f && __builtin_fabsf(v) < 0.5f;
+        v[e] = pv[e] * nm.down;
         E q[NP];
-        split_f16(v, q);
+        split_f16<0>(v[e], q);
 #pragma unroll
         for (int z = 0; z < NP; ++z) fp[z][e] = q[z];
       }
+      const bool small = some_below(v, smallest_f16<0>());
       if (__builtin_expect(__any(small), 0)) {
         Fp32::x8 p;
 #pragma unroll
