@@ -159,7 +159,7 @@ __device__ __forceinline__ uint64_t load_bytes(const int8_t* p, int n) {
 // j plus j's pieces, so slots are unique without a prefix sum, and there are at most n / size + adapters + 1 of them.
 // One wave finds j by counting bases <= t, four loads under way together.  Returns false for a slot that no piece has.
 struct Piece {
-  int adapter, begin, end, run_begin, run_end;
+  int adapter, index, begin, end, run_begin, run_end;      // index: of the run's pieces
 };
 __device__ __forceinline__ bool find_piece(const int* starts, int segments, int size, int t, Piece& out) {
   const int lane = threadIdx.x & 63;
@@ -178,14 +178,15 @@ __device__ __forceinline__ bool find_piece(const int* starts, int segments, int 
   out.adapter = j;
   out.run_begin = starts[j];
   out.run_end = starts[j + 1];
-  out.begin = out.run_begin + (t - (out.run_begin / size + j)) * size;
+  out.index = t - (out.run_begin / size + j);
+  out.begin = out.run_begin + out.index * size;
   out.end = out.begin + size < out.run_end ? out.begin + size : out.run_end;
   return out.begin < out.run_end;
 }
 
 // The same where there are more adapters than tokens: slot t is the t-th place of the sorted batch where an adapter's tokens or a
 // multiple of SIZE begins; no more than n / SIZE + n slots, and n tokens to look at instead of all adapters (17 tokens x 2048 x 2048,
-// 4096 adapters of rank 64 577 -> 12 us).  (run_begin and run_end are not looked for.)
+// 4096 adapters of rank 64 577 -> 12 us).  (index, run_begin and run_end are not looked for.)
 template <int SIZE> __device__ __forceinline__ bool find_piece_by_tokens(const int* seg, int n, int t, Piece& out) {
   static_assert(64 % SIZE == 0, "a piece ends inside the 64 tokens it begins in");
   const int lane = threadIdx.x & 63;

@@ -213,7 +213,7 @@ enum { DIRECT, STAGED, QUANT };    // u: global -> LDS by hardware / through reg
 
 struct GradArgs {
   int rows, rank, n, none, chunk, slots;
-  bool trans;
+  bool trans, halves;
   const void* u; int64_t ldu;
   const uint8_t* exponents; int64_t lde;
   const float* p; int64_t ldp;
@@ -438,7 +438,7 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
   }
   const bool whole = piece.run_end - piece.run_begin <= g.chunk;
   const float sj = whole ? g.scale[piece.adapter] : 1.0f;
-  float* out = whole ? g.g + (int64_t)piece.adapter * g.stride_g : g.partial + (int64_t)blockIdx.y * g.rows * g.rank;
+  float* out = whole ? g.g + (int64_t)piece.adapter * g.stride_g : g.partial + (int64_t)(g.halves ? 2 * piece.run_begin / g.chunk + piece.index : (int)blockIdx.y) * g.rows * g.rank;
   const int64_t ld = whole ? g.ldg : (TRANS ? g.rank : g.rows);
   const float beta = whole ? g.beta : 0.0f;
   const int limit = TRANS ? g.rank : g.rows;
@@ -462,10 +462,13 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
 }
 
 // G_j = beta G_j + s_j (sum of j's pieces, in the order of the batch).
+// Where the sums of a run's first piece stand, of those that a run of several pieces leaves to the join.  begin / chunk + j keeps them apart
+// (find_piece), with room for every adapter; so does 2 begin / chunk (`halves`), as a run of more than `chunk` tokens has no more pieces
+// than half chunks, with room for the tokens: whichever is less.
 __global__ __launch_bounds__(256) void lora_grad_join_kernel(GradArgs g) {
   const int j = blockIdx.y, begin = g.starts[j], count = g.starts[j + 1] - begin;
   if (count <= g.chunk) return;
-  const int pieces = (count + g.chunk - 1) / g.chunk, slot = begin / g.chunk + j;
+  const int pieces = (count + g.chunk - 1) / g.chunk, slot = (g.halves ? 2 * begin : begin) / g.chunk + (g.halves ? 0 : j);
   const int64_t size = (int64_t)g.rows * g.rank;
   const int fast = g.trans ? g.rank : g.rows;
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < size; q += (int64_t)gridDim.x * 256) {
@@ -551,13 +554,14 @@ hipError_t lora_device(const LoraArgs& c, hipStream_t s) {
 
 int64_t lora_grad_work_bytes(int64_t rows, int64_t n, int64_t rank, int64_t adapters) {
   const int chunk = grad_chunk(std::max<int64_t>(rows, 1), n);
-  return n > chunk ? (n / chunk + adapters + 1) * rows * rank * 4 : 0;
+  return n > chunk ? std::min(2 * n / chunk, n / chunk + adapters + 1) * rows * rank * 4 : 0;
 }
 
 hipError_t lora_grad_device(const LoraGradArgs& c, hipStream_t s) {
   GradArgs g;
   g.rows = (int)c.rows; g.rank = (int)c.rank; g.n = (int)c.n; g.none = c.plan.adapters;
   g.chunk = grad_chunk(c.rows, c.n);
+  g.halves = 2 * c.n / g.chunk < c.n / g.chunk + g.none + 1;
   g.trans = c.trans;
   g.u = c.u; g.ldu = c.ldu; g.exponents = c.exponents; g.lde = c.lde;
   g.p = c.p; g.ldp = c.ldp; g.scale = c.scale;

@@ -63,3 +63,11 @@ def test_lora_wgrad_with_many_adapters(kind, n, rank, count):
                 for j in range(count):
                     c.G.matrix(j).as_strided().copy_(turned(c.g0[j], opg))
             c.run().check()
+
+
+@pytest.mark.parametrize("opg", "NT")
+@pytest.mark.parametrize("count", [61, 4096])
+def test_lora_wgrad_of_runs_just_longer_than_a_piece(opg, count):
+    """Pieces are 128 tokens here: runs of one token more, twice as many and one, one less, one by one behind each other."""
+    ids = [j for j, length in enumerate([129, 257, 129, 128, 385, 1, 127, 129, 130, 255, 256, 257] * 5) for _ in range(length)]
+    Grad(_lib.BF16, 40, len(ids), 5, count, opg, ids=ids).run().check()
