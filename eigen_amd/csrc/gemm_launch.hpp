@@ -377,6 +377,7 @@ static void describe_plan(const GemmCall& c, const char* variable, int* out) {
   if (out[0]) describe_whole<SMALL>(c, out);
   else describe_whole<LARGE>(c, out);
 }
+double modelled_gemm_f32(int64_t m, int64_t n, int64_t k);   // microseconds of the form that launch_gemm_f32 takes
 void describe_gemm_f32(const GemmCall&, int*);
 void describe_gemm_f64(const GemmCall&, int*);
 void describe_gemm_c32(const GemmCall&, int*);

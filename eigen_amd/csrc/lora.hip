@@ -16,7 +16,8 @@
 namespace eigamd {
 
 // lora_few.hip
-bool lora_few(bool f32, int64_t m, int64_t n, int64_t k);
+bool lora_few_half(int64_t m, int64_t n, int64_t k);
+bool lora_few_f32(bool w_trans, int64_t m, int64_t n, int64_t k);
 int64_t lora_few_work_bytes(int64_t m, int64_t n, int64_t k);
 hipError_t lora_few_device(int kind, bool w_trans, const HalfGemm& g, const ProjectArgs& q, hipStream_t s);
 
@@ -145,7 +146,7 @@ struct HalfWork {
 HalfWork half_work(bool w_trans, int64_t m, int64_t n, int64_t k, const void* w, int64_t ldw, const void* x, int64_t ldx) {
   HalfWork need = {0, 0, 0};
   const bool w_whole = whole_chunks(w, ldw, w_trans ? k : m);
-  if (lora_few(false, m, n, k)) {
+  if (lora_few_half(m, n, k)) {
     need.sums = lora_few_work_bytes(m, n, k);      // (read where they are, whatever their alignment; chunks of 8 rows have to exist)
     if (!w_trans && m < 8) need.w_copy = padded_bytes(m, k);
   } else {
@@ -177,7 +178,7 @@ HalfGemm gemm_args(const LoraArgs& c) {
   return g;
 }
 // The few-token form in single precision; where W is not transposed, chunks of 4 rows have to exist.
-bool few_f32(bool w_trans, int64_t m, int64_t n, int64_t k) { return (w_trans || m >= 4) && lora_few(true, m, n, k); }
+bool few_f32(bool w_trans, int64_t m, int64_t n, int64_t k) { return (w_trans || m >= 4) && lora_few_f32(w_trans, m, n, k); }
 
 template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArgs& q, hipStream_t s) {
   HalfGemm g = gemm_args(c);
@@ -197,7 +198,7 @@ template <typename T> hipError_t launch_half(const LoraArgs& c, const ProjectArg
   }
   hipError_t e = launch_pad_copy(w_copy, x_copy, s);
   if (e != hipSuccess) return e;
-  if (lora_few(false, c.m, c.n, c.k)) return lora_few_device(c.kind, c.w_trans, g, q, s);
+  if (lora_few_half(c.m, c.n, c.k)) return lora_few_device(c.kind, c.w_trans, g, q, s);
   if (q.p && (e = launch_project<T>(q, s)) != hipSuccess) return e;
   const TilePlan plan = plan_tiles(c.m, c.n, c.k);
   g.splits = plan.splits;

@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cstdint>
 
+#include "gemm_launch.hpp"
 #include "half_gemm.hpp"
 #include "lora_project.hpp"
 #include "lowrank.hpp"
@@ -417,19 +418,32 @@ template <typename T, int LA> hipError_t launch_few(HalfGemm g, const ProjectArg
 // Up to 64 tokens, and beyond as long as this is one round and quicker than large tiles with the projection in front of them: 3 us,
 // and 5 + 4.4 per thousand positions a round, against the plan's time, 6 us and 1.25 per thousand positions for the projection
 // (256 tokens x 1024 x 1024 18.7 -> 10.4 us, 142 x 2456 x 4032 29.6 -> 17.9, 192 x 4096 x 4096 31.5 -> 25.1; not 96 x 4096 x 16384,
-// 62.5 -> 69.2).  Single precision: against the library's product, which has larger tiles still, up to two rounds (777 x 1024 x
-// 1536 72.6 -> 45.9 us, 1500 x 1000 x 2000 114 -> 108, 2048 x 2048 x 2048 180 -> 214; W not transposed 439 x 384 x 2048 50 -> 24, 1024 x
-// 2048 x 2048 111 -> 118).
+// 62.5 -> 69.2).
 // The projection counts with the workgroups that n tokens of one adapter take, however many there are: with many adapters the large
 // tiles lose more than it takes (100 x 4096 x 4096, 48 adapters of rank 128 67 -> 186 us, 200 x 2048 x 2048, rank 64 25 -> 53).
-bool lora_few(bool f32, int64_t m, int64_t n, int64_t k) {
+bool lora_few_half(int64_t m, int64_t n, int64_t k) {
   if (n <= 64) return true;
   const int64_t blocks = (m + 63) / 64 * ((n + 63) / 64), project = n / kProjTokens;
-  if (f32) return blocks <= 512;
   if (blocks + project > 256) return false;
   int64_t piece;
   const int64_t pieces = few_pieces(m, n, k, project, &piece), rounds = (blocks * pieces + project + 255) / 256;
   return 3.0 + (double)rounds * (5.0 + 4.4e-3 * (double)piece) < plan_tiles(m, n, k).us + 6.0 + 1.25e-3 * (double)k;
+}
+// Single precision, against the library's product with the projection and the low-rank part around it.  Measured: 19 us, 19.5 per
+// thousand positions a round where W's reduction is contiguous and 21.8 where its rows are (4 % more in a single round), and the
+// projection's workgroups in front, 0.06 per thousand positions each; the product takes 1.02 times its model, 1.27 where tiles are not
+// whole, 8 us and 2 per thousand positions around it (777 tokens x 1024 x 1536 72 -> 46 us, 2000 x 1000 x 2048 132 -> 111; not 768 x 2048 x
+// 2048, 93 and 109).  Within 3 % it is this one.  More tokens bring more of the projection than of W (8192 x 128 x 2048 80 and 126).
+bool lora_few_f32(bool w_trans, int64_t m, int64_t n, int64_t k) {
+  const int64_t blocks = (m + 63) / 64 * ((n + 63) / 64), project = n / kProjTokens;
+  if (n <= 64) return true;
+  if (blocks > (n > 2048 ? 256 : 512) || n > 5120) return false;
+  int64_t piece;
+  const int64_t pieces = few_pieces(m, n, k, project, &piece);
+  const double rounds = blocks * pieces <= 256 ? 1.04 : pieces > 1 ? (double)(blocks * pieces) / 256.0 : 2.0;
+  const double us = 19.0 + rounds * (w_trans ? 19.5e-3 : 21.8e-3) * (double)piece + 6e-5 * (double)(project * k);
+  const bool whole = m % 128 == 0 && n % 128 == 0;
+  return us < 1.03 * (modelled_gemm_f32(m, n, k) * (whole ? 1.02 : 1.27) + 8.0 + 2e-3 * (double)k);
 }
 int64_t lora_few_work_bytes(int64_t m, int64_t n, int64_t k) {
   int64_t pieces = 1;
