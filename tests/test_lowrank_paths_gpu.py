@@ -1,12 +1,14 @@
-"""The adapter operators without adapters and with very many."""
+"""The adapter operators without adapters and with very many, and wide projections."""
 import pytest
 import torch
 
+import eigen_amd
 from eigen_amd import _lib, lowrank
 from lowrank_ref import KINDS, NAME
 from test_lowrank_gpu import Case, Grad, turned
 
 pytestmark = pytest.mark.gpu
+F32, BF16, F16 = eigen_amd.F32, eigen_amd.BF16, eigen_amd.F16
 
 
 # ------------------------------------------------------------------------------------------------------------- no adapters
@@ -71,3 +73,19 @@ def test_lora_wgrad_of_runs_just_longer_than_a_piece(opg, count):
     """Pieces are 128 tokens here: runs of one token more, twice as many and one, one less, one by one behind each other."""
     ids = [j for j, length in enumerate([129, 257, 129, 128, 385, 1, 127, 129, 130, 255, 256, 257] * 5) for _ in range(length)]
     Grad(_lib.BF16, 40, len(ids), 5, count, opg, ids=ids).run().check()
+
+
+# --------------------------------------------------------------------------------------------------------- wide projections
+# With this many tokens the projection takes 32 ranks a workgroup (4100 tokens: rank 33, 40, 64) or 64 (8200 tokens, and rank 100 and
+# 128), and the call is larger than the few-token form takes.
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("ops", ["TTT", "TNN"])
+@pytest.mark.parametrize("n, rank, k", [(4100, 33, 72), (4100, 40, 200), (4100, 64, 1288), (8200, 40, 83), (8200, 64, 264), (4100, 100, 136), (4100, 128, 603)])
+def test_wide_projections(kind, ops, n, rank, k):
+    Case(kind, 520 if kind == F32 and n < 8000 else 264, n, k, rank, 3, ops).run().check()
+
+
+@pytest.mark.parametrize("kind", [BF16, F16], ids=NAME.get)
+@pytest.mark.parametrize("ops", ["TTT", "NNN"])
+def test_large_tiles_with_several_turns_of_ranks(kind, ops):
+    Case(kind, 256 * 15 + 8, 256 * 14 + 37, 200, 100, 6, ops).run().check()
