@@ -1,4 +1,5 @@
-"""The adapter operators without adapters and with very many, and wide projections."""
+"""The adapter operators on paths that small shapes do not reach: no adapters, very many, wide projections, large calls in single
+precision."""
 import pytest
 import torch
 
@@ -89,3 +90,40 @@ def test_wide_projections(kind, ops, n, rank, k):
 @pytest.mark.parametrize("ops", ["TTT", "NNN"])
 def test_large_tiles_with_several_turns_of_ranks(kind, ops):
     Case(kind, 256 * 15 + 8, 256 * 14 + 37, 200, 100, 6, ops).run().check()
+
+
+# ------------------------------------------------------------------------------------------------ large single precision calls
+@pytest.mark.parametrize("ops", ["TTT", "NNN"])
+@pytest.mark.parametrize("m, n, k, rank, count, pad", [(2051, 1100, 72, 7, 3, 0), (1030, 2047, 136, 40, 5, 3), (2048, 1024 + 64, 2056, 16, 2, 0), (2050, 1090, 1003, 16, 9, 1)])
+def test_large_calls_in_single_precision(ops, m, n, k, rank, count, pad):
+    """More than 512 blocks of 64 x 64: the library's product, and the low-rank part behind it."""
+    Case(F32, m, n, k, rank, count, ops, pad=pad).run().check()
+
+
+def test_large_single_precision_calls_repeat_in_graphs_and_on_streams():
+    cases = [Case(F32, 2051, 1100, 264, 7, 3, "TTT", seed=s) for s in (1, 50)]
+    want = []
+    for c in cases:
+        c.run().check()
+        want.append((c.Y.storage.clone(), c.P.storage.clone()))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for c, s in zip(cases, streams):
+            c.run(stream=s)
+    torch.cuda.synchronize()
+    for c, (y, p) in zip(cases, want):
+        assert torch.equal(c.Y.storage, y) and torch.equal(c.P.storage, p)
+    c, (y, p) = cases[0], want[0]
+    work = torch.empty(lowrank.lora_work_bytes("T", c.W, c.X), dtype=torch.uint8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.run(work=work)
+    for _ in range(3):
+        c.Y.as_strided().zero_()
+        c.P.as_strided().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(c.Y.storage, y) and torch.equal(c.P.storage, p)
+        c.run(work=work)
+        torch.cuda.synchronize()
