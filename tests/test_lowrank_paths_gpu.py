@@ -1,12 +1,12 @@
 """The adapter operators on paths that small shapes do not reach: no adapters, very many, wide projections, large calls in single
-precision."""
+precision, and what lies around the gradients' matrices."""
 import pytest
 import torch
 
 import eigen_amd
 from eigen_amd import _lib, lowrank
 from lowrank_ref import KINDS, NAME
-from test_lowrank_gpu import Case, Grad, turned
+from test_lowrank_gpu import MARK, Case, Grad, turned
 
 pytestmark = pytest.mark.gpu
 F32, BF16, F16 = eigen_amd.F32, eigen_amd.BF16, eigen_amd.F16
@@ -127,3 +127,19 @@ def test_large_single_precision_calls_repeat_in_graphs_and_on_streams():
         assert torch.equal(c.Y.storage, y) and torch.equal(c.P.storage, p)
         c.run(work=work)
         torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------------------------------- around the gradients
+@pytest.mark.parametrize("kind", KINDS, ids=NAME.get)
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("opg", "NT")
+@pytest.mark.parametrize("rows, n, rank", [(1, 3, 1), (264, 70, 16), (261, 140, 7), (130, 1300, 33), (300, 90, 130)])
+def test_lora_wgrad_writes_its_matrices_only(kind, packed, opg, rows, n, rank):
+    """Rows below, columns behind and the gaps between neighbouring adapters' matrices: one with several pieces, one with one, one empty."""
+    for beta, pad in ((0.0, 1), (0.5, 4)):
+        c = Grad(kind, rows, n, rank, 4, opg, beta, pad, 0, packed, ids=[(0, 1, 1, 1, -1, 3)[i * 6 // n] for i in range(n)]).run()
+        c.check()
+        inside = torch.zeros(c.G.storage.numel(), dtype=torch.bool, device="cuda")
+        for j in range(c.count):
+            torch.as_strided(inside, (c.G.rows, c.G.cols), (1, c.G.ld), j * c.G.stride).fill_(True)
+        assert bool((c.G.storage[~inside] == MARK).all())
