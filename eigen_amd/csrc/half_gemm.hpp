@@ -44,15 +44,14 @@ static __device__ __align__(64) unsigned char zero_page[64];
 
 // Global memory to LDS without passing through registers: lane l's 16 bytes land at `to` + 16 l (`to` the same in every lane).
 // In assembly, because the compiler would wait for every such load before the next read of any LDS; it is waited for, with
-// everything else, in slice_barrier().  M0 holds the LDS address; nothing else in these kernels uses it.  The second form takes
-// a base that is the same in every lane.
+// everything else, in slice_barrier().  M0 holds the LDS address.  The second form takes a base that is the same in every lane.
 __device__ __forceinline__ void load_to_lds(const char* from, char* to) {
   const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)EIGAMD_LDS(char, to));
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(at), "v"(from) : "memory");
 }
 __device__ __forceinline__ void load_to_lds(const char* base, unsigned off, char* to) {
   const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)EIGAMD_LDS(char, to));
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(base) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(at), "v"(off), "s"(base) : "memory");
 }
 // This wave's LDS accesses and all but its newest KEEP loads are done, then those of the workgroup.
 template <int KEEP> __device__ __forceinline__ void slice_barrier() {
