@@ -15,6 +15,14 @@ _KIND_OF_TORCH = {v: k for k, v in _TORCH_OF_KIND.items()}
 _OPCODE = {"N": _lib.OP_N, "T": _lib.OP_T, "C": _lib.OP_C, "J": _lib.OP_CONJ}
 
 
+def _np_of(*kinds):
+    """The numpy type of the first of these kinds; the dense entries take none of the 16-bit ones."""
+    for kind in kinds:
+        if kind not in _NP_OF_KIND:
+            raise ValueError("the kind must be F32, F64, C32 or C64 (16-bit matrices: eigen_amd.lowrank)")
+    return _NP_OF_KIND[kinds[0]]
+
+
 def _stream_ptr(stream=None):
     s = torch.cuda.current_stream() if stream is None else stream
     return ctypes.c_void_p(s.cuda_stream)
@@ -60,6 +68,8 @@ class DeviceMatrix:
         return torch.as_strided(self.storage, (self.rows, self.cols), (1, self.ld), self.offset)
 
     def to_numpy(self):
+        if self.kind == _lib.BF16:
+            raise ValueError("numpy has no bf16: as_strided() is the matrix as a torch tensor")
         return np.asfortranarray(self.as_strided().cpu().numpy())
 
     @classmethod
@@ -80,7 +90,7 @@ def gemm_dev(opa, opb, alpha, a, b, beta, c, stream=None, noalloc=False):
     oa, ob = _OPCODE[opa], _OPCODE[opb]
     m, n = c.rows, c.cols
     k = a.cols if oa in (_lib.OP_N, _lib.OP_CONJ) else a.rows
-    dt = _NP_OF_KIND[c.kind]
+    dt = _np_of(c.kind)
     al, be = np.array([alpha], dtype=dt), np.array([beta], dtype=dt)
     fn = lib.eigamd_gemm_dev_noalloc if noalloc else lib.eigamd_gemm_dev
     rc = fn(c.kind, oa, ob, m, n, k, ctypes.c_void_p(al.ctypes.data), ctypes.c_void_p(a.ptr), a.ld,
@@ -97,7 +107,7 @@ def gemm_mixed_dev(opa, opb, alpha, a, b, beta, c, stream=None):
     oa, ob = _OPCODE[opa], _OPCODE[opb]
     m, n = c.rows, c.cols
     k = a.cols if oa in (_lib.OP_N, _lib.OP_CONJ) else a.rows
-    dt = _NP_OF_KIND[c.kind]
+    dt = _np_of(c.kind, a.kind, b.kind)
     al, be = np.array([alpha], dtype=dt), np.array([beta], dtype=dt)
     rc = lib.eigamd_gemm_mixed_dev(c.kind, a_real, b_real, oa, ob, m, n, k, ctypes.c_void_p(al.ctypes.data),
                                    ctypes.c_void_p(a.ptr), a.ld, ctypes.c_void_p(b.ptr), b.ld,
@@ -111,7 +121,7 @@ def trsm_dev(side, uplo, transa, diag, alpha, a, b, stream=None):
     x overwriting b; asynchronous on ``stream`` (``eigamd_trsm_dev``)."""
     if a.kind != b.kind:
         raise ValueError("operands must share one scalar kind")
-    al = np.array([alpha], dtype=_NP_OF_KIND[b.kind])
+    al = np.array([alpha], dtype=_np_of(b.kind))
     rc = lib.eigamd_trsm_dev(b.kind, "LR".index(side.upper()), "UL".index(uplo.upper()), _OPCODE[transa.upper()],
                              "NU".index(diag.upper()), b.rows, b.cols, ctypes.c_void_p(al.ctypes.data),
                              ctypes.c_void_p(a.ptr), a.ld, ctypes.c_void_p(b.ptr), b.ld, _stream_ptr(stream))
@@ -124,7 +134,7 @@ def syrk_dev(uplo, trans, alpha, a, beta, c, stream=None):
     the uplo triangle of the square DeviceMatrix c (``eigamd_syrk_dev``)."""
     if a.kind != c.kind:
         raise ValueError("operands must share one scalar kind")
-    dt = _NP_OF_KIND[c.kind]
+    dt = _np_of(c.kind)
     al, be = np.array([alpha], dtype=dt), np.array([beta], dtype=dt)
     k = a.cols if trans.upper() == "N" else a.rows
     rc = lib.eigamd_syrk_dev(c.kind, "UL".index(uplo.upper()), _OPCODE[trans.upper()], c.rows, k,
@@ -139,6 +149,7 @@ def herk_dev(uplo, trans, alpha, a, beta, c, stream=None):
     uplo triangle of the square complex DeviceMatrix c; alpha and beta real (``eigamd_herk_dev``)."""
     if a.kind != c.kind:
         raise ValueError("operands must share one scalar kind")
+    _np_of(c.kind)
     rdt = np.float32 if c.kind == _lib.C32 else np.float64
     al, be = np.array([alpha], dtype=rdt), np.array([beta], dtype=rdt)
     k = a.cols if trans.upper() == "N" else a.rows
@@ -152,7 +163,7 @@ def herk_dev(uplo, trans, alpha, a, beta, c, stream=None):
 def syr2k_dev(uplo, trans, alpha, a, b, beta, c, hermitian=False, stream=None):
     """c <- alpha * op(a) * op(b)^T + alpha * op(b) * op(a)^T + beta * c on the uplo triangle of c, or
     the Hermitian form (^H, conj(alpha) in the second term, beta real) (``eigamd_syr2k_dev``)."""
-    dt = _NP_OF_KIND[c.kind]
+    dt = _np_of(c.kind, a.kind, b.kind)
     al, be = np.array([alpha], dtype=dt), np.array([beta], dtype=dt)
     k = a.cols if trans.upper() == "N" else a.rows
     rc = lib.eigamd_syr2k_dev(c.kind, "UL".index(uplo.upper()), _OPCODE[trans.upper()], int(bool(hermitian)), c.rows, k,
@@ -165,7 +176,7 @@ def syr2k_dev(uplo, trans, alpha, a, b, beta, c, hermitian=False, stream=None):
 def symm_dev(side, uplo, alpha, a, b, beta, c, hermitian=False, stream=None):
     """c <- alpha * a * b + beta * c (side 'L') or alpha * b * a + beta * c (side 'R'), a symmetric
     (Hermitian if asked) and read through its uplo triangle only (``eigamd_symm_dev``)."""
-    dt = _NP_OF_KIND[c.kind]
+    dt = _np_of(c.kind, a.kind, b.kind)
     al, be = np.array([alpha], dtype=dt), np.array([beta], dtype=dt)
     rc = lib.eigamd_symm_dev(c.kind, "LR".index(side.upper()), "UL".index(uplo.upper()), int(bool(hermitian)), c.rows,
                              c.cols, ctypes.c_void_p(al.ctypes.data), ctypes.c_void_p(a.ptr), a.ld, ctypes.c_void_p(b.ptr),
@@ -177,7 +188,7 @@ def symm_dev(side, uplo, alpha, a, b, beta, c, hermitian=False, stream=None):
 def trmm_dev(side, uplo, transa, diag, alpha, a, b, stream=None):
     """b <- alpha * op(a) * b (side 'L') or alpha * b * op(a) (side 'R'), a triangular
     (``eigamd_trmm_dev``)."""
-    al = np.array([alpha], dtype=_NP_OF_KIND[b.kind])
+    al = np.array([alpha], dtype=_np_of(b.kind, a.kind))
     rc = lib.eigamd_trmm_dev(b.kind, "LR".index(side.upper()), "UL".index(uplo.upper()), _OPCODE[transa.upper()],
                              "NU".index(diag.upper()), b.rows, b.cols, ctypes.c_void_p(al.ctypes.data),
                              ctypes.c_void_p(a.ptr), a.ld, ctypes.c_void_p(b.ptr), b.ld, _stream_ptr(stream))

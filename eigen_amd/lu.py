@@ -102,7 +102,8 @@ def laswp_dev(a, transp, k0, k1, stream=None):
 
 def trsm_llnu_dev(l, b, stream=None):
     """b <- l^-1 b with `l` the unit lower triangle of a square DeviceMatrix block."""
-    from .device import _stream_ptr
+    from .device import _np_of, _stream_ptr
+    _np_of(b.kind, l.kind)
     rc = lib.eigamd_trsm_llnu_dev(b.kind, b.rows, b.cols, ctypes.c_void_p(l.ptr), l.ld, ctypes.c_void_p(b.ptr), b.ld,
                                   _stream_ptr(stream))
     _lib.check(rc, "eigamd_trsm_llnu_dev")
@@ -127,7 +128,8 @@ def getrs(trans, lu, ipiv, b):
 def getrs_dev(op, lu, transp, b, stream=None):
     """op(A) X = B on DeviceMatrix operands: `lu` and `transp` (int32 device tensor, 0-based) as getrf_dev
     leaves them; X overwrites `b`.  Asynchronous on `stream`."""
-    from .device import _stream_ptr
+    from .device import _np_of, _stream_ptr
+    _np_of(lu.kind, b.kind)
     rc = lib.eigamd_getrs_dev(lu.kind, op, lu.rows, b.cols, ctypes.c_void_p(lu.ptr), lu.ld, ctypes.c_void_p(transp.data_ptr()),
                               ctypes.c_void_p(b.ptr), b.ld, _stream_ptr(stream))
     _lib.check(rc, "eigamd_getrs_dev")
