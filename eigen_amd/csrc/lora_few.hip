@@ -17,7 +17,7 @@ template <typename E, int N> using Part = E __attribute__((ext_vector_type(N)));
 
 // Y for few tokens, 16 NG of them a workgroup: the time is that of reading W, from as many compute units as there are.  A
 // workgroup owns 64 rows and one piece of the reduction, so that X, which every workgroup reads its piece of, costs little beside
-// W (with 16 rows and the whole reduction X was four times the traffic: 64 tokens x 4096 x 4096 took 22 us, now 12).  Its eight
+// W (with 16 rows and the whole reduction X was four times the traffic: 64 tokens x 4096 x 4096 took 22 us, now 13).  Its eight
 // waves share the piece, 64 (32) positions a turn, turned in the wave's own LDS (W's reduction contiguous: as a RowBlock; its rows: read
 // back transposed, single precision one element at a time).  The sums go to memory in 32 bits; the second kernel adds the
 // pieces up and the low-rank part to them.
@@ -371,7 +371,7 @@ bool piece_allowed(int64_t blocks, int64_t k, int64_t pieces) {
 }
 // A compute unit runs one of these workgroups at a time, so the 64-row blocks times the pieces and the projection's workgroups
 // should fill whole rounds of 256; a round costs what its piece does plus the latencies at both ends, about as much as 600
-// positions (64 tokens x 4096 x 4096: 16.8 us, with pieces for 512 at a time 21.1).
+// positions (64 tokens x 4096 x 4096: 13.2 us, the call 17.5; with pieces for 512 at a time 16.8 and 21.9).
 int few_pieces(int64_t m, int64_t n, int64_t k, int64_t project, int64_t* k_piece) {
   const int64_t blocks = (m + 63) / 64 * ((n + 63) / 64);
   int64_t best = 1, best_cost = INT64_MAX;
