@@ -177,7 +177,7 @@ __device__ __forceinline__ unsigned long long by_column(bool say) {
 // one adapter's factor must not reach another request's column, so the products are selected, not multiplied by zero).
 // P goes through the matrix unit as three 16-bit pieces per value, which hold all of its 32 bits.  f16 has not P's range: there it is
 // normalised per token and 32 ranks, and the second and third piece are 2^10 times as large and summed up apart.  Columns with a P below
-// 2^-26 of that largest are left to adapters_in_single (`again`, a bit a column).
+// about 2^-26 of that largest are left to adapters_in_single (`again`, a bit a column).
 // Per 32 ranks, P's fragments do not depend on the adapter; of the adapters' factors the next one's are under way while one is
 // multiplied.
 template <typename T, int NI, int NJ>

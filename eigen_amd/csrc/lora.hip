@@ -293,7 +293,7 @@ template <typename T, int SRC> struct GradTile {
 // G_j over one piece of j's tokens: 256 rows x 16 RT ranks per workgroup, 32 tokens a turn.  p keeps all of its 32 bits, as three 16-bit
 // pieces; the sums are the matrix unit's 32 bits.  A run that is one piece goes straight to G_j.
 // f16 has neither p's range nor room for three pieces of what is far below the largest: a turn's p is normalised rank by rank, and a wave
-// that holds a p below 2^-16 of its rank's largest (one turn in fifty of normally distributed p) takes that turn's products in single
+// that holds a p below about 2^-16 of its rank's largest (one turn in fifty of normally distributed p) takes that turn's products in single
 // precision, six times the work.
 // The product of an infinity and a piece of p that is zero is a NaN, where that with p is an infinity: where a NaN has come up, a wave's
 // sums are made again in single precision, from memory as it is.

@@ -200,3 +200,36 @@ def test_what_a_request_gets_does_not_depend_on_infinities_beside_it(kind, m, n,
     rest = ((c.ids != 1) & (c.ids != 3)).cuda()
     assert torch.equal(c.Y.as_strided()[:, rest], y[:, rest]) and torch.equal(c.P.as_strided()[:, rest], p[:, rest])
     assert not torch.equal(c.Y.as_strided(), y)
+
+
+# ------------------------------------------------------------------------- where f16's pieces end and single precision begins
+@pytest.mark.parametrize("kind", [BF16, F16], ids=NAME.get)
+@pytest.mark.parametrize("m, n, rank", [(1100, 1130, 16), (1601, 130, 100)])
+@pytest.mark.parametrize("spread", [10, 20, 23, 24, 25, 26, 27])
+def test_quiet_ranks_at_every_distance_reach_y(kind, m, n, rank, spread):
+    c = Case(kind, m, n, 72, rank, 2, "TTT")
+    quiet = (torch.arange(rank) % 5 > 0).double()
+    c.a = (rand(c.a.shape, kind, 41) * 2.0 ** (12.0 - spread * quiet).unsqueeze(1)).to(TORCH[kind]).double()
+    c.b = c.b * quiet
+    c.w = torch.zeros_like(c.w)
+    c.scale = torch.tensor([2.0 ** (spread - 18), -2.0 ** (spread - 17)])
+    c.S = c.scale.cuda()
+    c.W, c.A, c.B = store(turned(c.w, "T"), kind), store_stack(turned(c.a, "T"), kind), store_stack(turned(c.b, "T"), kind)
+    c.run()
+    y, p, ya, pa = ref.lora(*[t.cuda() for t in (c.w, c.x, c.a, c.b)], c.scale.double().cuda(), c.ids.cuda())
+    tol = ref.HALF[kind] * y.abs() + (2 * c.k + rank + 32) * 2.0 ** -23 * ya * (1 + ref.HALF[kind]) + ref.SMALL[kind]
+    err = (c.Y.as_strided().double() - y).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
+
+
+@pytest.mark.parametrize("kind", [BF16, F16], ids=NAME.get)
+@pytest.mark.parametrize("opg", "NT")
+@pytest.mark.parametrize("spread", [8, 13, 14, 15, 16, 17, 18, 25])
+def test_quiet_tokens_at_every_distance_keep_their_digits(kind, opg, spread):
+    """Every second token's p is 2^-spread times the others', and rows of u in which only these tokens are not zero."""
+    c = Grad(kind, 80, 200, 20, 1, opg, ids=[0] * 200)
+    quiet = torch.arange(200) % 2 == 1
+    c.p = torch.where(quiet, c.p * 2.0 ** -spread, c.p).float().double()
+    c.u = torch.where((torch.arange(80) % 2 == 0).unsqueeze(1) | quiet, c.u, torch.zeros(()).double())
+    c.P, c.U = store(c.p, F32), store(c.u, kind)
+    c.run().check()
