@@ -439,7 +439,8 @@ template <typename T, int SRC, int RT, bool TRANS> __global__ __launch_bounds__(
   }
   const bool whole = piece.run_end - piece.run_begin <= g.chunk;
   const float sj = whole ? g.scale[piece.adapter] : 1.0f;
-  float* out = whole ? g.g + (int64_t)piece.adapter * g.stride_g : g.partial + (int64_t)(g.halves ? 2 * piece.run_begin / g.chunk + piece.index : (int)blockIdx.y) * g.rows * g.rank;
+  const int slot = g.halves ? 2 * piece.run_begin / g.chunk + piece.index : (int)blockIdx.y;      // (lora_grad_join_kernel)
+  float* out = whole ? g.g + (int64_t)piece.adapter * g.stride_g : g.partial + (int64_t)slot * g.rows * g.rank;
   const int64_t ld = whole ? g.ldg : (TRANS ? g.rank : g.rows);
   const float beta = whole ? g.beta : 0.0f;
   const int limit = TRANS ? g.rank : g.rows;
